@@ -519,6 +519,85 @@ int soinfer_decode_layers_fused(const soinfer_fused_layer* layers, int64_t num_l
 int soinfer_quantize_pack_int4(const void* w, int32_t dtype, int64_t N, int64_t K, int64_t ld,
                                int64_t group_size, uint8_t* packed, float* scale, void* stream);
 
+/* ---- Paged KV cache and prompt attention (no reference counterpart: the
+ * reference keeps one contiguous fp16 cache and runs a prompt token by token,
+ * python/soinfer/runtime/generate.py:429-463).
+ *
+ * A pool holds num_pages pages of page_size positions (a power of two >= 16)
+ * for num_kv_heads heads of head_dim (64 or 128) values; row b of block_table
+ * (int32, table_cols entries, row stride table_stride) names the pages of
+ * sequence b: position p lies in page block_table[b][p / page_size], slot
+ * p % page_size.  Entries outside [0, num_pages) name no page.
+ *   bits 16: k_pages / v_pages fp16 [num_pages, num_kv_heads, page_size, head_dim].
+ *   bits 4:  k_pages bytes [num_pages, num_kv_heads, page_size * (head_dim/2 + head_dim/16)]: per (page, head)
+ *            page_size * head_dim/2 bytes of codes, then page_size * head_dim/32 fp16 scales (one per 32 values);
+ *            word t * (head_dim/32) + j of a position (t < 4) holds values 32 j + 8 t + (0..7), value 2 i in nibble i,
+ *            2 i + 1 in nibble i + 4.
+ *            v_pages bytes [num_pages, num_kv_heads, page_size * (head_dim/2 + 2)]: codes, then page_size fp16 scales
+ *            (one per position); positions 2 m and 2 m + 1 share head_dim/4 words, word w holds values 4 w + (0..3), the
+ *            even position's in nibbles 0..3, the odd one's in nibbles 4..7.
+ *            scale = fp16(max(amax / 7, 2^-14)), code = clamp(rint(x / scale), -7, 7) (two's complement), value =
+ *            code * scale.  A group that holds an infinity or a NaN, or whose scale exceeds fp16, reads as NaN. */
+typedef struct soinfer_paged_cache {
+  void* k_pages;
+  void* v_pages;
+  const int32_t* block_table;
+  int64_t table_stride, table_cols, num_pages, num_kv_heads, page_size, head_dim, bits;
+} soinfer_paged_cache;
+
+/* Rows of packed tokens: [tokens, heads, head_dim] fp16, strides in elements
+ * (multiples of 8), 16-byte aligned. */
+typedef struct soinfer_rows {
+  const soinfer_half* data;
+  int64_t token_stride, head_stride;
+} soinfer_rows;
+
+/* Token j of sequence b (packed rows cu_seqlens[b] ..; NULL: one token per
+ * sequence) stands at position start[b] + j: per-head RMSNorm of q and k
+ * (q_norm / k_norm fp16 [head_dim], NULL: none), rotate-half RoPE with that row
+ * of cos_table / sin_table (fp32 [table_rows, head_dim/2]), then k and v stored
+ * at that position.  q_out [tokens, num_q_heads, head_dim] and k_out (may be
+ * NULL) receive the rotated rows; one rounding at the end.  num_q_heads may be
+ * 0.  A token of no sequence or beyond the tables: zeros, nothing stored; a
+ * position without a page: rotated, not stored.  No two tokens of a call may
+ * name the same place.  cu_seqlens, start and the block table are read on the
+ * device (capturable). */
+int soinfer_paged_kv_append(const soinfer_paged_cache* cache, const soinfer_rows* q, const soinfer_rows* k,
+                            const soinfer_rows* v, soinfer_half* q_out, soinfer_half* k_out, int64_t tokens,
+                            int64_t num_q_heads, int64_t num_seqs, const int32_t* cu_seqlens, const int32_t* start,
+                            const float* cos_table, const float* sin_table, int64_t table_rows,
+                            const soinfer_half* q_norm, const soinfer_half* k_norm, float eps, void* stream);
+
+/* Positions 0 .. of every sequence b as packed fp16 rows cu_seqlens[b] ..
+ * cu_seqlens[b + 1] of k_out / v_out [tokens, num_kv_heads, head_dim] (4-bit
+ * rows as the values they stand for; a position without a page: zeros; rows of
+ * no sequence: left as they were). */
+int soinfer_paged_kv_read(const soinfer_paged_cache* cache, const int32_t* cu_seqlens, int64_t num_seqs, int64_t tokens,
+                          soinfer_half* k_out, soinfer_half* v_out, void* stream);
+
+/* One query per sequence over its first seq_lens[b] cached positions (at most
+ * table_cols * page_size; read on the device), grouped heads, scale
+ * 1/sqrt(head_dim), fp32 softmax and sums: out [num_seqs, num_q_heads,
+ * head_dim].  Positions without a page are skipped; a sequence without
+ * positions gives zeros.  num_seqs <= 32768. */
+int64_t soinfer_paged_decode_workspace_bytes(int64_t num_seqs, int64_t num_q_heads, int64_t num_kv_heads,
+                                             int64_t head_dim);
+int soinfer_paged_decode_attention(const soinfer_paged_cache* cache, const soinfer_rows* q, soinfer_half* out,
+                                   int64_t num_seqs, int64_t num_q_heads, const int32_t* seq_lens, void* workspace,
+                                   int64_t workspace_bytes, void* stream);
+
+/* Causal attention of packed prompts: sequence b's queries are rows
+ * cu_seqlens_q[b] .. cu_seqlens_q[b + 1] of q, its keys and values rows
+ * cu_seqlens_k[b] .. of k / v; query i of Lq sees keys j <= i + Lk - Lq (the
+ * last query sees every key).  Grouped heads, scale 1/sqrt(head_dim), fp32
+ * softmax and sums.  out [tokens_q, num_q_heads, head_dim]; a query without
+ * keys gives zeros, rows of no sequence are left as they were.  Row bounds
+ * are read on the device and clamped to the given token counts. */
+int soinfer_prefill_attention(const soinfer_rows* q, const soinfer_rows* k, const soinfer_rows* v, soinfer_half* out,
+                              int64_t tokens_q, int64_t tokens_k, int64_t num_seqs, const int32_t* cu_seqlens_q,
+                              const int32_t* cu_seqlens_k, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                              void* stream);
+
 /* ---- Tensor-parallel exchange over peer memory (no reference counterpart:
  * the reference runs on one GPU; this is the row-parallel all-reduce, the
  * all-gather and the greedy-token agreement of tensor-parallel decode across

@@ -917,6 +917,169 @@ int soinfer_quantize_pack_int4(const void* w, int32_t dtype, int64_t N, int64_t 
                      name);
 }
 
+// ---------------------------------------------------------------- paged KV cache
+
+namespace {
+int to_paged_cache(const char* name, const soinfer_paged_cache* in, PagedCache& c) {
+  REQUIRE(in, "%s: null cache", name);
+  REQUIRE(in->head_dim == 64 || in->head_dim == 128, "%s: head_dim must be 64 or 128", name);
+  REQUIRE(in->page_size >= 16 && in->page_size <= (1 << 16) && (in->page_size & (in->page_size - 1)) == 0,
+          "%s: page_size must be a power of two in [16, 65536]", name);
+  REQUIRE(in->bits == 16 || in->bits == 4, "%s: bits must be 16 or 4", name);
+  REQUIRE(in->num_kv_heads >= 1 && in->num_kv_heads <= 1024, "%s: num_kv_heads must be in [1, 1024]", name);
+  REQUIRE(in->num_pages >= 0 && in->num_pages < (1ll << 31) && in->table_cols >= 0 && in->table_cols < (1ll << 31) &&
+              in->table_stride >= in->table_cols,
+          "%s: invalid num_pages / table_cols / table_stride", name);
+  REQUIRE(in->num_pages == 0 || (in->k_pages && in->v_pages), "%s: null pages", name);
+  REQUIRE(in->table_cols == 0 || in->block_table, "%s: null block_table", name);
+  REQUIRE(aligned(in->k_pages, 16) && aligned(in->v_pages, 16) && aligned(in->block_table, 4),
+          "%s: pages must be 16-byte aligned, block_table 4-byte aligned", name);
+  c.k = static_cast<uint8_t*>(in->k_pages);
+  c.v = static_cast<uint8_t*>(in->v_pages);
+  c.table = in->block_table;
+  c.table_stride = in->table_stride;
+  c.table_cols = (int)in->table_cols;
+  c.num_pages = (int)in->num_pages;
+  c.nkv = (int)in->num_kv_heads;
+  c.page_shift = 0;
+  while ((1ll << c.page_shift) < in->page_size) ++c.page_shift;
+  c.hd = (int)in->head_dim;
+  c.q4 = in->bits == 4;
+  return SOINFER_OK;
+}
+
+int check_rows(const char* name, const char* what, const soinfer_rows* r) {
+  REQUIRE(r && r->data, "%s: null %s", name, what);
+  REQUIRE(aligned(r->data, 16) && r->token_stride >= 0 && r->head_stride >= 0 && r->token_stride % 8 == 0 &&
+              r->head_stride % 8 == 0,
+          "%s: %s must be 16-byte aligned with non-negative strides that are multiples of 8 elements", name, what);
+  return SOINFER_OK;
+}
+}  // namespace
+
+int soinfer_paged_kv_append(const soinfer_paged_cache* cache, const soinfer_rows* q, const soinfer_rows* k,
+                            const soinfer_rows* v, soinfer_half* q_out, soinfer_half* k_out, int64_t tokens,
+                            int64_t num_q_heads, int64_t num_seqs, const int32_t* cu_seqlens, const int32_t* start,
+                            const float* cos_table, const float* sin_table, int64_t table_rows,
+                            const soinfer_half* q_norm, const soinfer_half* k_norm, float eps, void* stream) {
+  const char* name = "paged_kv_append";
+  PagedAppendParams P{};
+  if (int st = to_paged_cache(name, cache, P.cache)) return st;
+  REQUIRE(tokens >= 0 && tokens < (1ll << 31) && num_seqs >= 0 && num_seqs < (1ll << 31), "%s: invalid tokens / num_seqs",
+          name);
+  REQUIRE(num_q_heads >= 0 && num_q_heads <= 1024, "%s: num_q_heads must be in [0, 1024]", name);
+  REQUIRE(table_rows >= 1 && table_rows < (1ll << 31), "%s: table_rows must be >= 1", name);
+  REQUIRE(eps >= 0.f, "%s: eps must be >= 0", name);
+  if (tokens == 0) return SOINFER_OK;
+  if (num_q_heads > 0) {
+    if (int st = check_rows(name, "q", q)) return st;
+    REQUIRE(q_out && aligned(q_out, 16), "%s: q_out null or not 16-byte aligned", name);
+    P.q = as_half(q->data), P.q_token = q->token_stride, P.q_head = q->head_stride;
+  }
+  if (int st = check_rows(name, "k", k)) return st;
+  if (int st = check_rows(name, "v", v)) return st;
+  REQUIRE(aligned(k_out, 16), "%s: k_out must be 16-byte aligned", name);
+  REQUIRE((num_seqs == 0 || start) && cos_table && sin_table, "%s: null start / cos_table / sin_table", name);
+  REQUIRE(aligned(cos_table, 16) && aligned(sin_table, 16) && aligned(q_norm, 16) && aligned(k_norm, 16),
+          "%s: tables and norm weights must be 16-byte aligned", name);
+  P.k = as_half(k->data), P.k_token = k->token_stride, P.k_head = k->head_stride;
+  P.v = as_half(v->data), P.v_token = v->token_stride, P.v_head = v->head_stride;
+  P.q_out = as_half(q_out);
+  P.k_out = as_half(k_out);
+  P.tokens = (int)tokens;
+  P.nq = (int)num_q_heads;
+  P.nkv = P.cache.nkv;
+  P.seqs = (int)num_seqs;
+  P.cu = cu_seqlens;
+  P.start = start;
+  P.cos_t = cos_table;
+  P.sin_t = sin_table;
+  P.table_rows = table_rows;
+  P.q_norm = as_half(q_norm);
+  P.k_norm = as_half(k_norm);
+  P.eps = eps;
+  return cuda_result(launch_paged_append(P, as_stream(stream)), name);
+}
+
+int soinfer_paged_kv_read(const soinfer_paged_cache* cache, const int32_t* cu_seqlens, int64_t num_seqs, int64_t tokens,
+                          soinfer_half* k_out, soinfer_half* v_out, void* stream) {
+  const char* name = "paged_kv_read";
+  PagedCache C{};
+  if (int st = to_paged_cache(name, cache, C)) return st;
+  REQUIRE(tokens >= 0 && tokens < (1ll << 31) && num_seqs >= 0 && num_seqs < (1ll << 31), "%s: invalid tokens / num_seqs",
+          name);
+  if (tokens == 0 || num_seqs == 0) return SOINFER_OK;
+  REQUIRE(cu_seqlens && k_out && v_out, "%s: null pointer", name);
+  REQUIRE(aligned(k_out, 16) && aligned(v_out, 16), "%s: outputs must be 16-byte aligned", name);
+  return cuda_result(
+      launch_paged_read(C, cu_seqlens, (int)num_seqs, (int)tokens, as_half(k_out), as_half(v_out), as_stream(stream)),
+      name);
+}
+
+int64_t soinfer_paged_decode_workspace_bytes(int64_t num_seqs, int64_t num_q_heads, int64_t num_kv_heads,
+                                             int64_t head_dim) {
+  if (num_seqs < 1 || num_q_heads < 1 || num_kv_heads < 1 || head_dim < 1 || num_q_heads % num_kv_heads) return 0;
+  return paged_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim);
+}
+
+int soinfer_paged_decode_attention(const soinfer_paged_cache* cache, const soinfer_rows* q, soinfer_half* out,
+                                   int64_t num_seqs, int64_t num_q_heads, const int32_t* seq_lens, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
+  const char* name = "paged_decode_attention";
+  PagedDecodeParams P{};
+  if (int st = to_paged_cache(name, cache, P.cache)) return st;
+  REQUIRE(num_seqs >= 0 && num_seqs <= 32768, "%s: num_seqs must be in [0, 32768]", name);
+  REQUIRE(num_q_heads >= 1 && num_q_heads <= 1024 && num_q_heads % P.cache.nkv == 0,
+          "%s: num_q_heads must be a multiple of num_kv_heads, at most 1024", name);
+  if (num_seqs == 0) return SOINFER_OK;
+  if (int st = check_rows(name, "q", q)) return st;
+  REQUIRE(out && seq_lens, "%s: null pointer", name);
+  REQUIRE(workspace && aligned(workspace, 16) &&
+              workspace_bytes >= paged_decode_workspace_bytes(num_seqs, num_q_heads, P.cache.nkv, P.cache.hd),
+          "%s: workspace too small or not 16-byte aligned", name);
+  P.q = as_half(q->data), P.q_token = q->token_stride, P.q_head = q->head_stride;
+  P.out = as_half(out);
+  P.seqs = (int)num_seqs;
+  P.nq = (int)num_q_heads;
+  P.lens = seq_lens;
+  P.ws = static_cast<float*>(workspace);
+  return cuda_result(launch_paged_decode(P, as_stream(stream)), name);
+}
+
+int soinfer_prefill_attention(const soinfer_rows* q, const soinfer_rows* k, const soinfer_rows* v, soinfer_half* out,
+                              int64_t tokens_q, int64_t tokens_k, int64_t num_seqs, const int32_t* cu_seqlens_q,
+                              const int32_t* cu_seqlens_k, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                              void* stream) {
+  const char* name = "prefill_attention";
+  REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128", name);
+  REQUIRE(num_kv_heads >= 1 && num_q_heads >= 1 && num_q_heads <= 1024 && num_q_heads % num_kv_heads == 0,
+          "%s: num_q_heads must be a multiple of num_kv_heads, at most 1024", name);
+  REQUIRE(tokens_q >= 0 && tokens_q <= (1ll << 30) && tokens_k >= 0 && tokens_k <= (1ll << 30) && num_seqs >= 0 &&
+              num_seqs <= (1 << 20),
+          "%s: invalid tokens / num_seqs", name);
+  if (tokens_q == 0 || num_seqs == 0) return SOINFER_OK;
+  if (int st = check_rows(name, "q", q)) return st;
+  PrefillParams P{};
+  if (tokens_k > 0) {
+    if (int st = check_rows(name, "k", k)) return st;
+    if (int st = check_rows(name, "v", v)) return st;
+    P.k = as_half(k->data), P.k_token = k->token_stride, P.k_head = k->head_stride;
+    P.v = as_half(v->data), P.v_token = v->token_stride, P.v_head = v->head_stride;
+  }
+  REQUIRE(out && aligned(out, 16) && cu_seqlens_q && cu_seqlens_k, "%s: null pointer or misaligned out", name);
+  P.q = as_half(q->data), P.q_token = q->token_stride, P.q_head = q->head_stride;
+  P.out = as_half(out);
+  P.tokens_q = (int)tokens_q;
+  P.tokens_k = (int)tokens_k;
+  P.seqs = (int)num_seqs;
+  P.nq = (int)num_q_heads;
+  P.nkv = (int)num_kv_heads;
+  P.hd = (int)head_dim;
+  P.cu_q = cu_seqlens_q;
+  P.cu_k = cu_seqlens_k;
+  return cuda_result(launch_prefill_attention(P, as_stream(stream)), name);
+}
+
 // ---------------------------------------------------------------- tensor-parallel exchange
 
 static_assert(sizeof(cudaIpcMemHandle_t) == SOINFER_IPC_HANDLE_BYTES, "IPC handle size");

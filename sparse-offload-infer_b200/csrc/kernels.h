@@ -296,4 +296,53 @@ bool plan_decode_fused(FusedDecodeParams& P, void* workspace, int64_t workspace_
 cudaError_t launch_decode_fused(const FusedDecodeParams& P, int sms, cudaStream_t stream);
 cudaError_t read_and_clear_decode_fused_error(int* out);
 
+// Paged KV cache (paged_kv.cu, paged_attention.cu): pools of pages, block tables, fp16 or 4-bit rows (layout in
+// paged_cache.cuh).  head_dim 64 or 128, page size a power of two >= 16.
+struct PagedCache {
+  uint8_t* k;            // [num_pages, nkv] blocks
+  uint8_t* v;
+  const int32_t* table;  // [seqs, table_cols] page ids, row stride table_stride
+  int64_t table_stride;
+  int table_cols, num_pages, nkv, page_shift, hd;
+  bool q4;
+};
+struct PagedAppendParams {
+  PagedCache cache;
+  const half *q, *k, *v;  // strides in elements
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  half* q_out;            // [tokens, nq, hd]
+  half* k_out;            // [tokens, nkv, hd] or null
+  int tokens, nq, nkv, seqs;
+  const int32_t* cu;      // [seqs + 1], or null: one token per sequence
+  const int32_t* start;   // [seqs] positions already cached
+  const float *cos_t, *sin_t;
+  int64_t table_rows;
+  const half *q_norm, *k_norm;
+  float eps;
+};
+cudaError_t launch_paged_append(const PagedAppendParams& P, cudaStream_t stream);
+cudaError_t launch_paged_read(const PagedCache& C, const int32_t* cu, int seqs, int tokens, half* k_out, half* v_out,
+                              cudaStream_t stream);
+struct PagedDecodeParams {
+  PagedCache cache;
+  const half* q;
+  int64_t q_token, q_head;
+  half* out;              // [seqs, nq, hd]
+  int seqs, nq;
+  const int32_t* lens;    // [seqs]
+  float* ws;              // partial results of split sequences
+};
+int64_t paged_decode_workspace_bytes(int64_t seqs, int64_t nq, int64_t nkv, int64_t hd);
+cudaError_t launch_paged_decode(const PagedDecodeParams& P, cudaStream_t stream);
+
+// Causal attention of packed prompts (prefill_attention.cu).
+struct PrefillParams {
+  const half *q, *k, *v;  // strides in elements
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  half* out;              // [tokens_q, nq, hd]
+  int tokens_q, tokens_k, seqs, nq, nkv, hd;
+  const int32_t *cu_q, *cu_k;
+};
+cudaError_t launch_prefill_attention(const PrefillParams& P, cudaStream_t stream);
+
 }  // namespace soinfer

@@ -1,0 +1,73 @@
+// Pages of a KV cache: addressing and the 4-bit row format shared by the append, read and decode kernels.
+//
+// A (page, kv head) pair owns one block of K bytes and one of V bytes.
+//   fp16:   [page][hd] halves each.
+//   4 bits: K = page * hd/2 bytes of codes, then page * hd/32 fp16 scales (one per 32 values);
+//           V = page * hd/2 bytes of codes, then page fp16 scales (one per position).
+// Codes are two's-complement nibbles in [-7, 7] and a value is code * scale.  The words are ordered for the matrix
+// instruction that reads them, so that a lane's share of a tile is one contiguous piece:
+//   K: word t * (hd/32) + j of a position holds values 32 j + 8 t + (0..7), value 2 i in nibble i and 2 i + 1 in nibble
+//      i + 4 (masking one nibble of each 16-bit half gives two consecutive values).  Lane t of a quad reads words
+//      t * (hd/32) ..: 16 bytes at hd = 128, every pair of matrix steps inside one scale group.
+//   V: positions 2 m and 2 m + 1 share hd/4 words; word w holds values 4 w + (0..3), the even position's in the low half
+//      and the odd one's in the high half (masking gives one value at two positions, the product's reduction axis).  Each
+//      position owns whole 16-bit units, so rows are appended without reading what is there.
+// A scale is fp16(max(amax / 7, 2^-14)) and the code is chosen against the rounded scale.  A row (K: group) that holds
+// an infinity or a NaN gets code 0 and a non-finite scale: it reads as NaN throughout.
+#pragma once
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace soinfer {
+
+constexpr int kKGroup = 32;                 // values of a key that share a scale
+constexpr float kMinScale = 6.103515625e-5f;  // 2^-14, the smallest normal fp16
+
+__host__ __device__ __forceinline__ int64_t k_block_bytes(int page, int hd, bool q4) {
+  return q4 ? (int64_t)page * (hd / 2 + hd / 16) : (int64_t)page * hd * 2;
+}
+__host__ __device__ __forceinline__ int64_t v_block_bytes(int page, int hd, bool q4) {
+  return q4 ? (int64_t)page * (hd / 2 + 2) : (int64_t)page * hd * 2;
+}
+
+// Pool page of position pos (>= 0) of sequence b, or -1 when the table or the pool does not hold it.
+__device__ __forceinline__ int page_of(const PagedCache& c, int b, int pos) {
+  const int col = pos >> c.page_shift;
+  if (col >= c.table_cols) return -1;
+  const int id = __ldg(c.table + (int64_t)b * c.table_stride + col);
+  return (id >= 0 && id < c.num_pages) ? id : -1;
+}
+
+// Sequence that owns packed row t: how many of cu[1..n] are <= t (all lanes get it; n = no sequence owns the row).
+__device__ __forceinline__ int owner_of(const int32_t* cu, int n, int t, int lane) {
+  int b = 0;
+  for (int base = 0; base < n; base += 32) {
+    const int i = base + lane;
+    const unsigned m = __ballot_sync(0xffffffffu, i < n && __ldg(cu + i + 1) <= t);
+    b += __popc(m);
+    if (m != 0xffffffffu) break;
+  }
+  return b;
+}
+
+// fp16 scale of a group with largest magnitude amax (NaN and infinity stay what they are).
+__device__ __forceinline__ half scale_of(float amax) {
+  const float s = __fdiv_rn(amax, 7.f);
+  return __float2half_rn(s < kMinScale ? kMinScale : s);
+}
+
+// Code of x against the fp16 scale s: clamp(rint(x / s), -7, 7), 0 where the quotient is NaN.
+__device__ __forceinline__ int code_of(float x, float s) {
+  const float r = rintf(__fdiv_rn(x, s));
+  return r != r ? 0 : (int)fminf(fmaxf(r, -7.f), 7.f);
+}
+
+// The larger magnitude, NaN if either is NaN.
+__device__ __forceinline__ float amax_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(fabsf(b)));
+  return m;
+}
+
+}  // namespace soinfer

@@ -85,6 +85,11 @@ _SIGNATURES = {
     "soinfer_decode_layers_fused": (_INT, [_P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F32, _P, _P, _P, _P,
                                            _P, _I64, _P]),
     "soinfer_gemm_w4a16_batch": (_INT, [_P, _I64, _I64, _P, _I64, _P]),
+    "soinfer_paged_kv_append": (_INT, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _F32, _P]),
+    "soinfer_paged_kv_read": (_INT, [_P, _P, _I64, _I64, _P, _P, _P]),
+    "soinfer_paged_decode_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
+    "soinfer_paged_decode_attention": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _I64, _P]),
+    "soinfer_prefill_attention": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P]),
     "soinfer_tp_allreduce_add_rmsnorm": (_INT, [_P, _P, _P, _P, _P, _P, _I64, _F32, _P]),
     "soinfer_gemv_w4a16_tp_partial": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P]),
     "soinfer_gemv_w4a16_batch_tp": (_INT, [_P, _P, _I64, _P, _I64, _P]),
@@ -872,6 +877,185 @@ def head_norm_rope(q, k, v, q_norm, k_norm, cos_vals, sin_vals, k_cache, v_cache
         _call("soinfer_head_norm_rope", _ptr(q), _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(cos_vals),
               _ptr(sin_vals), table_rows, _ptr(k_cache), _ptr(v_cache), nq, nkv, hd, max_seq, pos, _ptr(pos_dev),
               float(eps), _stream(dev))
+
+
+# ------------------------------------------------------- paged KV cache, prompts
+class _PagedCache(ctypes.Structure):
+    _fields_ = [("k_pages", _P), ("v_pages", _P), ("block_table", _P), ("table_stride", _I64), ("table_cols", _I64),
+                ("num_pages", _I64), ("num_kv_heads", _I64), ("page_size", _I64), ("head_dim", _I64), ("bits", _I64)]
+
+
+class _Rows(ctypes.Structure):
+    _fields_ = [("data", _P), ("token_stride", _I64), ("head_stride", _I64)]
+
+
+PAGED_HEAD_DIMS = (64, 128)
+
+
+def paged_kv_alloc(num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, bits: int = 16, device="cuda"):
+    """Zeroed page pools (k_pages, v_pages): fp16 [num_pages, num_kv_heads,
+    page_size, head_dim], or for bits = 4 uint8 with head_dim/2 + head_dim/16
+    (K) and head_dim/2 + 2 (V) bytes per position as the last dimension."""
+    name = "paged_kv_alloc"
+    _check(head_dim in PAGED_HEAD_DIMS, name, ": head_dim must be 64 or 128")
+    _check(page_size >= 16 and page_size <= 1 << 16 and page_size & (page_size - 1) == 0, name,
+           ": page_size must be a power of two in [16, 65536]")
+    _check(bits in (4, 16), name, ": bits must be 16 or 4")
+    _check(num_pages >= 0 and num_kv_heads >= 1, name, ": invalid num_pages / num_kv_heads")
+    if bits == 16:
+        widths, dtype = (head_dim, head_dim), torch.float16
+    else:
+        widths, dtype = (head_dim // 2 + head_dim // 16, head_dim // 2 + 2), torch.uint8
+    return tuple(torch.zeros(num_pages, num_kv_heads, page_size, w, dtype=dtype, device=device) for w in widths)
+
+
+def _paged_cache(name: str, k_pages, v_pages, block_table, head_dim: int | None = None) -> _PagedCache:
+    """The checked C form of a paged cache (head_dim None: taken from the pages)."""
+    _check(k_pages.is_cuda and v_pages.is_cuda and block_table.is_cuda, name, ": pages and block_table must be CUDA tensors")
+    _check(k_pages.dtype == v_pages.dtype and k_pages.dtype in (torch.float16, torch.uint8), name,
+           ": k_pages / v_pages must both be float16 or both uint8 (4 bits)")
+    ks, vs = k_pages.shape, v_pages.shape
+    _check(len(ks) == 4 and len(vs) == 4 and ks[:3] == vs[:3] and k_pages.is_contiguous() and v_pages.is_contiguous(), name,
+           ": k_pages / v_pages must be contiguous [num_pages, num_kv_heads, page_size, width]")
+    bits = 16 if k_pages.dtype == torch.float16 else 4
+    hd = ks[3] if bits == 16 else ks[3] * 16 // 9
+    _check(hd in PAGED_HEAD_DIMS and (ks[3] == vs[3] if bits == 16 else ks[3] == hd // 2 + hd // 16 and vs[3] == hd // 2 + 2),
+           name, ": page widths must be head_dim (64 or 128), or for 4 bits head_dim/2 + head_dim/16 and head_dim/2 + 2")
+    _check(head_dim is None or head_dim == hd, name, ": head_dim of the rows and of the pages disagree")
+    _check(ks[2] >= 16 and ks[2] <= 1 << 16 and ks[2] & (ks[2] - 1) == 0, name,
+           ": page_size must be a power of two in [16, 65536]")
+    _check(block_table.dtype == torch.int32 and block_table.dim() == 2
+           and (block_table.size(1) <= 1 or block_table.stride(1) == 1), name,
+           ": block_table must be int32 [num_seqs, max_pages] with contiguous rows")
+    cols = block_table.size(1) if block_table.size(0) else 0
+    stride = block_table.stride(0) if block_table.size(0) > 1 else cols
+    _check(stride >= cols, name, ": block_table rows must not overlap")
+    return _PagedCache(_ptr(k_pages), _ptr(v_pages), _ptr(block_table), stride, cols, ks[0], ks[1], ks[2], hd, bits)
+
+
+def _rows(name: str, what: str, x) -> _Rows:
+    _check(x.is_cuda and x.dtype == torch.float16, name, "(", what, "): must be a float16 CUDA tensor")
+    _check(x.dim() == 3 and x.stride(2) == 1, name, "(", what, "): must be [tokens, heads, head_dim] with contiguous heads")
+    st, sh = x.stride(0), x.stride(1)
+    _check(st % 8 == 0 and sh % 8 == 0 and x.data_ptr() % 16 == 0, name, "(", what,
+           "): needs 16-byte aligned rows (strides in multiples of 8 elements)")
+    return _Rows(x.data_ptr(), st, sh)
+
+
+def _int32(name: str, what: str, t, n: int) -> None:
+    _check(t.is_cuda and t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.size(0) == n, name, "(", what,
+           f"): must be a contiguous int32 CUDA tensor of {n} elements")
+
+
+def _out_rows(name: str, out, shape, dev) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=torch.float16, device=dev)
+    _check(out.is_cuda and out.dtype == torch.float16 and tuple(out.shape) == tuple(shape) and out.is_contiguous()
+           and out.data_ptr() % 16 == 0, name, f": out must be a contiguous float16 CUDA tensor of shape {tuple(shape)}")
+    return out
+
+
+def paged_kv_append(q, k, v, k_pages, v_pages, block_table, start, cos_table, sin_table, cu_seqlens=None, q_norm=None,
+                    k_norm=None, eps: float = 1e-6, return_k: bool = False):
+    name = "paged_kv_append"
+    rk, rv = _rows(name, "k", k), _rows(name, "v", v)
+    rq = _rows(name, "q", q) if q is not None else None
+    T, nkv, hd = k.shape
+    nq = q.size(1) if q is not None else 0
+    cache = _paged_cache(name, k_pages, v_pages, block_table, hd)
+    _check(v.shape == k.shape and nkv == cache.num_kv_heads, name, ": k / v must be [tokens, num_kv_heads, head_dim]")
+    _check(q is None or (q.size(0) == T and q.size(2) == hd), name, ": q must be [tokens, num_q_heads, head_dim]")
+    B = block_table.size(0)
+    _int32(name, "start", start, B)
+    if cu_seqlens is not None:
+        _int32(name, "cu_seqlens", cu_seqlens, B + 1)
+    else:
+        _check(T == B, name, ": without cu_seqlens there must be one token per sequence")
+    for t, what in ((cos_table, "cos_table"), (sin_table, "sin_table")):
+        _f32(t, f"{name}({what})")
+        _check(t.dim() == 2 and t.size(0) >= 1 and t.size(1) == hd // 2, name, f"({what}): must be [max_pos, head_dim / 2]")
+    _check(cos_table.size(0) == sin_table.size(0), name, ": cos_table and sin_table must have the same shape")
+    for t, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if t is not None:
+            _f16(t, f"{name}({what})")
+            _check(t.numel() == hd and t.data_ptr() % 16 == 0, name, f"({what}): must be [head_dim], 16-byte aligned")
+    dev = _same_device(k, v, k_pages, v_pages, block_table, start, cos_table, sin_table,
+                       *(t for t in (q, cu_seqlens, q_norm, k_norm) if t is not None))
+    q_out = torch.empty(T, nq, hd, dtype=torch.float16, device=dev) if q is not None else None
+    k_out = torch.empty(T, nkv, hd, dtype=torch.float16, device=dev) if return_k else None
+    if T == 0:
+        return q_out, k_out
+    with torch.cuda.device(dev):
+        _call("soinfer_paged_kv_append", ctypes.byref(cache), ctypes.byref(rq) if rq is not None else None,
+              ctypes.byref(rk), ctypes.byref(rv), _ptr(q_out), _ptr(k_out), T, nq, B, _ptr(cu_seqlens), _ptr(start),
+              _ptr(cos_table), _ptr(sin_table), cos_table.size(0), _ptr(q_norm), _ptr(k_norm), float(eps), _stream(dev))
+    return q_out, k_out
+
+
+def paged_kv_read(k_pages, v_pages, block_table, cu_seqlens, total: int, out=None):
+    name = "paged_kv_read"
+    cache = _paged_cache(name, k_pages, v_pages, block_table)
+    B = block_table.size(0)
+    _int32(name, "cu_seqlens", cu_seqlens, B + 1)
+    _check(total >= 0, name, ": total must be >= 0")
+    dev = _same_device(k_pages, v_pages, block_table, cu_seqlens)
+    shape = (total, cache.num_kv_heads, cache.head_dim)
+    ko, vo = (_out_rows(name, t, shape, dev) for t in (out if out is not None else (None, None)))
+    _same_device(k_pages, ko, vo)
+    if total == 0:
+        return ko, vo
+    with torch.cuda.device(dev):
+        _call("soinfer_paged_kv_read", ctypes.byref(cache), _ptr(cu_seqlens), B, total, _ptr(ko), _ptr(vo), _stream(dev))
+    return ko, vo
+
+
+def paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, out=None) -> torch.Tensor:
+    name = "paged_decode_attention"
+    rq = _rows(name, "q", q)
+    B, nq, hd = q.shape
+    cache = _paged_cache(name, k_pages, v_pages, block_table, hd)
+    nkv = cache.num_kv_heads
+    _check(nq >= 1 and nq % nkv == 0, name, ": num_q_heads must be a multiple of num_kv_heads")
+    _check(block_table.size(0) == B, name, ": block_table must have one row per query")
+    _int32(name, "seq_lens", seq_lens, B)
+    dev = _same_device(q, k_pages, v_pages, block_table, seq_lens)
+    out = _out_rows(name, out, (B, nq, hd), dev)
+    _same_device(q, out)
+    if B == 0:
+        return out
+    with torch.cuda.device(dev):
+        # a workspace of the call's own: two captured graphs or streams never share one
+        ws = torch.empty(lib().soinfer_paged_decode_workspace_bytes(B, nq, nkv, hd), dtype=torch.uint8, device=dev)
+        _call("soinfer_paged_decode_attention", ctypes.byref(cache), ctypes.byref(rq), _ptr(out), B, nq, _ptr(seq_lens),
+              ws.data_ptr(), ws.numel(), _stream(dev))
+    return out
+
+
+def prefill_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None) -> torch.Tensor:
+    name = "prefill_attention"
+    rq, rk, rv = _rows(name, "q", q), _rows(name, "k", k), _rows(name, "v", v)
+    Tq, nq, hd = q.shape
+    Tk, nkv = k.shape[:2]
+    _check(v.shape == k.shape and k.size(2) == hd, name, ": k / v must be [tokens, num_kv_heads, head_dim]")
+    _check(hd in PAGED_HEAD_DIMS, name, ": head_dim must be 64 or 128")
+    _check(nkv >= 1 and nq >= 1 and nq % nkv == 0, name, ": num_q_heads must be a multiple of num_kv_heads")
+    _check(cu_seqlens.dim() == 1 and cu_seqlens.size(0) >= 1, name, ": cu_seqlens must be [num_seqs + 1]")
+    n = cu_seqlens.size(0)
+    _int32(name, "cu_seqlens", cu_seqlens, n)
+    if cu_seqlens_k is None:
+        _check(Tk == Tq, name, ": without cu_seqlens_k, q and k must have the same tokens")
+        cu_seqlens_k = cu_seqlens
+    else:
+        _int32(name, "cu_seqlens_k", cu_seqlens_k, n)
+    dev = _same_device(q, k, v, cu_seqlens, cu_seqlens_k)
+    out = _out_rows(name, out, (Tq, nq, hd), dev)
+    _same_device(q, out)
+    if Tq == 0:
+        return out
+    with torch.cuda.device(dev):
+        _call("soinfer_prefill_attention", ctypes.byref(rq), ctypes.byref(rk), ctypes.byref(rv), _ptr(out), Tq, Tk, n - 1,
+              _ptr(cu_seqlens), _ptr(cu_seqlens_k), nq, nkv, hd, _stream(dev))
+    return out
 
 
 def rope_apply_at(x, cos_table, sin_table, pos_dev) -> None:

@@ -229,3 +229,56 @@ def gemm_w4a16(Wq_packed: torch.Tensor, scale: torch.Tensor, X: torch.Tensor, K:
     """B200 addition: batched decode -- Y [M, N] = X [M, K] W^T for M <= 8 tokens in one pass over the INT4
     weights (each row of Y is the reference's gemv_w4a16_group_lop3 of that token)."""
     return _C.gemm_w4a16(Wq_packed, scale, X, K, group_size)
+
+
+# ------------------------------------------------------------------ B200 additions: paged KV cache, whole prompts
+def paged_kv_alloc(num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, bits: int = 16, device="cuda"):
+    """B200 addition: zeroed page pools (k_pages, v_pages) of a paged KV cache.  bits = 16: fp16 [num_pages,
+    num_kv_heads, page_size, head_dim].  bits = 4: uint8 blocks of codes and fp16 scales (K: one scale per 32 values, V:
+    one per position; the layout stands in include/soinfer_b200.h), 4.5 and 4.125 bits a value at head_dim 128.
+    head_dim 64 or 128, page_size a power of two in [16, 65536]."""
+    return _C.paged_kv_alloc(num_pages, num_kv_heads, page_size, head_dim, bits, device)
+
+
+def paged_kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
+                    v_pages: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor, cos_table: torch.Tensor,
+                    sin_table: torch.Tensor, cu_seqlens: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
+                    k_norm: torch.Tensor | None = None, eps: float = 1e-6, return_k: bool = False):
+    """B200 addition: the new tokens of several sequences enter a paged cache.  Token j of sequence b (rows
+    cu_seqlens[b] .. of q [T, NQ, hd] and k / v [T, NKV, hd]; without cu_seqlens one token per sequence) stands at
+    position start[b] + j: optional per-head RMSNorm (q_norm / k_norm), rotate-half RoPE with that row of the tables
+    (precompute_rope_table), k and v stored in the page that block_table (int32 [B, max_pages]) names, as fp16 or 4 bits.
+    Returns (rotated q or None, rotated k if return_k else None); q, k, v may be strided slices of one projection.  The
+    arithmetic is fp32 with one rounding at the end (head_norm_rope also rounds the normalised row).  A token of no
+    sequence or beyond the tables comes back as zeros and is not stored; a position without a page is not stored.  No two
+    tokens may name the same place.  start, cu_seqlens and block_table are read on the device: graph-capturable."""
+    return _C.paged_kv_append(q, k, v, k_pages, v_pages, block_table, start, cos_table, sin_table, cu_seqlens, q_norm,
+                              k_norm, eps, return_k)
+
+
+def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                  total: int, out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """B200 addition: the first cu_seqlens[b + 1] - cu_seqlens[b] cached positions of every sequence as packed fp16 rows
+    (k, v), each [total, NKV, hd], total = cu_seqlens[-1] -- the context that prefill_attention needs to continue a
+    prompt.  4-bit rows come back as the values they stand for, positions without a page as zeros.  out = (k, v): rows of
+    no sequence are left as they were (in fresh outputs they are unset)."""
+    return _C.paged_kv_read(k_pages, v_pages, block_table, cu_seqlens, total, out)
+
+
+def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                      cu_seqlens_k: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """B200 addition: causal attention of packed prompts in one pass.  Sequence b's queries are rows cu_seqlens[b] ..
+    cu_seqlens[b + 1] (int32, on the device) of q [T, NQ, hd], its keys and values rows cu_seqlens_k[b] .. (default: the
+    same rows) of k / v [Tk, NKV, hd]; query i of Lq sees keys j <= i + Lk - Lq, so a chunk of a prompt attends to the
+    context before it.  Query head h reads kv head h // (NQ // NKV); scale 1/sqrt(hd), fp32 softmax and sums; hd 64 or
+    128.  A query without keys gives zeros; rows of no sequence are left as they were in out (unset in a fresh one)."""
+    return _C.prefill_attention(q, k, v, cu_seqlens, cu_seqlens_k, out)
+
+
+def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                           seq_lens: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """B200 addition: decode_attention for sequences of different lengths over a paged cache (fp16 or 4-bit pages): one
+    query per sequence, q [B, NQ, hd], over its first seq_lens[b] positions (int32 [B], read on the device:
+    graph-capturable; at most max_pages * page_size).  Positions without a page are skipped; a sequence without positions
+    gives zeros."""
+    return _C.paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, out)
