@@ -98,6 +98,8 @@ int soinfer_device_errors(int* flags) {
   *flags |= f;
   if (int st = cuda_result(read_and_clear_decode_fused_error(&f), "device_errors")) return st;
   *flags |= f;
+  if (int st = cuda_result(read_and_clear_prefill_error(&f), "device_errors")) return st;
+  *flags |= f;
   return SOINFER_OK;
 }
 
@@ -1067,6 +1069,10 @@ int soinfer_prefill_attention(const soinfer_rows* q, const soinfer_rows* k, cons
     P.v = as_half(v->data), P.v_token = v->token_stride, P.v_head = v->head_stride;
   }
   REQUIRE(out && aligned(out, 16) && cu_seqlens_q && cu_seqlens_k, "%s: null pointer or misaligned out", name);
+  REQUIRE((tokens_q == 1 || q->token_stride) && (num_q_heads == 1 || q->head_stride) &&
+              (tokens_k <= 1 || (k->token_stride && v->token_stride)) &&
+              (num_kv_heads == 1 || tokens_k == 0 || (k->head_stride && v->head_stride)),
+          "%s: strides must be positive", name);
   P.q = as_half(q->data), P.q_token = q->token_stride, P.q_head = q->head_stride;
   P.out = as_half(out);
   P.tokens_q = (int)tokens_q;

@@ -344,5 +344,6 @@ struct PrefillParams {
   const int32_t *cu_q, *cu_k;
 };
 cudaError_t launch_prefill_attention(const PrefillParams& P, cudaStream_t stream);
+cudaError_t read_and_clear_prefill_error(int* out);
 
 }  // namespace soinfer

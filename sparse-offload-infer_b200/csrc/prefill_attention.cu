@@ -1,55 +1,504 @@
-// Causal attention of packed prompts (grouped heads, sequences of different lengths).
+// Causal attention of packed prompts (grouped heads, sequences of different lengths) on the tcgen05 tensor cores.
+//
+//   o_i = sum_{j <= i + Lk - Lq} exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i),   s_ij = q_i . k_j / sqrt(hd)
+//
+// One pass over the keys with the running maximum and sum of the softmax; scores and outputs never leave the SM.  Two
+// products of 4 hd flop per pair together and one exponential per pair: at hd = 128 a 128 x 128 tile costs the tensor
+// core 2 x 512 cycles and the exponential unit (16 per cycle and SM) 1024, so both bound it and have to overlap.
+//
+// A CTA holds two tiles of 128 query rows that share a kv head (stages 0 and 1: two heads of the group, or two row
+// tiles).  Their scores S (fp32, 128 columns each) and outputs O (fp32, hd columns each) fill the tensor memory; the
+// probabilities P (fp16) overwrite the scores they come from and feed the second product from there.
+//   warps 0-3, 4-7: the softmax of stage 0 / 1, one thread per row.
+//   warp 8: loads Q, then K and V tiles of 128 keys through a ring of four slots (TMA, 128-byte swizzle).  A last V tile
+//           with fewer keys has its other rows cleared: what lies behind a sequence may be anything, and 0 * NaN counts.
+//   warp 9: one thread issues the products in the order  S0(j) P1V(j-1) S1(j) P0V(j) -- while the tensor core works on one
+//           stage, the other stage's softmax runs.  Products of one thread run in order, so S(j+1) overwrites P(j) only
+//           after P(j) V has read it; a commit covers everything issued before it, so scores that have arrived say that
+//           the O before them is complete.
+// The running maximum moves only when a row exceeds it by 2^8 (O is rescaled in place then, by the softmax warps); the
+// probabilities carry a factor 2^7 so that fp16 keeps 11 bits down to 2^-21 of the largest; the sum is fp32 over the
+// unrounded ones and the factor cancels.
+// A masked score is selected away, but a non-finite V in a masked place of a shared tile would still reach the product:
+// rows whose result is not finite are computed again one by one over exactly the keys they see.
+//
+// The grid holds one CTA per pair of tiles and kv head, an upper bound from the token counts (row bounds are read on the
+// device); within a sequence the longest rows come first, so that the short ones fill the end.
+#include <cuda.h>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.cuh"
+#include "tcgen05.cuh"
 
 namespace soinfer {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kTile = 128;            // query rows and keys per tile
+constexpr int kSlots = 4;             // K / V tiles in flight
+constexpr int kThreads = 320;
+constexpr uint64_t kTimeoutNs = 1000000000ull;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.f;          // the maximum follows when exceeded by 2^8
+constexpr float kLift = 7.f;          // factor 2^7 on the probabilities
 
-// One warp per (query row, head): row i of a sequence sees keys j <= i + len_k - len_q.
+__device__ int g_prefill_error;
+
+struct Shared {
+  uint64_t q_full[2], kv_full[kSlots], kv_empty[kSlots], v_landed, s_full[2], p_full[2], o_full[2], drained;
+  uint32_t tmem;
+  int abort;
+};
+
+// Waits for a phase with a time limit; a wait that runs out tells the others and the host, and every later wait is short.
+__device__ __forceinline__ bool wait(Shared& sh, uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*reinterpret_cast<volatile int*>(&sh.abort)) return false;
+    if (globaltimer_ns() - t0 > kTimeoutNs) {
+      *reinterpret_cast<volatile int*>(&sh.abort) = 1;
+      atomicOr(&g_prefill_error, kErrCopyTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A CTA's work: two query tiles of sequence rows q0.., keys k0.., kv head kvh.
+struct Work {
+  int q0, lq, k0, lk, kvh;
+  int row[2], head[2], tiles[2];  // first row in the sequence, query head, key tiles (0: nothing to do)
+};
+
+// The pair of query tiles that blockIdx.x stands for (warp-wide; false: none).  Query tile t of a sequence and kv head
+// is head t % rep, rows (t / rep) * 128 ..; pairs run from the last to the first.
+__device__ __forceinline__ bool find_work(const PrefillParams& P, int lane, Work& w) {
+  const int rep = P.nq / P.nkv;
+  w.kvh = blockIdx.x % P.nkv;
+  const int want = blockIdx.x / P.nkv;
+  int before = 0;
+  for (int base = 0; base < P.seqs; base += 32) {
+    const int i = base + lane;
+    int q0 = 0, lq = 0;
+    if (i < P.seqs) {
+      const int a = __ldg(P.cu_q + i), e = __ldg(P.cu_q + i + 1);
+      q0 = a < 0 ? 0 : a;
+      lq = (e > P.tokens_q ? P.tokens_q : e) - q0;
+      if (lq < 0) lq = 0;
+    }
+    const int pairs = ((lq + kTile - 1) / kTile * rep + 1) / 2;
+    int sum = pairs;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    const int c = want - before;
+    const unsigned owns = __ballot_sync(0xffffffffu, c >= sum - pairs && c < sum);
+    if (owns) {
+      const int src = __ffs(owns) - 1, b = base + src;
+      w.q0 = __shfl_sync(0xffffffffu, q0, src);
+      w.lq = __shfl_sync(0xffffffffu, lq, src);
+      const int last = __shfl_sync(0xffffffffu, sum, src) - 1 - c;  // pairs from the sequence's end
+      const int ka = __ldg(P.cu_k + b), ke = __ldg(P.cu_k + b + 1);
+      w.k0 = ka < 0 ? 0 : ka;
+      w.lk = (ke > P.tokens_k ? P.tokens_k : ke) - w.k0;
+      if (w.lk < 0) w.lk = 0;
+      const int tiles = (w.lq + kTile - 1) / kTile * rep;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int t = 2 * last + s;
+        w.row[s] = t / rep * kTile;
+        w.head[s] = w.kvh * rep + t % rep;
+        const int rows = w.lq - w.row[s] < kTile ? w.lq - w.row[s] : kTile;
+        int keys = w.row[s] + rows + w.lk - w.lq;  // what the tile's last row sees
+        keys = keys < 0 ? 0 : keys;
+        w.tiles[s] = t < tiles ? (keys + kTile - 1) / kTile : -1;
+      }
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return false;
+}
+
+// One row over the n keys it sees, by a whole warp (rows whose tile result is not finite).
 template <int HD>
-__global__ void __launch_bounds__(32 * kWarps) prefill_rows_kernel(const PrefillParams P, const float scale_log2) {
+__device__ __noinline__ void redo_row(const PrefillParams& P, const half* q, int k0, int n, int kvh, half* out,
+                                      float scale_log2, int lane) {
   constexpr int E = HD / 32;
-  pdl_launch_dependents();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int row = blockIdx.x * kWarps + (threadIdx.x >> 5), h = blockIdx.y;
-  if (row >= P.tokens_q) return;
-  int b = 0;
-  while (b < P.seqs && P.cu_q[b + 1] <= row) ++b;
-  if (b >= P.seqs || row < P.cu_q[b]) return;
-  const int q0 = max(P.cu_q[b], 0), lq = min(P.cu_q[b + 1], P.tokens_q) - q0;
-  const int k0 = max(P.cu_k[b], 0), lk = max(min(P.cu_k[b + 1], P.tokens_k) - k0, 0);
-  const int kvh = h / (P.nq / P.nkv), n = row - q0 + 1 + lk - lq;
-  float q[E], acc[E], m = -INFINITY, l = 0.f;
+  float qf[E], acc[E], m = -INFINITY, l = 0.f;
+#pragma unroll
   for (int e = 0; e < E; ++e) {
-    q[e] = __half2float(P.q[row * P.q_token + h * P.q_head + lane * E + e]) * scale_log2;
+    qf[e] = __half2float(q[lane * E + e]) * scale_log2;
     acc[e] = 0.f;
   }
   for (int j = 0; j < n; ++j) {
-    const half* k = P.k + (k0 + j) * P.k_token + kvh * P.k_head + lane * E;
-    const half* v = P.v + (k0 + j) * P.v_token + kvh * P.v_head + lane * E;
+    const half* k = P.k + (int64_t)(k0 + j) * P.k_token + kvh * P.k_head + lane * E;
+    const half* v = P.v + (int64_t)(k0 + j) * P.v_token + kvh * P.v_head + lane * E;
     float s = 0.f;
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], __half2float(k[e]), s);
+#pragma unroll
+    for (int e = 0; e < E; ++e) s = fmaf(qf[e], __half2float(k[e]), s);
     s = warp_sum(s);
     const float top = fmaxf(m, s), f = m == top ? 1.f : exp2f(m - top), p = exp2f(s - top);
     m = top;
     l = fmaf(l, f, p);
+#pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = fmaf(p, __half2float(v[e]), acc[e] * f);
   }
-  for (int e = 0; e < E; ++e)
-    P.out[((int64_t)row * P.nq + h) * HD + lane * E + e] = __float2half_rn(n > 0 ? acc[e] / l : 0.f);
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[lane * E + e] = __float2half_rn(acc[e] / l);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                   const __grid_constant__ CUtensorMap v_map, const PrefillParams P, const float scale_log2) {
+  constexpr int kBox = kTile * 128;              // bytes of a TMA box: 128 rows of 64 fp16
+  constexpr int kBoxes = HD / 64;
+  constexpr int kTileBytes = kBoxes * kBox;
+  constexpr uint32_t kO = 2 * kTile;             // tensor memory columns: S0, S1, O0, O1
+  constexpr uint32_t kColumns = 512;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Shared sh;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_q = smem;                           // two tiles
+  uint8_t* s_kv = smem + 2 * kTileBytes;         // kSlots tiles
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_launch_dependents();
+  pdl_wait();
+  Work w;
+  if (!find_work(P, lane, w)) return;            // the same for every warp
+  const int steps = w.tiles[0] > w.tiles[1] ? w.tiles[0] : w.tiles[1];
+
+  if (warp == 9) {
+    tc::alloc(&sh.tmem, kColumns);
+  } else if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sh.q_full[s], 1);
+      mbar_init(&sh.s_full[s], 1);
+      mbar_init(&sh.p_full[s], kTile);
+      mbar_init(&sh.o_full[s], 1);
+    }
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&sh.kv_full[i], 1);
+      mbar_init(&sh.kv_empty[i], 1);
+    }
+    mbar_init(&sh.v_landed, 1);
+    mbar_init(&sh.drained, 1);
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- loads
+    // Key tile j is ring entry 2 j, value tile j entry 2 j + 1.
+    int issued = 0;
+    bool ok = true;
+    if (lane == 0) {
+      tc::prefetch_map(&q_map);
+      tc::prefetch_map(&k_map);
+      tc::prefetch_map(&v_map);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (w.tiles[s] > 0) {
+          mbar_arrive_expect_tx(&sh.q_full[s], kTileBytes);
+          for (int x = 0; x < kBoxes; ++x)
+            tc::tma_load_3d(s_q + s * kTileBytes + x * kBox, &q_map, 64 * x, w.head[s], w.q0 + w.row[s], &sh.q_full[s]);
+        }
+    }
+    for (int e = 0; e < 2 * steps && ok; ++e) {
+      const int slot = e % kSlots, j = e >> 1;
+      if (e >= kSlots) ok = wait(sh, &sh.kv_empty[slot], ((e / kSlots) - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      uint8_t* dst = s_kv + slot * kTileBytes;
+      const int rows = w.lk - j * kTile;         // valid rows of the tile
+      const bool clear = (e & 1) && rows < kTile;
+      uint64_t* bar = clear ? &sh.v_landed : &sh.kv_full[slot];
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, kTileBytes);
+        for (int x = 0; x < kBoxes; ++x)
+          tc::tma_load_3d(dst + x * kBox, e & 1 ? &v_map : &k_map, 64 * x, w.kvh, w.k0 + j * kTile, bar);
+      }
+      ++issued;
+      if (clear) {                               // at most once: the sequence's last tile
+        ok = __all_sync(0xffffffffu, wait(sh, &sh.v_landed, 0));
+        if (!ok) break;
+        for (int x = 0; x < kBoxes; ++x)
+          for (int i = rows * 8 + lane; i < kTile * 8; i += 32)
+            reinterpret_cast<uint4*>(dst + x * kBox)[i] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.kv_full[slot]);
+      }
+    }
+    if (!ok) {  // a wait ran out: let the copies in flight land before the CTA ends
+      const uint64_t t0 = globaltimer_ns();
+      for (int s = 0; s < 2; ++s)
+        while (w.tiles[s] > 0 && !mbar_try_wait(&sh.q_full[s], 0) && globaltimer_ns() - t0 < kTimeoutNs) {
+        }
+      for (int e = issued < kSlots ? 0 : issued - kSlots; e < issued; ++e)
+        while (!mbar_try_wait(&sh.kv_full[e % kSlots], (e / kSlots) & 1) && globaltimer_ns() - t0 < kTimeoutNs) {
+        }
+    }
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- products
+    if (lane == 0) {
+      constexpr uint32_t kIdescS = tc::instr_desc(kTile, kTile, false), kIdescO = tc::instr_desc(kTile, HD, true);
+      bool ok = true;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (w.tiles[s] > 0) ok = ok && wait(sh, &sh.q_full[s], 0);
+      auto scores = [&](int s, int j) {          // S_s = Q_s K_j^T
+        const uint32_t a = smem_u32(s_q + s * kTileBytes), b = smem_u32(s_kv + (2 * j % kSlots) * kTileBytes);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t at = (k / 4) * kBox + (k % 4) * 32;
+          tc::mma_ss(tmem + s * kTile, tc::smem_desc(a + at, 16, 1024), tc::smem_desc(b + at, 16, 1024), kIdescS, k > 0);
+        }
+        tc::commit(&sh.s_full[s]);
+      };
+      auto outputs = [&](int s, int j) {         // O_s (+)= P_s V_j
+        ok = ok && wait(sh, &sh.p_full[s], j & 1);
+        if (!ok) return;
+        tc::fence_after();
+        const uint32_t b = smem_u32(s_kv + ((2 * j + 1) % kSlots) * kTileBytes);
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          tc::mma_ts(tmem + kO + s * HD, tmem + s * kTile + k * 8, tc::smem_desc(b + k * 2048, kBox, 1024), kIdescO,
+                     j > 0 || k > 0);
+        if (j == w.tiles[s] - 1) tc::commit(&sh.o_full[s]);
+      };
+      for (int j = 0; j <= steps && ok; ++j) {
+        if (j < steps) ok = wait(sh, &sh.kv_full[2 * j % kSlots], (2 * j / kSlots) & 1);
+        if (!ok) break;
+        tc::fence_after();
+        if (j < w.tiles[0]) scores(0, j);
+        if (j > 0) {
+          if (j - 1 < w.tiles[1]) {
+            ok = wait(sh, &sh.kv_full[(2 * j - 1) % kSlots], ((2 * j - 1) / kSlots) & 1);
+            if (ok) outputs(1, j - 1);
+            if (!ok) break;
+          }
+          tc::commit(&sh.kv_empty[(2 * j - 1) % kSlots]);
+        }
+        if (j == steps) break;
+        if (j < w.tiles[1]) scores(1, j);
+        tc::commit(&sh.kv_empty[2 * j % kSlots]);
+        if (j < w.tiles[0]) {
+          ok = wait(sh, &sh.kv_full[(2 * j + 1) % kSlots], ((2 * j + 1) / kSlots) & 1);
+          if (ok) outputs(0, j);
+        }
+      }
+      if (!ok) {  // let the products in flight end before the tensor memory is given back
+        tc::commit(&sh.drained);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&sh.drained, 0) && globaltimer_ns() - t0 < kTimeoutNs) {
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int s = warp >> 2, r = threadIdx.x & (kTile - 1);
+    const int tiles = w.tiles[s], row = w.row[s] + r;
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+    const uint32_t S = lanes + s * kTile, O = lanes + kO + s * HD;
+    const bool valid = row < w.lq;
+    int limit = valid ? row + 1 + w.lk - w.lq : 0;  // keys this row sees
+    if (limit < 0) limit = 0;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < tiles && ok; ++j) {
+      ok = __all_sync(0xffffffffu, wait(sh, &sh.s_full[s], j & 1));
+      if (!ok) break;
+      tc::fence_after();
+      uint32_t x[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tc::ld32(x[c], S + 32 * c);
+      tc::wait_ld();
+      const int left = limit - j * kTile;
+      if (__any_sync(0xffffffffu, left < kTile)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * c + i >= left) x[c][i] = 0xff800000u;  // -inf
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[c][i]));
+      top *= scale_log2;
+      const bool move = top > m + kLazy;  // also the first finite maximum
+      if (__any_sync(0xffffffffu, move)) {
+        const float f = move ? ex2(m - top) : 1.f;
+        if (move) m = top;
+        l *= f;
+        if (j > 0) {
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            tc::ld32(o, O + 32 * c);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tc::st32(O + 32 * c, o);
+          }
+        }
+      }
+      const float shift = m == -INFINITY ? 0.f : kLift - m;
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float a = ex2(fmaf(__uint_as_float(x[c][2 * i]), scale_log2, shift));
+          const float b = ex2(fmaf(__uint_as_float(x[c][2 * i + 1]), scale_log2, shift));
+          sum[0] += a;
+          sum[1] += b;
+          p[i] = h2_as_u32(__floats2half2_rn(a, b));
+        }
+        tc::st16(S + 16 * c, p);
+      }
+      l += sum[0] + sum[1];
+      tc::wait_st();
+      tc::fence_before();
+      mbar_arrive(&sh.p_full[s]);
+    }
+    // the row's result
+    if (tiles >= 0 && ok) {
+      half* out = P.out + ((int64_t)(w.q0 + row) * P.nq + w.head[s]) * HD;
+      bool good = true;
+      if (tiles > 0) {
+        ok = __all_sync(0xffffffffu, wait(sh, &sh.o_full[s], 0));
+        tc::fence_after();
+      }
+      if (ok) {
+        const float inv = limit > 0 ? 1.f / l : 0.f;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          if (tiles > 0) {
+            tc::ld32(o, O + 32 * c);
+            tc::wait_ld();
+          }
+          uint4 v[4];
+          uint32_t* h = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float a = 0.f, b = 0.f;
+            if (limit > 0) a = __uint_as_float(o[2 * i]) * inv, b = __uint_as_float(o[2 * i + 1]) * inv;
+            good = good && fabsf(a) <= 3.4e38f && fabsf(b) <= 3.4e38f;
+            h[i] = h2_as_u32(__floats2half2_rn(a, b));
+          }
+          if (valid)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(out)[4 * c + i] = v[i];
+        }
+        unsigned again = __ballot_sync(0xffffffffu, valid && !good);
+        while (again) {
+          const int src = __ffs(again) - 1, rr = w.row[s] + (r & ~31) + src;
+          again &= again - 1;
+          __syncwarp();
+          redo_row<HD>(P, P.q + (int64_t)(w.q0 + rr) * P.q_token + w.head[s] * P.q_head, w.k0, rr + 1 + w.lk - w.lq,
+                       w.kvh, P.out + ((int64_t)(w.q0 + rr) * P.nq + w.head[s]) * HD, scale_log2, lane);
+        }
+      }
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc::fence_after();
+    tc::dealloc(tmem, kColumns);
+  }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// Map of rows [tokens, heads, hd] with boxes of 64 values x 1 head x 128 tokens.
+cudaError_t make_map(CUtensorMap* map, const half* data, int64_t tokens, int64_t heads, int hd, int64_t token_stride,
+                     int64_t head_stride) {
+  const EncodeTiled encode = encoder();
+  if (!encode) return cudaErrorNotSupported;
+  // a dimension of one entry may have any stride
+  if (heads == 1) head_stride = hd;
+  if (tokens == 1) token_stride = heads * hd;
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
+  const cuuint32_t box[3] = {64, 1, kTile}, ones[3] = {1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<half*>(data), dims, strides, box, ones,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <int HD>
+cudaError_t prefill_hd(const PrefillParams& P, cudaStream_t stream) {
+  CUtensorMap q, k, v;
+  cudaError_t e = make_map(&q, P.q, P.tokens_q, P.nq, HD, P.q_token, P.q_head);
+  if (e != cudaSuccess) return e;
+  k = v = q;  // no keys: never read
+  if (P.tokens_k > 0) {
+    if ((e = make_map(&k, P.k, P.tokens_k, P.nkv, HD, P.k_token, P.k_head)) != cudaSuccess) return e;
+    if ((e = make_map(&v, P.v, P.tokens_k, P.nkv, HD, P.v_token, P.v_head)) != cudaSuccess) return e;
+  }
+  const int smem = (2 + kSlots) * kTile * HD * 2 + 1024;
+  if ((e = ensure_smem_attr<prefill_kernel<HD>>(smem)) != cudaSuccess) return e;
+  // sum over sequences of ceil(rep ceil(lq / 128) / 2) <= (rep (tokens / 128 + seqs') + seqs') / 2, seqs' of them not empty
+  const int64_t rep = P.nq / P.nkv, seqs = P.seqs < P.tokens_q ? P.seqs : P.tokens_q;
+  const int64_t pairs = (rep * (P.tokens_q / kTile + seqs) + seqs + 1) / 2;
+  if (pairs * P.nkv > 0x7fffffff) return cudaErrorInvalidValue;
+  const float scale_log2 = (1.0f / sqrtf((float)HD)) * kLog2e;
+  return launch_ex(prefill_kernel<HD>, dim3((unsigned)(pairs * P.nkv)), dim3(kThreads), (size_t)smem, stream, 1, true, q,
+                   k, v, P, scale_log2);
 }
 
 }  // namespace
 
 cudaError_t launch_prefill_attention(const PrefillParams& P, cudaStream_t stream) {
-  const float scale_log2 = (1.0f / sqrtf((float)P.hd)) * 1.4426950408889634f;
-  const dim3 grid((unsigned)((P.tokens_q + kWarps - 1) / kWarps), (unsigned)P.nq);
-  return launch_ex(P.hd == 128 ? prefill_rows_kernel<128> : prefill_rows_kernel<64>, grid, dim3(32 * kWarps), 0, stream,
-                   1, true, P, scale_log2);
+  return P.hd == 128 ? prefill_hd<128>(P, stream) : prefill_hd<64>(P, stream);
+}
+
+cudaError_t read_and_clear_prefill_error(int* out) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, g_prefill_error, sizeof(int));
+  if (e != cudaSuccess) return e;
+  const int zero = 0;
+  return cudaMemcpyToSymbol(g_prefill_error, &zero, sizeof(int));
 }
 
 }  // namespace soinfer

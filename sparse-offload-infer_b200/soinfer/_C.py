@@ -1033,6 +1033,9 @@ def paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, out=None)
 
 def prefill_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None) -> torch.Tensor:
     name = "prefill_attention"
+    # rows are loaded as boxes of a tensor map, which has no zero strides (an expanded dimension)
+    q, k, v = (t.contiguous() if t.dim() == 3 and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())) else t
+               for t in (q, k, v))
     rq, rk, rv = _rows(name, "q", q), _rows(name, "k", k), _rows(name, "v", v)
     Tq, nq, hd = q.shape
     Tk, nkv = k.shape[:2]
