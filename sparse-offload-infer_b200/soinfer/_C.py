@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -880,16 +881,16 @@ def head_norm_rope(q, k, v, q_norm, k_norm, cos_vals, sin_vals, k_cache, v_cache
 
 
 # ------------------------------------------------------- paged KV cache, prompts
-class _PagedCache(ctypes.Structure):
-    _fields_ = [("k_pages", _P), ("v_pages", _P), ("block_table", _P), ("table_stride", _I64), ("table_cols", _I64),
-                ("num_pages", _I64), ("num_kv_heads", _I64), ("page_size", _I64), ("head_dim", _I64), ("bits", _I64)]
-
-
-class _Rows(ctypes.Structure):
-    _fields_ = [("data", _P), ("token_stride", _I64), ("head_stride", _I64)]
-
-
+# These calls serve single tokens too, where the host's share is what a user waits for: the C structs are packed as bytes,
+# messages are put together only for a failure, and the device is switched only when it is not the current one.
+_PAGED_CACHE = struct.Struct("PPPqqqqqqq")  # soinfer_paged_cache
+_ROWS = struct.Struct("Pqq")                # soinfer_rows
 PAGED_HEAD_DIMS = (64, 128)
+_F16, _U8, _I32 = torch.float16, torch.uint8, torch.int32
+
+
+def _fail(*msg) -> None:
+    raise RuntimeError("".join(str(m) for m in msg))
 
 
 def paged_kv_alloc(num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, bits: int = 16, device="cuda"):
@@ -909,155 +910,194 @@ def paged_kv_alloc(num_pages: int, num_kv_heads: int, page_size: int, head_dim: 
     return tuple(torch.zeros(num_pages, num_kv_heads, page_size, w, dtype=dtype, device=device) for w in widths)
 
 
-def _paged_cache(name: str, k_pages, v_pages, block_table, head_dim: int | None = None) -> _PagedCache:
-    """The checked C form of a paged cache (head_dim None: taken from the pages)."""
-    _check(k_pages.is_cuda and v_pages.is_cuda and block_table.is_cuda, name, ": pages and block_table must be CUDA tensors")
-    _check(k_pages.dtype == v_pages.dtype and k_pages.dtype in (torch.float16, torch.uint8), name,
-           ": k_pages / v_pages must both be float16 or both uint8 (4 bits)")
-    ks, vs = k_pages.shape, v_pages.shape
-    _check(len(ks) == 4 and len(vs) == 4 and ks[:3] == vs[:3] and k_pages.is_contiguous() and v_pages.is_contiguous(), name,
-           ": k_pages / v_pages must be contiguous [num_pages, num_kv_heads, page_size, width]")
-    bits = 16 if k_pages.dtype == torch.float16 else 4
-    hd = ks[3] if bits == 16 else ks[3] * 16 // 9
-    _check(hd in PAGED_HEAD_DIMS and (ks[3] == vs[3] if bits == 16 else ks[3] == hd // 2 + hd // 16 and vs[3] == hd // 2 + 2),
-           name, ": page widths must be head_dim (64 or 128), or for 4 bits head_dim/2 + head_dim/16 and head_dim/2 + 2")
-    _check(head_dim is None or head_dim == hd, name, ": head_dim of the rows and of the pages disagree")
-    _check(ks[2] >= 16 and ks[2] <= 1 << 16 and ks[2] & (ks[2] - 1) == 0, name,
-           ": page_size must be a power of two in [16, 65536]")
-    _check(block_table.dtype == torch.int32 and block_table.dim() == 2
-           and (block_table.size(1) <= 1 or block_table.stride(1) == 1), name,
-           ": block_table must be int32 [num_seqs, max_pages] with contiguous rows")
-    cols = block_table.size(1) if block_table.size(0) else 0
-    stride = block_table.stride(0) if block_table.size(0) > 1 else cols
-    _check(stride >= cols, name, ": block_table rows must not overlap")
-    return _PagedCache(_ptr(k_pages), _ptr(v_pages), _ptr(block_table), stride, cols, ks[0], ks[1], ks[2], hd, bits)
+def _paged_cache(name: str, k_pages, v_pages, block_table, dev: int, head_dim: int | None = None):
+    """(the C form of a checked paged cache, its kv heads, its head_dim); dev: the device everything has to be on."""
+    if not (k_pages.is_cuda and v_pages.is_cuda and block_table.is_cuda):
+        _fail(name, ": pages and block_table must be CUDA tensors")
+    dtype = k_pages.dtype
+    if dtype != v_pages.dtype or (dtype != _F16 and dtype != _U8):
+        _fail(name, ": k_pages / v_pages must both be float16 or both uint8 (4 bits)")
+    ks, vs, ts = k_pages.shape, v_pages.shape, block_table.shape
+    if not (len(ks) == 4 and len(vs) == 4 and ks[:3] == vs[:3] and k_pages.is_contiguous() and v_pages.is_contiguous()):
+        _fail(name, ": k_pages / v_pages must be contiguous [num_pages, num_kv_heads, page_size, width]")
+    pages, nkv, page, wk = ks
+    if dtype == _F16:
+        bits, hd, fits = 16, wk, vs[3] == wk
+    else:
+        bits, hd = 4, wk * 16 // 9
+        fits = wk == hd // 2 + hd // 16 and vs[3] == hd // 2 + 2
+    if not fits or hd not in PAGED_HEAD_DIMS:
+        _fail(name, ": page widths must be head_dim (64 or 128), or for 4 bits head_dim/2 + head_dim/16 and head_dim/2 + 2")
+    if head_dim is not None and head_dim != hd:
+        _fail(name, ": head_dim of the rows and of the pages disagree")
+    if page < 16 or page > 1 << 16 or page & (page - 1):
+        _fail(name, ": page_size must be a power of two in [16, 65536]")
+    if block_table.dtype != _I32 or len(ts) != 2 or (ts[1] > 1 and block_table.stride(1) != 1):
+        _fail(name, ": block_table must be int32 [num_seqs, max_pages] with contiguous rows")
+    cols = ts[1] if ts[0] else 0
+    stride = block_table.stride(0) if ts[0] > 1 else cols
+    if stride < cols:
+        _fail(name, ": block_table rows must not overlap")
+    if not (k_pages.get_device() == v_pages.get_device() == block_table.get_device() == dev):
+        _fail(name, ": all tensors must be on the same CUDA device")
+    return (_PAGED_CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), stride, cols, pages, nkv, page,
+                              hd, bits), nkv, hd)
 
 
-def _rows(name: str, what: str, x) -> _Rows:
-    _check(x.is_cuda and x.dtype == torch.float16, name, "(", what, "): must be a float16 CUDA tensor")
-    _check(x.dim() == 3 and x.stride(2) == 1, name, "(", what, "): must be [tokens, heads, head_dim] with contiguous heads")
-    st, sh = x.stride(0), x.stride(1)
-    _check(st % 8 == 0 and sh % 8 == 0 and x.data_ptr() % 16 == 0, name, "(", what,
-           "): needs 16-byte aligned rows (strides in multiples of 8 elements)")
-    return _Rows(x.data_ptr(), st, sh)
+def _rows(name: str, what: str, x):
+    """(the C form of checked rows [tokens, heads, head_dim], their shape)."""
+    if not x.is_cuda or x.dtype != _F16:
+        _fail(name, "(", what, "): must be a float16 CUDA tensor")
+    shape, stride, at = x.shape, x.stride(), x.data_ptr()
+    if len(shape) != 3 or stride[2] != 1:
+        _fail(name, "(", what, "): must be [tokens, heads, head_dim] with contiguous heads")
+    if stride[0] & 7 or stride[1] & 7 or at & 15:
+        _fail(name, "(", what, "): needs 16-byte aligned rows (strides in multiples of 8 elements)")
+    return _ROWS.pack(at, stride[0], stride[1]), shape
 
 
-def _int32(name: str, what: str, t, n: int) -> None:
-    _check(t.is_cuda and t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.size(0) == n, name, "(", what,
-           f"): must be a contiguous int32 CUDA tensor of {n} elements")
+def _int32(name: str, what: str, t, n: int, dev: int) -> int:
+    if not t.is_cuda or t.dtype != _I32 or t.dim() != 1 or t.size(0) != n or not t.is_contiguous():
+        _fail(name, "(", what, f"): must be a contiguous int32 CUDA tensor of {n} elements")
+    if t.get_device() != dev:
+        _fail(name, ": all tensors must be on the same CUDA device")
+    return t.data_ptr()
 
 
-def _out_rows(name: str, out, shape, dev) -> torch.Tensor:
+def _out_rows(name: str, out, like, shape) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=torch.float16, device=dev)
-    _check(out.is_cuda and out.dtype == torch.float16 and tuple(out.shape) == tuple(shape) and out.is_contiguous()
-           and out.data_ptr() % 16 == 0, name, f": out must be a contiguous float16 CUDA tensor of shape {tuple(shape)}")
+        return like.new_empty(shape, dtype=_F16)
+    if not (out.is_cuda and out.dtype == _F16 and tuple(out.shape) == shape and out.is_contiguous()
+            and out.data_ptr() % 16 == 0):
+        _fail(name, f": out must be a contiguous, 16-byte aligned float16 CUDA tensor of shape {shape}")
+    if out.get_device() != like.get_device():
+        _fail(name, ": all tensors must be on the same CUDA device")
     return out
+
+
+def _call_on(dev: int, fn_name: str, *args) -> None:
+    """_call with the device's current stream as the last argument and the device current."""
+    if torch._C._cuda_getDevice() == dev:
+        _call(fn_name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _call(fn_name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def paged_kv_append(q, k, v, k_pages, v_pages, block_table, start, cos_table, sin_table, cu_seqlens=None, q_norm=None,
                     k_norm=None, eps: float = 1e-6, return_k: bool = False):
     name = "paged_kv_append"
-    rk, rv = _rows(name, "k", k), _rows(name, "v", v)
-    rq = _rows(name, "q", q) if q is not None else None
-    T, nkv, hd = k.shape
-    nq = q.size(1) if q is not None else 0
-    cache = _paged_cache(name, k_pages, v_pages, block_table, hd)
-    _check(v.shape == k.shape and nkv == cache.num_kv_heads, name, ": k / v must be [tokens, num_kv_heads, head_dim]")
-    _check(q is None or (q.size(0) == T and q.size(2) == hd), name, ": q must be [tokens, num_q_heads, head_dim]")
+    rk, ks = _rows(name, "k", k)
+    rv, vs = _rows(name, "v", v)
+    T, nkv, hd = ks
+    dev = k.get_device()
+    cache, heads, _ = _paged_cache(name, k_pages, v_pages, block_table, dev, hd)
+    if ks != vs or nkv != heads:
+        _fail(name, ": k / v must be [tokens, num_kv_heads, head_dim]")
+    rq, nq, q_out, k_out = None, 0, None, None
+    if q is not None:
+        rq, (tq, nq, hq) = _rows(name, "q", q)
+        if tq != T or hq != hd:
+            _fail(name, ": q must be [tokens, num_q_heads, head_dim]")
     B = block_table.size(0)
-    _int32(name, "start", start, B)
+    start_at = _int32(name, "start", start, B, dev)
+    cu_at = None
     if cu_seqlens is not None:
-        _int32(name, "cu_seqlens", cu_seqlens, B + 1)
-    else:
-        _check(T == B, name, ": without cu_seqlens there must be one token per sequence")
+        cu_at = _int32(name, "cu_seqlens", cu_seqlens, B + 1, dev)
+    elif T != B:
+        _fail(name, ": without cu_seqlens there must be one token per sequence")
     for t, what in ((cos_table, "cos_table"), (sin_table, "sin_table")):
-        _f32(t, f"{name}({what})")
-        _check(t.dim() == 2 and t.size(0) >= 1 and t.size(1) == hd // 2, name, f"({what}): must be [max_pos, head_dim / 2]")
-    _check(cos_table.size(0) == sin_table.size(0), name, ": cos_table and sin_table must have the same shape")
-    for t, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or t.size(1) != hd // 2:
+            _fail(name, f"({what}): must be a contiguous float32 CUDA tensor [max_pos, head_dim / 2]")
+    rows = cos_table.size(0)
+    if rows != sin_table.size(0):
+        _fail(name, ": cos_table and sin_table must have the same shape")
+    norms = [None, None]
+    for i, t in enumerate((q_norm, k_norm)):
         if t is not None:
-            _f16(t, f"{name}({what})")
-            _check(t.numel() == hd and t.data_ptr() % 16 == 0, name, f"({what}): must be [head_dim], 16-byte aligned")
-    dev = _same_device(k, v, k_pages, v_pages, block_table, start, cos_table, sin_table,
-                       *(t for t in (q, cu_seqlens, q_norm, k_norm) if t is not None))
-    q_out = torch.empty(T, nq, hd, dtype=torch.float16, device=dev) if q is not None else None
-    k_out = torch.empty(T, nkv, hd, dtype=torch.float16, device=dev) if return_k else None
+            norms[i] = t.data_ptr()
+            if not t.is_cuda or t.dtype != _F16 or t.numel() != hd or not t.is_contiguous() or norms[i] % 16:
+                _fail(name, "(", ("q_norm", "k_norm")[i], "): must be a float16 CUDA tensor [head_dim], 16-byte aligned")
+    for t in (q, v, cos_table, sin_table, q_norm, k_norm):
+        if t is not None and t.get_device() != dev:
+            _fail(name, ": all tensors must be on the same CUDA device")
+    if q is not None:
+        q_out = k.new_empty((T, nq, hd))
+    if return_k:
+        k_out = k.new_empty((T, nkv, hd))
     if T == 0:
         return q_out, k_out
-    with torch.cuda.device(dev):
-        _call("soinfer_paged_kv_append", ctypes.byref(cache), ctypes.byref(rq) if rq is not None else None,
-              ctypes.byref(rk), ctypes.byref(rv), _ptr(q_out), _ptr(k_out), T, nq, B, _ptr(cu_seqlens), _ptr(start),
-              _ptr(cos_table), _ptr(sin_table), cos_table.size(0), _ptr(q_norm), _ptr(k_norm), float(eps), _stream(dev))
+    _call_on(dev, "soinfer_paged_kv_append", cache, rq, rk, rv, q_out.data_ptr() if nq else None,
+             k_out.data_ptr() if return_k else None, T, nq, B, cu_at, start_at, cos_table.data_ptr(), sin_table.data_ptr(),
+             rows, norms[0], norms[1], eps)
     return q_out, k_out
 
 
 def paged_kv_read(k_pages, v_pages, block_table, cu_seqlens, total: int, out=None):
     name = "paged_kv_read"
-    cache = _paged_cache(name, k_pages, v_pages, block_table)
+    dev = k_pages.get_device()
+    cache, nkv, hd = _paged_cache(name, k_pages, v_pages, block_table, dev)
     B = block_table.size(0)
-    _int32(name, "cu_seqlens", cu_seqlens, B + 1)
-    _check(total >= 0, name, ": total must be >= 0")
-    dev = _same_device(k_pages, v_pages, block_table, cu_seqlens)
-    shape = (total, cache.num_kv_heads, cache.head_dim)
-    ko, vo = (_out_rows(name, t, shape, dev) for t in (out if out is not None else (None, None)))
-    _same_device(k_pages, ko, vo)
-    if total == 0:
-        return ko, vo
-    with torch.cuda.device(dev):
-        _call("soinfer_paged_kv_read", ctypes.byref(cache), _ptr(cu_seqlens), B, total, _ptr(ko), _ptr(vo), _stream(dev))
+    cu_at = _int32(name, "cu_seqlens", cu_seqlens, B + 1, dev)
+    if total < 0:
+        _fail(name, ": total must be >= 0")
+    ko, vo = (_out_rows(name, t, k_pages, (total, nkv, hd)) for t in (out if out is not None else (None, None)))
+    if total:
+        _call_on(dev, "soinfer_paged_kv_read", cache, cu_at, B, total, ko.data_ptr(), vo.data_ptr())
     return ko, vo
 
 
 def paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, out=None) -> torch.Tensor:
     name = "paged_decode_attention"
-    rq = _rows(name, "q", q)
-    B, nq, hd = q.shape
-    cache = _paged_cache(name, k_pages, v_pages, block_table, hd)
-    nkv = cache.num_kv_heads
-    _check(nq >= 1 and nq % nkv == 0, name, ": num_q_heads must be a multiple of num_kv_heads")
-    _check(block_table.size(0) == B, name, ": block_table must have one row per query")
-    _int32(name, "seq_lens", seq_lens, B)
-    dev = _same_device(q, k_pages, v_pages, block_table, seq_lens)
-    out = _out_rows(name, out, (B, nq, hd), dev)
-    _same_device(q, out)
-    if B == 0:
-        return out
-    with torch.cuda.device(dev):
+    rq, (B, nq, hd) = _rows(name, "q", q)
+    dev = q.get_device()
+    cache, nkv, _ = _paged_cache(name, k_pages, v_pages, block_table, dev, hd)
+    if nkv < 1 or nq < 1 or nq % nkv:
+        _fail(name, ": num_q_heads must be a multiple of num_kv_heads")
+    if block_table.size(0) != B:
+        _fail(name, ": block_table must have one row per query")
+    lens_at = _int32(name, "seq_lens", seq_lens, B, dev)
+    out = _out_rows(name, out, q, (B, nq, hd))
+    if B:
         # a workspace of the call's own: two captured graphs or streams never share one
-        ws = torch.empty(lib().soinfer_paged_decode_workspace_bytes(B, nq, nkv, hd), dtype=torch.uint8, device=dev)
-        _call("soinfer_paged_decode_attention", ctypes.byref(cache), ctypes.byref(rq), _ptr(out), B, nq, _ptr(seq_lens),
-              ws.data_ptr(), ws.numel(), _stream(dev))
+        nbytes = lib().soinfer_paged_decode_workspace_bytes(B, nq, nkv, hd)
+        ws = q.new_empty((nbytes // 2,))
+        _call_on(dev, "soinfer_paged_decode_attention", cache, rq, out.data_ptr(), B, nq, lens_at, ws.data_ptr(), nbytes)
     return out
 
 
 def prefill_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None) -> torch.Tensor:
     name = "prefill_attention"
-    # rows are loaded as boxes of a tensor map, which has no zero strides (an expanded dimension)
-    q, k, v = (t.contiguous() if t.dim() == 3 and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())) else t
-               for t in (q, k, v))
-    rq, rk, rv = _rows(name, "q", q), _rows(name, "k", k), _rows(name, "v", v)
-    Tq, nq, hd = q.shape
-    Tk, nkv = k.shape[:2]
-    _check(v.shape == k.shape and k.size(2) == hd, name, ": k / v must be [tokens, num_kv_heads, head_dim]")
-    _check(hd in PAGED_HEAD_DIMS, name, ": head_dim must be 64 or 128")
-    _check(nkv >= 1 and nq >= 1 and nq % nkv == 0, name, ": num_q_heads must be a multiple of num_kv_heads")
-    _check(cu_seqlens.dim() == 1 and cu_seqlens.size(0) >= 1, name, ": cu_seqlens must be [num_seqs + 1]")
-    n = cu_seqlens.size(0)
-    _int32(name, "cu_seqlens", cu_seqlens, n)
-    if cu_seqlens_k is None:
-        _check(Tk == Tq, name, ": without cu_seqlens_k, q and k must have the same tokens")
-        cu_seqlens_k = cu_seqlens
+    rq, (Tq, nq, hd) = _rows(name, "q", q)
+    rk, ks = _rows(name, "k", k)
+    rv, vs = _rows(name, "v", v)
+    Tk, nkv, _ = ks
+    if vs != ks or ks[2] != hd:
+        _fail(name, ": k / v must be [tokens, num_kv_heads, head_dim]")
+    if hd not in PAGED_HEAD_DIMS:
+        _fail(name, ": head_dim must be 64 or 128")
+    if nkv < 1 or nq < 1 or nq % nkv:
+        _fail(name, ": num_q_heads must be a multiple of num_kv_heads")
+    for x in (q, k, v):
+        # rows are loaded as boxes of a tensor map, which has no zero strides (an expanded dimension)
+        if 0 in x.stride() and any(n > 1 and st == 0 for n, st in zip(x.shape, x.stride())):
+            return prefill_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu_seqlens, cu_seqlens_k, out)
+    dev = q.get_device()
+    if k.get_device() != dev or v.get_device() != dev:
+        _fail(name, ": all tensors must be on the same CUDA device")
+    n = cu_seqlens.numel()
+    if n < 1:
+        _fail(name, "(cu_seqlens): must be [num_seqs + 1]")
+    cu_at = _int32(name, "cu_seqlens", cu_seqlens, n, dev)
+    if cu_seqlens_k is not None:
+        cu_k_at = _int32(name, "cu_seqlens_k", cu_seqlens_k, n, dev)
     else:
-        _int32(name, "cu_seqlens_k", cu_seqlens_k, n)
-    dev = _same_device(q, k, v, cu_seqlens, cu_seqlens_k)
-    out = _out_rows(name, out, (Tq, nq, hd), dev)
-    _same_device(q, out)
-    if Tq == 0:
-        return out
-    with torch.cuda.device(dev):
-        _call("soinfer_prefill_attention", ctypes.byref(rq), ctypes.byref(rk), ctypes.byref(rv), _ptr(out), Tq, Tk, n - 1,
-              _ptr(cu_seqlens), _ptr(cu_seqlens_k), nq, nkv, hd, _stream(dev))
+        cu_k_at = cu_at
+        if Tk != Tq:
+            _fail(name, ": without cu_seqlens_k, q and k must have the same tokens")
+    out = _out_rows(name, out, q, (Tq, nq, hd))
+    if Tq:
+        _call_on(dev, "soinfer_prefill_attention", rq, rk, rv, out.data_ptr(), Tq, Tk, n - 1, cu_at, cu_k_at, nq, nkv, hd)
     return out
 
 

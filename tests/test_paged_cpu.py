@@ -1,8 +1,6 @@
 """The paged-cache and prompt-attention entry points without a GPU: argument
 errors come back as status codes before anything is launched, sizes of the
 workspace, and the Python front end's checks on CPU tensors."""
-import ctypes
-
 import pytest
 import torch
 
@@ -16,11 +14,13 @@ def _cache(**kw):
     f = dict(k_pages=P, v_pages=P, block_table=P, table_stride=4, table_cols=4, num_pages=8, num_kv_heads=2, page_size=16,
              head_dim=128, bits=16)
     f.update(kw)
-    return ctypes.byref(_C._PagedCache(**f))
+    order = ("k_pages", "v_pages", "block_table", "table_stride", "table_cols", "num_pages", "num_kv_heads", "page_size",
+             "head_dim", "bits")
+    return _C._PAGED_CACHE.pack(*(f[n] or 0 for n in order))
 
 
 def _rows(data=P, token=1024, head=128):
-    return ctypes.byref(_C._Rows(data, token, head))
+    return _C._ROWS.pack(data or 0, token, head)
 
 
 def _err():
