@@ -33,12 +33,12 @@ GROUP = 32  # values of a key that share a scale
 
 
 def _ops():
-    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sparse-offload-infer_b200")
-    if at not in sys.path:
-        sys.path.insert(0, at)
-    from soinfer import ops
-
-    return ops
+    """The framework's operators, imported once as a program does."""
+    if "soinfer.ops" not in sys.modules:
+        root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+        sys.path.insert(0, os.path.join(root, "sparse-offload-infer_b200"))
+        import soinfer.ops  # noqa: F401
+    return sys.modules["soinfer.ops"]
 
 
 # ------------------------------------------------------------------ cases
