@@ -1021,9 +1021,9 @@ int soinfer_paged_kv_read(const soinfer_paged_cache* cache, const int32_t* cu_se
 }
 
 int64_t soinfer_paged_decode_workspace_bytes(int64_t num_seqs, int64_t num_q_heads, int64_t num_kv_heads,
-                                             int64_t head_dim) {
+                                             int64_t head_dim, int64_t max_positions) {
   if (num_seqs < 1 || num_q_heads < 1 || num_kv_heads < 1 || head_dim < 1 || num_q_heads % num_kv_heads) return 0;
-  return paged_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim);
+  return paged_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, max_positions);
 }
 
 int soinfer_paged_decode_attention(const soinfer_paged_cache* cache, const soinfer_rows* q, soinfer_half* out,
@@ -1038,9 +1038,10 @@ int soinfer_paged_decode_attention(const soinfer_paged_cache* cache, const soinf
   if (num_seqs == 0) return SOINFER_OK;
   if (int st = check_rows(name, "q", q)) return st;
   REQUIRE(out && seq_lens, "%s: null pointer", name);
-  REQUIRE(workspace && aligned(workspace, 16) &&
-              workspace_bytes >= paged_decode_workspace_bytes(num_seqs, num_q_heads, P.cache.nkv, P.cache.hd),
-          "%s: workspace too small or not 16-byte aligned", name);
+  const int64_t need = paged_decode_workspace_bytes(num_seqs, num_q_heads, P.cache.nkv, P.cache.hd,
+                                                    (int64_t)P.cache.table_cols << P.cache.page_shift);
+  REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need),
+          "%s: workspace too small or not 16-byte aligned (need %lld bytes)", name, (long long)need);
   P.q = as_half(q->data), P.q_token = q->token_stride, P.q_head = q->head_stride;
   P.out = as_half(out);
   P.seqs = (int)num_seqs;

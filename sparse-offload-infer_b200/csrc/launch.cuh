@@ -1,4 +1,4 @@
-// cudaLaunchKernelEx wrapper: optional thread-block cluster along y and
+// cudaLaunchKernelEx wrapper: optional thread-block cluster and
 // optional programmatic dependent launch (PDL).
 #pragma once
 
@@ -11,7 +11,7 @@ namespace soinfer {
 
 template <typename... KArgs, typename... Args>
 cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                      int cluster_y, bool pdl, Args&&... args) {
+                      dim3 cluster, bool pdl, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -19,11 +19,11 @@ cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sm
   cfg.stream = stream;
   cudaLaunchAttribute attrs[2];
   unsigned n = 0;
-  if (cluster_y > 1) {
+  if (cluster.x * cluster.y * cluster.z > 1) {
     attrs[n].id = cudaLaunchAttributeClusterDimension;
-    attrs[n].val.clusterDim.x = 1;
-    attrs[n].val.clusterDim.y = cluster_y;
-    attrs[n].val.clusterDim.z = 1;
+    attrs[n].val.clusterDim.x = cluster.x;
+    attrs[n].val.clusterDim.y = cluster.y;
+    attrs[n].val.clusterDim.z = cluster.z;
     ++n;
   }
   if (pdl) {
@@ -34,6 +34,13 @@ cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sm
   cfg.attrs = attrs;
   cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// The same with a cluster along y.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                      int cluster_y, bool pdl, Args&&... args) {
+  return launch_ex(kernel, grid, block, smem, stream, dim3(1, (unsigned)cluster_y, 1), pdl, std::forward<Args>(args)...);
 }
 
 // Raises Kernel's dynamic shared-memory limit to at least `bytes` on the

@@ -5,24 +5,28 @@
 // Memory bounds it: every cached row is read once and serves the query heads of its group.  Both products run on the
 // matrix instruction with the cached rows as its 16-row operand and up to 8 query heads as its 8 columns, so the work a
 // 4-bit value costs is its unpacking, not its dot products:
-//   scores:  16 positions x 16 values times 16 values x 8 heads.  4-bit codes enter as 72 + c (one LOP3 turns a nibble
-//            into the fp16 number 64 + (c + 8)), the product starts at -72 sum q, and the group's scale multiplies the
-//            fp32 result -- no code is rounded.
+//   scores:  16 positions x 16 values times 16 values x 8 heads.  One LOP3 turns a nibble into an fp16 number: half of the
+//            codes enter as 72 + c and the product starts at -72 sum q over their values, the others are freed of their
+//            1032 first (the integer and the fp16 pipe share the work).  The group's scale multiplies the fp32 result --
+//            no code is rounded.
 //   output:  16 values x 16 positions times 16 positions x 8 heads.  4-bit rows: the codes are exact fp16 numbers and a
 //            position's scale multiplies its probability.  The running maximum is taken over score + exponent of the
-//            scale, so that the product p * scale lies in (0, 1] whatever the scales are; it is lifted by 2^14 and rounded
-//            once to fp16 (11 bits, down to 2^-28 of the largest).  fp16 rows: the same with the scale 1.
+//            scale, so that the product p * scale lies in (0, 2^8] whatever the scales are; it is lifted by 2^7 and rounded
+//            once to fp16 (11 bits, down to 2^-21 of the largest).  fp16 rows: the same with the scale 1.
 // The softmax statistics and both sums are fp32.
 //
-// Work split: positions of all sequences together are cut into chunks of equal length, about as many as the GPU holds
-// CTAs, computed on the device from the lengths (no host read; a captured launch serves any lengths).  A CTA of four
-// warps takes a chunk of one sequence for one kv head and up to 8 of its query heads, each warp every fourth tile, and
-// joins the warps in shared memory.  A sequence cut into several chunks leaves (m, l, acc) per chunk in the workspace and
-// a second kernel joins them in order; one chunk is finished in place.
+// Work split, by the longest sequence the block table can name:
+//   up to kClusterMost positions: a sequence's kv head (and up to 8 of its query heads) is one cluster of eight CTAs, each
+//   an eighth of the positions; they join through distributed shared memory.  One launch, no workspace.
+//   beyond: positions of all sequences together are cut into chunks of equal length, about as many as the GPU holds CTAs,
+//   computed on the device from the lengths (no host read; a captured launch serves any lengths), one CTA each.  A
+//   sequence cut into several chunks leaves (m, l, acc) per chunk in the workspace and a second kernel joins them in
+//   order; a sequence of one chunk is finished in place.
+// A CTA has four warps, each with every fourth tile of the CTA's positions; they are joined in shared memory.
 //
-// Feeding: each warp has its own ring of three tiles in shared memory, filled by bulk copies (one per run of positions
-// inside a page: codes and scales of a small page are one piece) and waited for on a barrier per tile, so loads are two
-// tiles ahead and the registers hold only what is being multiplied.  Waits are bounded.
+// Feeding: each warp has its own ring of tiles in shared memory, filled by bulk copies (one per run of positions inside a
+// page: codes and scales of a small page are one piece) and waited for on a barrier per tile, so loads run ahead and the
+// registers hold only what is being multiplied.  Waits are bounded.
 #include "launch.cuh"
 #include "paged_cache.cuh"
 
@@ -31,20 +35,24 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStages = 3;
+constexpr int kCluster = 8;
+constexpr int64_t kClusterMost = 8192;
 constexpr int kCols = 8;          // query heads per CTA
 constexpr int kMostLen = 1 << 30;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLift = 14.f;     // factor 2^14 on the probabilities (it cancels)
+constexpr float kLazy = 8.f;      // the running maximum follows when exceeded by 2^8 (it moves in a few tiles, not in half)
+constexpr float kLift = 7.f;      // factor 2^7 on the probabilities (it cancels)
 constexpr uint64_t kTimeoutNs = 1000000000ull;
 
 __device__ int g_paged_error;
 
-// Positions a warp takes at a time, CTAs the GPU holds (shared memory: 4 per SM with 4-bit rows, 2 with fp16 rows).
+// Positions a warp takes at a time, tiles in its ring, CTAs that an SM holds (shared memory and registers).
 template <bool Q4>
 struct Plan {
-  static constexpr int kTile = Q4 ? 32 : 16;
-  static constexpr int kCtas = 148 * (Q4 ? 4 : 2);
+  static constexpr int kTile = Q4 ? 64 : 16;
+  static constexpr int kStages = Q4 ? 2 : 3;
+  static constexpr int kPerSm = Q4 ? 3 : 2;
+  static constexpr int kCtas = 148 * kPerSm;
   static constexpr int kMinChunk = kTile * kWarps;
 };
 template <int HD, bool Q4>
@@ -79,8 +87,8 @@ __device__ __forceinline__ int seq_len(const PagedDecodeParams& P, int b) {
   return n < 0 ? 0 : n > most ? most : n;
 }
 
-// Chunk length for the batch: a multiple of the smallest chunk that gives about as many chunks x head groups as the GPU
-// holds CTAs (warp-wide).
+// Chunk length for the batch: a multiple of the smallest chunk that gives at most as many chunks x head groups as the GPU
+// holds CTAs, where the sequences are fewer than that (warp-wide).
 template <bool Q4>
 __device__ __forceinline__ int chunk_len(const PagedDecodeParams& P, int units, int lane) {
   constexpr int kMin = Plan<Q4>::kMinChunk;
@@ -88,21 +96,19 @@ __device__ __forceinline__ int chunk_len(const PagedDecodeParams& P, int units, 
   for (int b = lane; b < P.seqs; b += 32) total += seq_len(P, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  const long long want = (total * units + Plan<Q4>::kCtas - 1) / Plan<Q4>::kCtas;
+  // every sequence's last chunk is a partial one: room for those keeps the launch in one wave
+  const int slots = (Plan<Q4>::kCtas + units - 1) / units;
+  const int rest = P.seqs < slots / 2 ? slots - P.seqs : (slots + 1) / 2;
+  const long long want = (total + rest - 1) / rest;
   const long long c = (want + kMin - 1) / kMin * kMin;
   return (int)(c < kMin ? kMin : c > kMostLen ? kMostLen : c);
 }
 
-__device__ __forceinline__ float half_of(uint32_t u, int i) {
-  return __half2float(__ushort_as_half((unsigned short)(u >> (16 * i))));
-}
-
-// A run of n positions of a tile in shared memory: 4 bits: K codes, K scales, V codes, V scales; fp16: K rows, V rows.
-template <int HD, bool Q4>
+// A run of N positions of a tile in shared memory: 4 bits: K codes, K scales, V codes, V scales; fp16: K rows, V rows.
+template <int HD, bool Q4, int N>
 struct Run {
   const uint8_t *k, *v;
-  int n;
-  __device__ __forceinline__ Run(const uint8_t* at, int n_) : k(at), v(at + n_ * (Q4 ? HD / 2 + HD / 16 : 2 * HD)), n(n_) {}
+  __device__ __forceinline__ explicit Run(const uint8_t* at) : k(at), v(at + N * (Q4 ? HD / 2 + HD / 16 : 2 * HD)) {}
 };
 
 template <int N>
@@ -119,34 +125,37 @@ __device__ __forceinline__ void lds_words(uint32_t* d, const uint8_t* p) {
 }
 
 // Scores of the 16 positions at slot0: D rows are positions g and g + 8, columns heads 2 t and 2 t + 1.
-template <int HD, bool Q4>
-__device__ __forceinline__ void scores(float s[4], const Run<HD, Q4>& R, int slot0, const uint32_t (*qf)[4],
+template <int HD, bool Q4, int N>
+__device__ __forceinline__ void scores(float s[4], const Run<HD, Q4, N>& R, int slot0, const uint32_t (*qf)[4],
                                        const float (*bias)[2], int g, int t) {
   constexpr int G = HD / 32;
   if constexpr (Q4) {
+    const half2 k1032 = __floats2half2_rn(1032.f, 1032.f);
     uint32_t k[2][G], ks[2][G / 2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int p = slot0 + g + 8 * r;
       lds_words<G>(k[r], R.k + p * (HD / 2) + t * (4 * G));
-      lds_words<G / 2>(ks[r], R.k + R.n * (HD / 2) + p * (2 * G));
+      lds_words<G / 2>(ks[r], R.k + N * (HD / 2) + p * (2 * G));
     }
 #pragma unroll
     for (int j = 0; j < G; ++j) {
       uint32_t x[2][4];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t w = k[r][j];  // nibble n at bits 4..7 and 20..23: fp16 64 + (c + 8)
-        x[r][0] = lop3_and_xor(w << 4, 0x00f000f0u, 0x54805480u);
+        // nibbles at bits 0..3: fp16 1024 + (c + 8), made c; at bits 4..7: fp16 64 + (c + 8), left with its 72
+        const uint32_t w = k[r][j], top = w >> 8;
+        x[r][0] = h2_as_u32(__hsub2(u32_as_h2(lop3_and_xor(w, 0x000f000fu, 0x64086408u)), k1032));
         x[r][1] = lop3_and_xor(w, 0x00f000f0u, 0x54805480u);
-        x[r][2] = lop3_and_xor(w >> 4, 0x00f000f0u, 0x54805480u);
-        x[r][3] = lop3_and_xor(w >> 8, 0x00f000f0u, 0x54805480u);
+        x[r][2] = h2_as_u32(__hsub2(u32_as_h2(lop3_and_xor(top, 0x000f000fu, 0x64086408u)), k1032));
+        x[r][3] = lop3_and_xor(top, 0x00f000f0u, 0x54805480u);
       }
       float d[4];
       const uint32_t a0[4] = {x[0][0], x[1][0], x[0][1], x[1][1]}, a1[4] = {x[0][2], x[1][2], x[0][3], x[1][3]};
       mma_from(d, a0, qf[j][0], qf[j][1], bias[j][0], bias[j][1]);
       mma_16816(d, a1, qf[j][2], qf[j][3]);
-      const float s0 = half_of(ks[0][j >> 1], j & 1), s1 = half_of(ks[1][j >> 1], j & 1);
+      const half2 h0 = u32_as_h2(ks[0][j >> 1]), h1 = u32_as_h2(ks[1][j >> 1]);
+      const float s0 = j & 1 ? __high2float(h0) : __low2float(h0), s1 = j & 1 ? __high2float(h1) : __low2float(h1);
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[e] = j == 0 ? d[e] * (e < 2 ? s0 : s1) : fmaf(d[e], e < 2 ? s0 : s1, s[e]);
     }
@@ -168,8 +177,8 @@ __device__ __forceinline__ void scores(float s[4], const Run<HD, Q4>& R, int slo
 
 // acc += V^T w.  w: weights of positions g, g + 8 (rows) for heads 2 t, 2 t + 1 (0 for positions that do not count);
 // n_valid positions of the 16 count: fp16 rows beyond them are taken as zeros.  acc[i] rows are values value_of(i, 0 / 1).
-template <int HD, bool Q4>
-__device__ __forceinline__ void accumulate(float (*acc)[4], const Run<HD, Q4>& R, int slot0, const float w[4], int n_valid,
+template <int HD, bool Q4, int N>
+__device__ __forceinline__ void accumulate(float (*acc)[4], const Run<HD, Q4, N>& R, int slot0, const float w[4], int n_valid,
                                            int g, int t) {
   uint32_t b[2];
 #pragma unroll
@@ -215,10 +224,43 @@ __device__ __forceinline__ int value_of(int i, int r, int g) {
   return Q4 ? g * (HD / 8) + 2 * i + r : 64 * (i >> 2) + 8 * g + 2 * (i & 3) + r;
 }
 
-template <int HD, bool Q4>
-__global__ void __launch_bounds__(kThreads, Q4 ? 4 : 2)
+// The four warps' sums of head h, value d.
+template <int HD>
+__device__ __forceinline__ void join_warps(const float* s_acc, const float (*s_m)[kCols], const float (*s_l)[kCols], int h,
+                                           int d, float& num, float& den, float& M) {
+  M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][h]);
+  num = den = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const float f = s_m[w][h] == -INFINITY ? 0.f : ex2(s_m[w][h] - M);
+    den = fmaf(f, s_l[w][h], den);
+    num = fmaf(f, s_acc[(w * kCols + h) * (HD + 4) + d], num);
+  }
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// The float at this CTA's shared-memory address p, in CTA `rank` of the cluster.
+__device__ __forceinline__ float cluster_read(const float* p, int rank) {
+  float v;
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}"
+               : "=f"(v)
+               : "r"(smem_u32(p)), "r"(rank)
+               : "memory");
+  return v;
+}
+
+// kRuns: a tile's runs (more than one where a page is smaller than a 4-bit tile).
+template <int HD, bool Q4, int kRuns, bool kJoined>
+__global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
     paged_decode_kernel(const PagedDecodeParams P, const int groups, const float scale_log2) {
   constexpr int G = HD / 32, kTile = Plan<Q4>::kTile, kSub = kTile / 16, kBytes = kTileBytes<HD, Q4>;
+  constexpr int kStages = Plan<Q4>::kStages;
+  constexpr int kMin = Plan<Q4>::kMinChunk, kRun = kTile / kRuns, kRunBytes = kBytes / kRuns;
   extern __shared__ __align__(128) uint8_t smem[];  // kWarps rings of kStages tiles, then the warps' results
   __shared__ uint64_t s_full[kWarps][kStages];
   __shared__ float s_m[kWarps][kCols], s_l[kWarps][kCols];
@@ -236,84 +278,88 @@ __global__ void __launch_bounds__(kThreads, Q4 ? 4 : 2)
   const PagedCache& C = P.cache;
   const int rep = P.nq / C.nkv, units = C.nkv * groups;
 
-  // which chunk of which sequence (every warp finds it for itself)
-  const int L = chunk_len<Q4>(P, units, lane);
-  int b = -1, len = 0, chunk = 0, count = 0;
-  for (int base = 0, before = 0; base < P.seqs; base += 32) {
-    const int i = base + lane;
-    const int n = i < P.seqs ? seq_len(P, i) : 0;
-    const int mine = i < P.seqs ? (n > L ? (n + L - 1) / L : 1) : 0;  // an empty sequence has one chunk: its zeros
-    int sum = mine;
+  int b = -1, len = 0, chunk = 0, count = 0, L;
+  if (kJoined) {
+    b = blockIdx.y;
+    chunk = blockIdx.z;  // the rank in the cluster
+    len = seq_len(P, b);
+    L = (len + kCluster * kMin - 1) / (kCluster * kMin) * kMin;
+  } else {
+    // which chunk of which sequence (every warp finds it for itself)
+    L = chunk_len<Q4>(P, units, lane);
+    for (int base = 0, before = 0; base < P.seqs; base += 32) {
+      const int i = base + lane;
+      const int n = i < P.seqs ? seq_len(P, i) : 0;
+      const int mine = i < P.seqs ? (n > L ? (n + L - 1) / L : 1) : 0;  // an empty sequence has one chunk: its zeros
+      int sum = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+      }
+      const int c = (int)blockIdx.y - before;
+      const unsigned owns = __ballot_sync(0xffffffffu, c >= sum - mine && c < sum);
+      if (owns) {
+        const int src = __ffs(owns) - 1;
+        b = base + src;
+        len = __shfl_sync(0xffffffffu, n, src);
+        count = __shfl_sync(0xffffffffu, mine, src);
+        chunk = c - __shfl_sync(0xffffffffu, sum - mine, src);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    const int c = (int)blockIdx.y - before;
-    const unsigned owns = __ballot_sync(0xffffffffu, c >= sum - mine && c < sum);
-    if (owns) {
-      const int src = __ffs(owns) - 1;
-      b = base + src;
-      len = __shfl_sync(0xffffffffu, n, src);
-      count = __shfl_sync(0xffffffffu, mine, src);
-      chunk = c - __shfl_sync(0xffffffffu, sum - mine, src);
-      break;
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
+    if (b < 0) return;
   }
-  if (b < 0) return;
   const int kvh = blockIdx.x / groups, h0 = (blockIdx.x - kvh * groups) * kCols;
   const int heads = rep - h0 < kCols ? rep - h0 : kCols;
   const int qh0 = kvh * rep + h0;
   const int p_begin = chunk * L, p_end = len - p_begin < L ? len : p_begin + L;
 
-  // the ring: tile i of this warp starts at position p_begin + (warp + i kWarps) kTile and consists of kTile / n runs of
-  // n = min(page, kTile) positions; lane c of the first lanes copies piece c % pieces of run c / pieces
-  const int page = 1 << C.page_shift, n = page < kTile ? page : kTile, runs = kTile / n;
-  const bool whole = !Q4 || n == page;             // K (V) codes and scales of the run are one piece
-  const int pieces = whole ? 2 : 4, run = lane / pieces, piece = lane - run * pieces;
-  const int run_bytes = kBytes / runs;
-  const int64_t k_block = k_block_bytes(page, HD, Q4), v_block = v_block_bytes(page, HD, Q4);
+  // the ring: tile i of this warp starts at position p_begin + (warp + i kWarps) kTile and consists of runs of positions
+  // inside a page; lane c of the first lanes copies piece c % pieces of run c / pieces
+  const int page = 1 << C.page_shift;
+  const bool whole = !Q4 || kRun == page;          // K (V) codes and scales of the run are one piece
+  const int pieces = whole ? 2 : 4, run = whole ? lane >> 1 : lane >> 2, piece = lane & (pieces - 1);
   const int p_warp = p_begin + warp * kTile, stride = kWarps * kTile;
   const int tiles = p_warp < p_end ? (p_end - p_warp + stride - 1) / stride : 0;
-  // what lane's piece is: its place in the run, its place in the (page, head) block, its size
-  int dst_off, src_off, src_step, bytes;
-  {
-    const int kb = n * (Q4 ? HD / 2 + HD / 16 : 2 * HD), kc = n * (HD / 2);
-    if (whole) {
-      dst_off = piece == 0 ? 0 : kb;
-      src_off = 0;
-      src_step = Q4 ? 0 : 2 * HD;                  // bytes per slot; a whole 4-bit page starts at its block
-      bytes = piece == 0 ? kb : run_bytes - kb;
-    } else {
-      const bool scales = piece & 2;
-      const int row = scales ? (piece & 1 ? 2 : HD / 16) : HD / 2;
-      dst_off = (piece & 1 ? kb : 0) + (scales ? kc : 0);
-      src_off = scales ? page * (HD / 2) : 0;
-      src_step = row;
-      bytes = n * row;
+  // what this lane copies: from where in its page's block (bytes per slot), to where in the tile, how much
+  constexpr int kKeys = kRun * (Q4 ? HD / 2 + HD / 16 : 2 * HD), kCodes = kRun * (HD / 2);
+  int dst = run * kRunBytes + (piece & 1 ? kKeys : 0), src_step = Q4 ? 0 : 2 * HD;
+  int bytes = piece & 1 ? kRunBytes - kKeys : kKeys;
+  const uint8_t* src = piece & 1 ? C.v : C.k;
+  const int64_t block = piece & 1 ? v_block_bytes(page, HD, Q4) : k_block_bytes(page, HD, Q4);
+  if (!whole) {
+    src_step = piece < 2 ? HD / 2 : piece == 2 ? HD / 16 : 2;
+    bytes = kRun * src_step;
+    if (piece & 2) {
+      dst += kCodes;
+      src += page * (HD / 2);
     }
   }
-  const uint8_t* pool = piece & 1 ? C.v : C.k;
-  const int64_t block = piece & 1 ? v_block : k_block;
+  src += kvh * block;
+  dst += (int)smem_u32(ring);
+  const int p_lane = p_warp + run * kRun;
+  const bool copies = run < kRuns;
   auto page_id = [&](int i) {                      // page of this lane's run of tile i
-    const int p = p_warp + i * stride + run * n;
-    return run < runs && p < p_end ? page_of(C, b, p) : -1;
+    const int p = p_lane + i * stride;
+    return copies && p < p_end ? page_of(C, b, p) : -1;
   };
-  unsigned there = 0;                              // per ring slot, which runs hold data (2 bits)
+  unsigned there = 0;                              // per ring slot, which runs hold data
   auto issue = [&](int i, int slot, int id) {
-    const unsigned on = __ballot_sync(0xffffffffu, id >= 0 && piece == 0);
-    there &= ~(3u << (2 * slot));
-    unsigned bits = on & 1u;
-    if (runs > 1) bits |= (on >> pieces & 1u) << 1;
-    there |= bits << (2 * slot);
-    if (lane == 0) mbar_arrive_expect_tx(&full[slot], __popc(bits) * run_bytes);
+    const unsigned on = __ballot_sync(0xffffffffu, id >= 0);
+    unsigned bits = on & 1u;  // (several runs: always two pieces each)
+#pragma unroll
+    for (int r = 1; r < kRuns; ++r) bits |= (on >> (2 * r) & 1u) << r;
+    there = (there & ~(15u << (4 * slot))) | bits << (4 * slot);
+    if (lane == 0) mbar_arrive_expect_tx(&full[slot], __popc(bits) * kRunBytes);
     __syncwarp();
-    if (id >= 0) {
-      const int p = (p_warp + i * stride + run * n) & (page - 1);
-      bulk_g2s(ring + slot * kBytes + run * run_bytes + dst_off,
-               pool + ((int64_t)id * C.nkv + kvh) * block + src_off + p * src_step, bytes, &full[slot]);
-    }
+    if (id >= 0)
+      asm volatile(
+          "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + slot * kBytes),
+          "l"(src + (int64_t)id * C.nkv * block + ((p_lane + i * stride) & (page - 1)) * src_step), "r"(bytes),
+          "r"(smem_u32(&full[slot]))
+          : "memory");
   };
   {
     int id[kStages];
@@ -337,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, Q4 ? 4 : 2)
     if (Q4) {
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 1; i < 4; i += 2) {  // the values whose codes carry the 72
         const float2 f = __half22float2(u32_as_h2(qf[j][i]));
         sum += f.x + f.y;
       }
@@ -367,38 +413,36 @@ __global__ void __launch_bounds__(kThreads, Q4 ? 4 : 2)
       break;
     }
     const int p0 = p_warp + i * stride;
-    const unsigned held = there >> (2 * slot);
+    const unsigned held = there >> (4 * slot);
     const uint8_t* tile = ring + slot * kBytes;
-    const bool full_tile = p0 + kTile <= p_end && (held & ((1u << runs) - 1)) == (1u << runs) - 1;
+    const bool full_tile = p0 + kTile <= p_end && (held & ((1u << kRuns) - 1)) == (1u << kRuns) - 1;
     float s[kSub][4], sv[kSub][2];
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      const int at = 16 * u / n;
-      const Run<HD, Q4> R(tile + at * run_bytes, n);
-      const int slot0 = 16 * u - at * n;
+      const Run<HD, Q4, kRun> R(tile + 16 * u / kRun * kRunBytes);
+      const int slot0 = 16 * u % kRun;
       scores<HD, Q4>(s[u], R, slot0, qf, bias, g, t);
       if (Q4) {
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          sv[u][r] = __half2float(reinterpret_cast<const half*>(R.v + n * (HD / 2))[slot0 + g + 8 * r]);
+          sv[u][r] = __half2float(reinterpret_cast<const half*>(R.v + kRun * (HD / 2))[slot0 + g + 8 * r]);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[u][e] *= scale_log2;
       if (!full_tile) {
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          if (!(p0 + 16 * u + g + 8 * r < p_end && (held >> at & 1))) {
+          if (!(p0 + 16 * u + g + 8 * r < p_end && (held >> (16 * u / kRun) & 1))) {
             s[u][2 * r] = s[u][2 * r + 1] = -INFINITY;
             sv[u][r] = 1.f;
           }
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        // exponent of the scale, rounded up: scale * 2^-e < 1
-        const float e = Q4 ? (float)((int)(__float_as_uint(sv[u][r]) >> 23) - 126) : 0.f;
+        // exponent of the scale, rounded up: scale * 2^-e < 1 (an integer put into a float's mantissa)
+        float e = 0.f;
+        if (Q4) e = __uint_as_float(__float_as_uint(sv[u][r]) >> 23 | 0x4b000000u) - (8388608.f + 126.f);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], s[u][2 * r + c] + e);
+        for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], fmaf(s[u][2 * r + c], scale_log2, e));
       }
     }
 #pragma unroll
@@ -406,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, Q4 ? 4 : 2)
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
     }
-    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+    if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
       float f[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -423,15 +467,15 @@ __global__ void __launch_bounds__(kThreads, Q4 ? 4 : 2)
     const float shift[2] = {m[0] == -INFINITY ? 0.f : kLift - m[0], m[1] == -INFINITY ? 0.f : kLift - m[1]};
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      const int at = 16 * u / n;
-      const Run<HD, Q4> R(tile + at * run_bytes, n);
+      const Run<HD, Q4, kRun> R(tile + 16 * u / kRun * kRunBytes);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[u][e] = ex2(s[u][e] + shift[e & 1]);
+        s[u][e] = ex2(fmaf(s[u][e], scale_log2, shift[e & 1]));
         l[e & 1] += s[u][e];
         if (Q4) s[u][e] *= sv[u][e >> 1];
       }
-      accumulate<HD, Q4>(acc, R, 16 * u - at * n, s[u], (held >> at & 1) ? p_end - p0 - 16 * u : 0, g, t);
+      accumulate<HD, Q4>(acc, R, 16 * u % kRun, s[u], full_tile ? 16 : (held >> (16 * u / kRun) & 1) ? p_end - p0 - 16 * u : 0,
+                         g, t);
     }
     __syncwarp();  // every lane has read the tile
     if (i + kStages < tiles) {
@@ -461,34 +505,56 @@ __global__ void __launch_bounds__(kThreads, Q4 ? 4 : 2)
     for (int e = 0; e < 4; ++e)
       s_acc[(warp * kCols + 2 * t + (e & 1)) * kRow + value_of<HD, Q4>(i, e >> 1, g)] = acc[i][e];
   __syncthreads();
-  for (int e = threadIdx.x; e < heads * HD; e += kThreads) {
-    const int h = e / HD, d = e - h * HD;
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][h]);
-    float den = 0.f, num = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = s_m[w][h] == -INFINITY ? 0.f : ex2(s_m[w][h] - M);
-      den = fmaf(f, s_l[w][h], den);
-      num = fmaf(f, s_acc[(w * kCols + h) * kRow + d], num);
+  if constexpr (kJoined) {
+    // this CTA's sums, over the first warp's; then every CTA finishes an eighth of the cluster's values
+    for (int e = threadIdx.x; e < heads * HD; e += kThreads) {
+      const int h = e / HD, d = e - h * HD;
+      float num, den, M;
+      join_warps<HD>(s_acc, s_m, s_l, h, d, num, den, M);
+      s_acc[h * kRow + d] = num;
+      if (d == 0) s_acc[h * kRow + HD] = M, s_acc[h * kRow + HD + 1] = den;
     }
-    if (count == 1) {
+    cluster_sync();
+    for (int e = chunk * kThreads + threadIdx.x; e < heads * HD; e += kCluster * kThreads) {
+      const int h = e / HD, d = e - h * HD;
+      const float* row = s_acc + h * kRow;
+      float m8[kCluster], M = -INFINITY, num = 0.f, den = 0.f;
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r) M = fmaxf(M, m8[r] = cluster_read(row + HD, r));
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r) {
+        const float f = m8[r] == -INFINITY ? 0.f : ex2(m8[r] - M);
+        den = fmaf(f, cluster_read(row + HD + 1, r), den);
+        num = fmaf(f, cluster_read(row + d, r), num);
+      }
       P.out[((int64_t)b * P.nq + qh0 + h) * HD + d] = __float2half_rn(M == -INFINITY ? 0.f : num / den);
-    } else {
-      float* ws = P.ws + ((int64_t)blockIdx.y * P.nq + qh0 + h) * (HD + 2);
-      ws[d] = num;
-      if (d == 0) ws[HD] = M, ws[HD + 1] = den;
+    }
+    cluster_sync();  // nobody leaves while its sums are read
+  } else {
+    for (int e = threadIdx.x; e < heads * HD; e += kThreads) {
+      const int h = e / HD, d = e - h * HD;
+      float num, den, M;
+      join_warps<HD>(s_acc, s_m, s_l, h, d, num, den, M);
+      if (count == 1) {
+        P.out[((int64_t)b * P.nq + qh0 + h) * HD + d] = __float2half_rn(M == -INFINITY ? 0.f : num / den);
+      } else {
+        float* ws = P.ws + ((int64_t)blockIdx.y * P.nq + qh0 + h) * (HD + 2);
+        ws[d] = num;
+        if (d == 0) ws[HD] = M, ws[HD + 1] = den;
+      }
     }
   }
 }
 
-// Joins the chunks of a sequence that has several, in order; one CTA per (sequence, query head).
+// Joins the chunks of a sequence that has several; one CTA per (sequence, query head), in kParts parts of the chunks that
+// are summed in order.  A lane looks at every 32nd chunk's maximum and sum; the rows' loads do not wait for one another.
+constexpr int kParts = 4;
 template <int HD, bool Q4>
-__global__ void __launch_bounds__(HD) paged_join_kernel(const PagedDecodeParams P, const int units) {
+__global__ void __launch_bounds__(HD * kParts) paged_join_kernel(const PagedDecodeParams P, const int units) {
+  __shared__ float s_num[kParts][HD], s_den[kParts];
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 31;
+  const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 31, part = threadIdx.x / HD, d = threadIdx.x % HD;
   const int n = seq_len(P, b);
   const int L = chunk_len<Q4>(P, units, lane);
   if (n <= L) return;  // finished by its only chunk
@@ -499,19 +565,38 @@ __global__ void __launch_bounds__(HD) paged_join_kernel(const PagedDecodeParams 
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(0xffffffffu, first, o);
-  const int count = (n + L - 1) / L;
+  const int count = (n + L - 1) / L, each = (count + kParts - 1) / kParts;
   const float* ws = P.ws + ((int64_t)first * P.nq + h) * (HD + 2);
   const int64_t step = (int64_t)P.nq * (HD + 2);
   float M = -INFINITY;
-  for (int c = 0; c < count; ++c) M = fmaxf(M, ws[c * step + HD]);
+  for (int c = lane; c < count; c += 32) M = fmaxf(M, ws[c * step + HD]);
+  M = warp_max(M);
   float num = 0.f, den = 0.f;
-  for (int c = 0; c < count; ++c) {
-    const float mc = ws[c * step + HD];
-    const float f = mc == -INFINITY ? 0.f : ex2(mc - M);
-    den = fmaf(f, ws[c * step + HD + 1], den);
-    num = fmaf(f, ws[c * step + threadIdx.x], num);
+  const int end = (part + 1) * each < count ? (part + 1) * each : count;
+  for (int c0 = part * each; c0 < end; c0 += 32) {
+    const int c = c0 + lane;
+    float f = 0.f;
+    if (c < end) {
+      const float2 ml = *reinterpret_cast<const float2*>(ws + c * step + HD);
+      f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+      den = fmaf(f, ml.y, den);
+    }
+    const int rows = end - c0 < 32 ? end - c0 : 32;
+    const float* row = ws + c0 * step + d;
+#pragma unroll 8
+    for (int i = 0; i < rows; ++i) num = fmaf(__shfl_sync(0xffffffffu, f, i), row[i * step], num);
   }
-  P.out[((int64_t)b * P.nq + h) * HD + threadIdx.x] = __float2half_rn(M == -INFINITY ? 0.f : num / den);
+  den = warp_sum(den);
+  s_num[part][d] = num;
+  if (d == 0) s_den[part] = den;
+  __syncthreads();
+  if (part > 0) return;
+#pragma unroll
+  for (int i = 1; i < kParts; ++i) {
+    num += s_num[i][d];
+    den += s_den[i];
+  }
+  P.out[((int64_t)b * P.nq + h) * HD + d] = __float2half_rn(M == -INFINITY ? 0.f : num / den);
 }
 
 // Chunks of any lengths: sum over sequences of max(1, ceil(len / L)) with L >= total * units / CTAs.
@@ -520,33 +605,53 @@ int64_t most_chunks(int64_t seqs, int64_t units, bool q4) {
   return seqs + (ctas + units - 1) / units;
 }
 
+// Whether a cluster of CTAs takes a whole sequence (see the file comment).
+bool joined(int64_t table_cols, int page_shift) { return (table_cols << page_shift) <= kClusterMost; }
+
 int64_t head_groups(int64_t nq, int64_t nkv) { return (nq / nkv + kCols - 1) / kCols; }
 
-template <int HD, bool Q4>
-cudaError_t decode_hd(const PagedDecodeParams& P, cudaStream_t stream) {
+template <int HD, bool Q4, int kRuns>
+cudaError_t decode_runs(const PagedDecodeParams& P, cudaStream_t stream) {
   const int groups = (int)head_groups(P.nq, P.cache.nkv), units = P.cache.nkv * groups;
   const float scale_log2 = (1.0f / sqrtf((float)HD)) * kLog2e;
-  constexpr int kSmem = kWarps * kStages * kTileBytes<HD, Q4>;
-  cudaError_t e = ensure_smem_attr<paged_decode_kernel<HD, Q4>>(kSmem);
+  constexpr int kSmem = kWarps * Plan<Q4>::kStages * kTileBytes<HD, Q4>;
+  cudaError_t e;
+  if (joined(P.cache.table_cols, P.cache.page_shift)) {
+    if ((e = ensure_smem_attr<paged_decode_kernel<HD, Q4, kRuns, true>>(kSmem)) != cudaSuccess) return e;
+    return launch_ex(paged_decode_kernel<HD, Q4, kRuns, true>, dim3((unsigned)units, (unsigned)P.seqs, kCluster),
+                     dim3(kThreads), kSmem, stream, dim3(1, 1, kCluster), true, P, groups, scale_log2);
+  }
+  if ((e = ensure_smem_attr<paged_decode_kernel<HD, Q4, kRuns, false>>(kSmem)) != cudaSuccess) return e;
+  e = launch_ex(paged_decode_kernel<HD, Q4, kRuns, false>,
+                dim3((unsigned)units, (unsigned)most_chunks(P.seqs, units, Q4)), dim3(kThreads), kSmem, stream, 1, true, P,
+                groups, scale_log2);
   if (e != cudaSuccess) return e;
-  e = launch_ex(paged_decode_kernel<HD, Q4>, dim3((unsigned)units, (unsigned)most_chunks(P.seqs, units, Q4)),
-                dim3(kThreads), kSmem, stream, 1, true, P, groups, scale_log2);
-  if (e != cudaSuccess) return e;
-  // a table that holds no more than one chunk never splits
-  if (((int64_t)P.cache.table_cols << P.cache.page_shift) <= Plan<Q4>::kMinChunk) return cudaSuccess;
-  return launch_ex(paged_join_kernel<HD, Q4>, dim3((unsigned)P.nq, (unsigned)P.seqs), dim3(HD), 0, stream, 1, true, P,
-                   units);
+  return launch_ex(paged_join_kernel<HD, Q4>, dim3((unsigned)P.nq, (unsigned)P.seqs), dim3(HD * kParts), 0, stream, 1, true,
+                   P, units);
+}
+
+template <int HD>
+cudaError_t decode_hd(const PagedDecodeParams& P, cudaStream_t stream) {
+  if (!P.cache.q4) return decode_runs<HD, false, 1>(P, stream);
+  static_assert(Plan<true>::kTile == 64, "the runs of a tile below");
+  switch (P.cache.page_shift) {
+    case 4: return decode_runs<HD, true, 4>(P, stream);
+    case 5: return decode_runs<HD, true, 2>(P, stream);
+    default: return decode_runs<HD, true, 1>(P, stream);
+  }
 }
 
 }  // namespace
 
-int64_t paged_decode_workspace_bytes(int64_t seqs, int64_t nq, int64_t nkv, int64_t hd) {
-  return most_chunks(seqs, nkv * head_groups(nq, nkv), true) * nq * (hd + 2) * (int64_t)sizeof(float);
+int64_t paged_decode_workspace_bytes(int64_t seqs, int64_t nq, int64_t nkv, int64_t hd, int64_t positions) {
+  if (positions <= kClusterMost) return 0;
+  const int64_t units = nkv * head_groups(nq, nkv);
+  const int64_t a = most_chunks(seqs, units, true), b = most_chunks(seqs, units, false);
+  return (a > b ? a : b) * nq * (hd + 2) * (int64_t)sizeof(float);
 }
 
 cudaError_t launch_paged_decode(const PagedDecodeParams& P, cudaStream_t stream) {
-  if (P.cache.hd == 128) return P.cache.q4 ? decode_hd<128, true>(P, stream) : decode_hd<128, false>(P, stream);
-  return P.cache.q4 ? decode_hd<64, true>(P, stream) : decode_hd<64, false>(P, stream);
+  return P.cache.hd == 128 ? decode_hd<128>(P, stream) : decode_hd<64>(P, stream);
 }
 
 cudaError_t read_and_clear_paged_error(int* out) {

@@ -88,7 +88,7 @@ _SIGNATURES = {
     "soinfer_gemm_w4a16_batch": (_INT, [_P, _I64, _I64, _P, _I64, _P]),
     "soinfer_paged_kv_append": (_INT, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _F32, _P]),
     "soinfer_paged_kv_read": (_INT, [_P, _P, _I64, _I64, _P, _P, _P]),
-    "soinfer_paged_decode_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
+    "soinfer_paged_decode_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "soinfer_paged_decode_attention": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _I64, _P]),
     "soinfer_prefill_attention": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P]),
     "soinfer_tp_allreduce_add_rmsnorm": (_INT, [_P, _P, _P, _P, _P, _P, _I64, _F32, _P]),
@@ -1059,10 +1059,11 @@ def paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, out=None)
     lens_at = _int32(name, "seq_lens", seq_lens, B, dev)
     out = _out_rows(name, out, q, (B, nq, hd))
     if B:
+        nbytes = lib().soinfer_paged_decode_workspace_bytes(B, nq, nkv, hd, block_table.size(1) * k_pages.size(2))
         # a workspace of the call's own: two captured graphs or streams never share one
-        nbytes = lib().soinfer_paged_decode_workspace_bytes(B, nq, nkv, hd)
-        ws = q.new_empty((nbytes // 2,))
-        _call_on(dev, "soinfer_paged_decode_attention", cache, rq, out.data_ptr(), B, nq, lens_at, ws.data_ptr(), nbytes)
+        ws = q.new_empty((nbytes // 2,)) if nbytes else None
+        _call_on(dev, "soinfer_paged_decode_attention", cache, rq, out.data_ptr(), B, nq, lens_at,
+                 ws.data_ptr() if nbytes else None, nbytes)
     return out
 
 

@@ -75,11 +75,13 @@ def test_read_decode_and_prefill_arguments():
     assert lib.soinfer_paged_kv_read(_cache(), None, 1, 1, P, P, None) == 1 and "null" in _err()
     assert lib.soinfer_paged_kv_read(_cache(), P, 1, 1, P + 2, P, None) == 1 and "16-byte" in _err()
     assert lib.soinfer_paged_kv_read(_cache(), P, 1, 0, None, None, None) == 0
-    need = lib.soinfer_paged_decode_workspace_bytes(3, 8, 2, 128)
-    assert need >= 3 * 8 * 130 * 4 and lib.soinfer_paged_decode_workspace_bytes(3, 7, 2, 128) == 0
+    need = lib.soinfer_paged_decode_workspace_bytes(3, 8, 2, 128, 100_000)
+    assert need >= 3 * 8 * 130 * 4 and lib.soinfer_paged_decode_workspace_bytes(3, 7, 2, 128, 100_000) == 0
+    assert lib.soinfer_paged_decode_workspace_bytes(3, 8, 2, 128, 64) == 0
     d = lib.soinfer_paged_decode_attention
-    assert d(_cache(), _rows(), P, 3, 8, P, P, need - 1, None) == 1 and "workspace" in _err()
-    assert d(_cache(), _rows(), P, 3, 8, P, None, need, None) == 1 and "workspace" in _err()
+    long = dict(table_cols=10_000, table_stride=10_000)
+    assert d(_cache(**long), _rows(), P, 3, 8, P, P, need - 1, None) == 1 and "workspace" in _err()
+    assert d(_cache(**long), _rows(), P, 3, 8, P, None, need, None) == 1 and "workspace" in _err()
     assert d(_cache(), _rows(), P, 3, 7, P, P, need, None) == 1 and "multiple of num_kv_heads" in _err()
     assert d(_cache(), _rows(), P, 40000, 8, P, P, 1 << 40, None) == 1 and "num_seqs" in _err()
     assert d(_cache(), _rows(), None, 3, 8, P, P, need, None) == 1 and "null" in _err()

@@ -256,6 +256,24 @@ def test_decode_attention(lens, page, nq, nkv, hd, bits):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("lens,page,nq,nkv,hd", [([3000, 0, 17, 12000], 16, 5, 1, 64), ([1], 64, 4, 2, 128),
+                                                 ([255, 256, 257, 513, 70], 32, 12, 1, 128),
+                                                 ([40] * 40 + [2000], 128, 2, 1, 64), ([20011], 64, 8, 1, 128)])
+def test_decode_attention_with_wide_tables(lens, page, nq, nkv, hd, bits):
+    """Tables that can name long sequences: positions cut into chunks over the GPU, joined afterwards."""
+    T, g = sum(lens), _gen(len(lens) + bits)
+    table, pages = _table(lens, page, T, cols=max(9000, max(lens) + 500) // page)
+    pools = _pools(pages, nkv, page, hd, bits)
+    q = torch.randn(len(lens), nq, hd, generator=g).half().to(DEV)
+    k, v = (torch.randn(T, nkv, hd, generator=g).half().to(DEV) for _ in range(2))
+    one, zero = torch.ones(max(lens), hd // 2, device=DEV), torch.zeros(max(lens), hd // 2, device=DEV)
+    start = torch.zeros(len(lens), dtype=torch.int32, device=DEV)
+    ops.paged_kv_append(None, k, v, *pools, table.to(DEV), start, one, zero, cu_seqlens=_cum(lens))
+    got = ops.paged_decode_attention(q, *pools, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV))
+    _check_decode(got, q, pools, bits, table, lens, pages)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
 def test_decode_attention_over_missing_pages_and_odd_lengths(bits):
     """Pages that are not there are skipped; lengths below zero and beyond the table are cut."""
     lens, page, nq, nkv, hd = [700, 64, 90, 33], 32, 4, 2, 128
