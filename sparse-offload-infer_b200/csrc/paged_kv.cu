@@ -1,15 +1,13 @@
 // Appending rotated keys and values to a paged cache, and reading cached rows back.
 //
-// Both move rows of hd fp16 values once: what bounds them is memory (a prompt) or the launch (one token).  A row is
-// hd/8 lanes x 16 bytes, so a warp holds 256/hd rows; it works on one token, whose position, page, cosines and sines it
-// looks up once, and has up to four row loads in flight per lane.
+// Both move rows of hd fp16 values once: what bounds them is memory (a prompt) or the launch (one token).
 #include "launch.cuh"
 #include "paged_cache.cuh"
 
 namespace soinfer {
 namespace {
 
-constexpr int kWarps = 8;  // warps per CTA
+constexpr int kWarps = 4;  // warps per CTA
 
 __device__ __forceinline__ void unpack8(const uint4& u, float x[8]) {
   const half2* p = reinterpret_cast<const half2*>(&u);
@@ -29,75 +27,96 @@ __device__ __forceinline__ uint4 pack8(const float x[8]) {
   return u;
 }
 
-// Stores this lane's 8 keys (values 8 l .. 8 l + 7) of one position; all lanes of the row take part.
-template <int HD>
-__device__ __forceinline__ void store_key_q4(uint8_t* block, int page, int slot, int l, bool on, const float x[8]) {
-  float a = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) a = amax_nan(a, x[i]);
-  a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));  // the 4 lanes of a 32-value group
-  a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
-  const half sh = scale_of(a);
-  const float s = __half2float(sh);
+// Word of 8 codes in key order (value 2 i in nibble i, 2 i + 1 in nibble i + 4).
+__device__ __forceinline__ uint32_t key_word(const float x[8], float s) {
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) w |= (uint32_t)(code_of(x[i], s) & 15) << (4 * ((i >> 1) + 4 * (i & 1)));
-  if (!on) return;
-  constexpr int G = HD / kKGroup;
-  const int j = l >> 2, t = l & 3;
-  *reinterpret_cast<uint32_t*>(block + (int64_t)slot * (HD / 2) + 4 * (t * G + j)) = w;
-  if (t == 0) reinterpret_cast<half*>(block + (int64_t)page * (HD / 2))[slot * G + j] = sh;
+  return w;
 }
 
-// Stores this lane's 8 values of one position.
-template <int HD>
-__device__ __forceinline__ void store_value_q4(uint8_t* block, int page, int slot, int l, bool on, const float x[8]) {
+__device__ __forceinline__ float amax8(const float x[8]) {
   float a = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) a = amax_nan(a, x[i]);
-#pragma unroll
-  for (int o = 1; o < HD / 8; o <<= 1) a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-  const half sh = scale_of(a);
-  const float s = __half2float(sh);
-  uint32_t w[2] = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i >> 2] |= (uint32_t)(code_of(x[i], s) & 15) << (4 * (i & 3));
-  if (!on) return;
-  uint8_t* at = block + (int64_t)(slot >> 1) * HD + 8 * l + 2 * (slot & 1);
-  *reinterpret_cast<uint16_t*>(at) = (uint16_t)w[0];
-  *reinterpret_cast<uint16_t*>(at + 4) = (uint16_t)w[1];
-  if (l == 0) reinterpret_cast<half*>(block + (int64_t)page * (HD / 2))[slot] = sh;
+  return a;
 }
 
-// A warp takes steps [s R, s R + R) of one token; a step is 256/HD rows of one kind (q heads, then k, then v).
+// Stores this lane's keys (x[half]: values half hd/2 + 8 l ..) of one position; the lanes of a row take part.
+template <int HD>
+__device__ __forceinline__ void store_key_q4(uint8_t* block, int page, int slot, int l, bool on, const float (*x)[8]) {
+  constexpr int G = HD / kKGroup;
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+    float a = amax8(x[f]);
+    a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));  // the 4 lanes of a 32-value group
+    a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
+    const half sh = scale_of(a);
+    const uint32_t w = key_word(x[f], __half2float(sh));
+    if (!on) continue;
+    const int j = f * (G / 2) + (l >> 2), t = l & 3;
+    *reinterpret_cast<uint32_t*>(block + (int64_t)slot * (HD / 2) + 4 * (t * G + j)) = w;
+    if (t == 0) reinterpret_cast<half*>(block + (int64_t)page * (HD / 2))[slot * G + j] = sh;
+  }
+}
+
+// Stores this lane's values of one position.
+template <int HD>
+__device__ __forceinline__ void store_value_q4(uint8_t* block, int page, int slot, int l, bool on, const float (*x)[8]) {
+  float a = amax_nan(amax8(x[0]), amax8(x[1]));
+#pragma unroll
+  for (int o = 1; o < HD / 16; o <<= 1) a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+  const half sh = scale_of(a);
+  const float s = __half2float(sh);
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i >> 2] |= (uint32_t)(code_of(x[f][i], s) & 15) << (4 * (i & 3));
+    if (!on) continue;
+    uint8_t* at = block + (int64_t)(slot >> 1) * HD + f * (HD / 2) + 8 * l + 2 * (slot & 1);
+    *reinterpret_cast<uint16_t*>(at) = (uint16_t)w[0];
+    *reinterpret_cast<uint16_t*>(at + 4) = (uint16_t)w[1];
+  }
+  if (on && l == 0) reinterpret_cast<half*>(block + (int64_t)page * (HD / 2))[slot] = sh;
+}
+
+// A warp takes `per` steps of one token; a step is 512/HD rows of one kind (q heads, then k, then v).  A row is hd/16
+// lanes, each with 8 values of the row's first half and the same 8 of its second, so that a rotation's pairs lie in one
+// lane; the token's position, page, cosines and sines are looked up once, and the next R steps' rows are on their way
+// while R are worked on.
 //   norm:   x^ = x / sqrt(mean x^2 + eps) * w    (optional; a key's sum in 64 bits: a code may lie next to a border, and
 //                                                 the 64-bit sum makes it the same whatever the order of the sum)
 //   rotate: y_i = x^_i c_i - x^_{i+h/2} s_i,  y_{i+h/2} = x^_{i+h/2} c_i + x^_i s_i
 // in fp32 with each operation rounded by itself, and one rounding to fp16 or to a code at the end.
 template <int HD, bool Q4, int R>
-__global__ void __launch_bounds__(32 * kWarps) paged_append_kernel(const PagedAppendParams P) {
-  constexpr int kLanes = HD / 8, kRows = 32 / kLanes;
+__global__ void __launch_bounds__(32 * kWarps) paged_append_kernel(const PagedAppendParams P, const int per) {
+  constexpr int kLanes = HD / 16, kRows = 32 / kLanes;
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, l = lane % kLanes, sub = lane / kLanes;
   const int q_steps = (P.nq + kRows - 1) / kRows, kv_steps = (P.nkv + kRows - 1) / kRows;
-  const int steps = q_steps + 2 * kv_steps, per_token = (steps + R - 1) / R;
+  const int steps = q_steps + 2 * kv_steps, parts = (steps + per - 1) / per;
   const int64_t warp = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (warp >= (int64_t)P.tokens * per_token) return;
-  const int t = (int)(warp / per_token), s0 = (int)(warp - (int64_t)t * per_token) * R;
+  if (warp >= (int64_t)P.tokens * parts) return;
+  const int t = (int)(warp / parts), s0 = (int)(warp - (int64_t)t * parts) * per;
+  const int s_end = s0 + per < steps ? s0 + per : steps;
 
-  // the rows first: their loads do not wait for the position
-  uint4 raw[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int s = s0 + r;
+  auto load = [&](int s, uint4 (&x)[2]) {
     const bool is_q = s < q_steps, is_k = !is_q && s < q_steps + kv_steps;
     const int h = (is_q ? s : is_k ? s - q_steps : s - q_steps - kv_steps) * kRows + sub;
     const half* src = is_q ? P.q + t * P.q_token + h * P.q_head
                            : is_k ? P.k + t * P.k_token + h * P.k_head : P.v + t * P.v_token + h * P.v_head;
-    raw[r] = make_uint4(0, 0, 0, 0);
-    if (s < steps && h < (is_q ? P.nq : P.nkv)) raw[r] = ldg_stream_u4(src + 8 * l);
-  }
+    x[0] = x[1] = make_uint4(0, 0, 0, 0);
+    if (s < s_end && h < (is_q ? P.nq : P.nkv)) {
+      x[0] = ldg_stream_u4(src + 8 * l);
+      x[1] = ldg_stream_u4(src + HD / 2 + 8 * l);
+    }
+  };
+  // the first rows before anything else: their loads do not wait for the position
+  uint4 raw[R][2];
+#pragma unroll
+  for (int r = 0; r < R; ++r) load(s0 + r, raw[r]);
 
   int b = t, at = 0;
   if (P.cu) {
@@ -111,13 +130,15 @@ __global__ void __launch_bounds__(32 * kWarps) paged_append_kernel(const PagedAp
   const bool placed = pos >= 0 && pos < P.table_rows;  // a token of no sequence, or beyond the tables: zeros, no row
   const int page = 1 << P.cache.page_shift;
   int id = -1;
-  if (placed && P.cache.k) id = page_of(P.cache, b, (int)pos);
+  if (placed) id = page_of(P.cache, b, (int)pos);
   const int slot = (int)pos & (page - 1);
+  const int64_t k_block = k_block_bytes(page, HD, Q4), v_block = v_block_bytes(page, HD, Q4);
+  uint8_t* k_base = P.cache.k + (int64_t)id * P.nkv * k_block;
+  uint8_t* v_base = P.cache.v + (int64_t)id * P.nkv * v_block;
 
-  float c[8], sn[8], wq[8], wk[8];
-  const bool first = l < kLanes / 2;
+  float c[8], sn[8];
   {
-    const int64_t row = (placed ? pos : 0) * (HD / 2) + 8 * (first ? l : l - kLanes / 2);
+    const int64_t row = (placed ? pos : 0) * (HD / 2) + 8 * l;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float4 a = __ldg(reinterpret_cast<const float4*>(P.cos_t + row) + i);
@@ -125,139 +146,214 @@ __global__ void __launch_bounds__(32 * kWarps) paged_append_kernel(const PagedAp
       c[4 * i] = a.x, c[4 * i + 1] = a.y, c[4 * i + 2] = a.z, c[4 * i + 3] = a.w;
       sn[4 * i] = e.x, sn[4 * i + 1] = e.y, sn[4 * i + 2] = e.z, sn[4 * i + 3] = e.w;
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sn[i] = first ? -sn[i] : sn[i];
-    if (P.q_norm) unpack8(__ldg(reinterpret_cast<const uint4*>(P.q_norm) + l), wq);
-    if (P.k_norm) unpack8(__ldg(reinterpret_cast<const uint4*>(P.k_norm) + l), wk);
   }
 
+  for (int s1 = s0; s1 < s_end; s1 += R) {
+    uint4 cur[R][2];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int s = s0 + r;
-    if (s >= steps) break;
-    const bool is_q = s < q_steps, is_k = !is_q && s < q_steps + kv_steps;
-    const int h = (is_q ? s : is_k ? s - q_steps : s - q_steps - kv_steps) * kRows + sub;
-    const bool on = h < (is_q ? P.nq : P.nkv);
-    const bool cached = on && id >= 0;
-    uint8_t* kb = nullptr;
-    uint8_t* vb = nullptr;
-    if (cached) {
-      kb = P.cache.k + ((int64_t)id * P.nkv + h) * k_block_bytes(page, HD, Q4);
-      vb = P.cache.v + ((int64_t)id * P.nkv + h) * v_block_bytes(page, HD, Q4);
-    }
-    if (!is_q && !is_k) {
+    for (int r = 0; r < R; ++r) cur[r][0] = raw[r][0], cur[r][1] = raw[r][1];
+    if (R > 1 && s1 + R < s_end)
+#pragma unroll
+      for (int r = 0; r < R; ++r) load(s1 + R + r, raw[r]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int s = s1 + r;
+      if (s >= s_end) break;
+      const bool is_q = s < q_steps, is_k = !is_q && s < q_steps + kv_steps;
+      const int h = (is_q ? s : is_k ? s - q_steps : s - q_steps - kv_steps) * kRows + sub;
+      const bool on = h < (is_q ? P.nq : P.nkv);
+      const bool cached = on && id >= 0;
+      float x[2][8];
+      unpack8(cur[r][0], x[0]);
+      unpack8(cur[r][1], x[1]);
+      if (!is_q && !is_k) {
+        uint8_t* vb = v_base + h * v_block;
+        if (Q4) {
+          store_value_q4<HD>(vb, page, slot, l, cached, x);
+        } else if (cached) {
+          uint4* dst = reinterpret_cast<uint4*>(vb) + (int64_t)slot * (HD / 8) + l;
+          dst[0] = cur[r][0];
+          dst[kLanes] = cur[r][1];
+        }
+        continue;
+      }
+      const half* w = is_q ? P.q_norm : P.k_norm;
+      if (w) {
+        float inv, wf[2][8];
+        unpack8(__ldg(reinterpret_cast<const uint4*>(w) + l), wf[0]);
+        unpack8(__ldg(reinterpret_cast<const uint4*>(w) + kLanes + l), wf[1]);
+        if (is_q) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], ss));
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          inv = rsqrtf(ss / (float)HD + P.eps);
+        } else {
+          double ss = 0.0;  // the squares are exact in fp32
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss += (double)__fmul_rn(x[0][i], x[0][i]) + (double)__fmul_rn(x[1][i], x[1][i]);
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          inv = (float)(1.0 / sqrt(ss / (double)HD + (double)P.eps));
+        }
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[f][i] = __fmul_rn(__fmul_rn(x[f][i], inv), wf[f][i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float a = x[0][i], e = x[1][i];
+        x[0][i] = placed ? __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(e, sn[i])) : 0.f;
+        x[1][i] = placed ? __fadd_rn(__fmul_rn(e, c[i]), __fmul_rn(a, sn[i])) : 0.f;
+      }
+      const uint4 lo = pack8(x[0]), hi = pack8(x[1]);
+      half* out = is_q ? P.q_out + ((int64_t)t * P.nq + h) * HD : P.k_out + ((int64_t)t * P.nkv + h) * HD;
+      if (on && (is_q || P.k_out)) {
+        reinterpret_cast<uint4*>(out)[l] = lo;
+        reinterpret_cast<uint4*>(out)[kLanes + l] = hi;
+      }
+      if (is_q) continue;
+      uint8_t* kb = k_base + h * k_block;
       if (Q4) {
-        float x[8];
-        unpack8(raw[r], x);
-        store_value_q4<HD>(vb, page, slot, l, cached, x);
+        store_key_q4<HD>(kb, page, slot, l, cached, x);
       } else if (cached) {
-        reinterpret_cast<uint4*>(vb)[(int64_t)slot * kLanes + l] = raw[r];
+        uint4* dst = reinterpret_cast<uint4*>(kb) + (int64_t)slot * (HD / 8) + l;
+        dst[0] = lo;
+        dst[kLanes] = hi;
       }
-      continue;
     }
-    float x[8], y[8];
-    unpack8(raw[r], x);
-    if (is_q ? P.q_norm != nullptr : P.k_norm != nullptr) {
-      float inv;
-      if (is_q) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        inv = rsqrtf(ss / (float)HD + P.eps);
-      } else {
-        double ss = 0.0;  // the squares are exact in fp32
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += (double)__fmul_rn(x[i], x[i]);
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        inv = (float)(1.0 / sqrt(ss / (double)HD + (double)P.eps));
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], inv), is_q ? wq[i] : wk[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float o = __shfl_xor_sync(0xffffffffu, x[i], kLanes / 2);
-      y[i] = placed ? __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(o, sn[i])) : 0.f;
-    }
-    if (is_q) {
-      if (on) *reinterpret_cast<uint4*>(P.q_out + ((int64_t)t * P.nq + h) * HD + 8 * l) = pack8(y);
-      continue;
-    }
-    const uint4 packed = pack8(y);
-    if (on && P.k_out) *reinterpret_cast<uint4*>(P.k_out + ((int64_t)t * P.nkv + h) * HD + 8 * l) = packed;
-    if (Q4)
-      store_key_q4<HD>(kb, page, slot, l, cached, y);
-    else if (cached)
-      reinterpret_cast<uint4*>(kb)[(int64_t)slot * kLanes + l] = packed;
   }
 }
 
-// A warp reads one position's rows of every kv head, keys then values.
+// Reads two packed rows t, t + 1 (mostly positions 2 m, 2 m + 1 of one sequence, which share their 4-bit values' words).
+// fp16: hd/8 lanes copy a row.  4 bits: 8 lanes take a kv head at a pair of positions: 4 lanes a position's key codes,
+// all of them the pair's values (hd = 64: half as many bytes each).  Every lane reads 16 + 16 bytes of codes and writes 128.
 template <int HD, bool Q4>
 __global__ void __launch_bounds__(32 * kWarps)
     paged_read_kernel(const PagedCache C, const int32_t* __restrict__ cu, const int seqs, const int tokens,
                       half* __restrict__ k_out, half* __restrict__ v_out) {
-  constexpr int kLanes = HD / 8, kRows = 32 / kLanes;
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, l = lane % kLanes, sub = lane / kLanes;
-  const int t = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (t >= tokens) return;
-  const int b = owner_of(cu, seqs, t, lane);
-  if (b >= seqs) return;  // behind the last sequence: left as it was
-  const int pos = t - __ldg(cu + b);
-  if (pos < 0) return;
-  const int page = 1 << C.page_shift, slot = pos & (page - 1);
-  const int id = page_of(C, b, pos);
+  const int lane = threadIdx.x & 31;
+  const int t0 = 2 * (blockIdx.x * kWarps + (threadIdx.x >> 5));
+  if (t0 >= tokens) return;
+  const int page = 1 << C.page_shift;
   const int64_t kbb = k_block_bytes(page, HD, Q4), vbb = v_block_bytes(page, HD, Q4);
+  int b = owner_of(cu, seqs, t0, lane);
+  for (int t = t0, n; t < t0 + 2 && t < tokens; t += n) {
+    n = 1;
+    if (t > t0) b = owner_of(cu, seqs, t, lane);
+    if (b >= seqs) return;  // behind the last sequence: left as it was
+    const int pos = t - __ldg(cu + b);
+    if (pos < 0) continue;
+    if (t == t0 && !(pos & 1) && t + 1 < tokens && t + 1 < __ldg(cu + b + 1)) n = 2;
+    const int slot = pos & (page - 1), id = page_of(C, b, pos);
+    const uint8_t* k_base = C.k + (int64_t)id * C.nkv * kbb;
+    const uint8_t* v_base = C.v + (int64_t)id * C.nkv * vbb;
+    if constexpr (!Q4) {
+      constexpr int kLanes = HD / 8, kRows = 32 / kLanes;
+      const int l = lane % kLanes;
+      for (int r = 0; r < n; ++r)
 #pragma unroll 4
-  for (int h = sub; h < C.nkv; h += kRows) {
-    uint4 ko = make_uint4(0, 0, 0, 0), vo = make_uint4(0, 0, 0, 0);
-    if (id >= 0) {
-      const uint8_t* kb = C.k + ((int64_t)id * C.nkv + h) * kbb;
-      const uint8_t* vb = C.v + ((int64_t)id * C.nkv + h) * vbb;
-      if (Q4) {
-        constexpr int G = HD / kKGroup;
-        const int j = l >> 2, tq = l & 3;
-        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(kb + (int64_t)slot * (HD / 2)) + tq * G + j);
-        const float ks = __half2float(reinterpret_cast<const half*>(kb + (int64_t)page * (HD / 2))[slot * G + j]);
-        const uint2 vw = __ldg(reinterpret_cast<const uint2*>(vb + (int64_t)(slot >> 1) * HD + 8 * l));
-        const float vs = __half2float(reinterpret_cast<const half*>(vb + (int64_t)page * (HD / 2))[slot]);
-        float kx[8], vx[8];
-        const int sh = 16 * (slot & 1);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int n = (w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15;
-          kx[i] = (float)((n ^ 8) - 8) * ks;
-          const int m = ((i < 4 ? vw.x : vw.y) >> (sh + 4 * (i & 3))) & 15;
-          vx[i] = (float)((m ^ 8) - 8) * vs;
+        for (int h = lane / kLanes; h < C.nkv; h += kRows) {
+          uint4 ko = make_uint4(0, 0, 0, 0), vo = ko;
+          if (id >= 0) {
+            ko = ldg_stream_u4(reinterpret_cast<const uint4*>(k_base + h * kbb) + (int64_t)(slot + r) * kLanes + l);
+            vo = ldg_stream_u4(reinterpret_cast<const uint4*>(v_base + h * vbb) + (int64_t)(slot + r) * kLanes + l);
+          }
+          const int64_t o = ((int64_t)(t + r) * C.nkv + h) * kLanes + l;
+          reinterpret_cast<uint4*>(k_out)[o] = ko;
+          reinterpret_cast<uint4*>(v_out)[o] = vo;
         }
-        ko = pack8(kx);
-        vo = pack8(vx);
-      } else {
-        ko = ldg_stream_u4(reinterpret_cast<const uint4*>(kb) + (int64_t)slot * kLanes + l);
-        vo = ldg_stream_u4(reinterpret_cast<const uint4*>(vb) + (int64_t)slot * kLanes + l);
+    } else {
+      constexpr int G = HD / kKGroup;
+      const int l = lane & 7, tq = l & 3, first = slot & 1;
+      const int kr = n == 2 ? l >> 2 : 0;  // which of the rows this lane's keys belong to
+#pragma unroll 2
+      for (int h = lane >> 3; h < C.nkv; h += 4) {
+        const bool keys = n == 2 || l < 4;
+        uint32_t kw[G], ks[G / 2], vw[G];
+        float vs[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < G; ++j) kw[j] = vw[j] = 0;
+#pragma unroll
+        for (int j = 0; j < G / 2; ++j) ks[j] = 0;
+        if (id >= 0) {
+          const uint8_t *kb = k_base + h * kbb, *vb = v_base + h * vbb;
+          const uint32_t* kc = reinterpret_cast<const uint32_t*>(kb + (int64_t)(slot + kr) * (HD / 2)) + tq * G;
+          const uint32_t* kg = reinterpret_cast<const uint32_t*>(kb + (int64_t)page * (HD / 2) + (slot + kr) * (2 * G));
+          const uint32_t* vc = reinterpret_cast<const uint32_t*>(vb + (int64_t)(slot >> 1) * HD) + l * G;
+          if constexpr (G == 4) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(kc)), e = __ldg(reinterpret_cast<const uint4*>(vc));
+            const uint2 f = __ldg(reinterpret_cast<const uint2*>(kg));
+            kw[0] = a.x, kw[1] = a.y, kw[2] = a.z, kw[3] = a.w, vw[0] = e.x, vw[1] = e.y, vw[2] = e.z, vw[3] = e.w;
+            ks[0] = f.x, ks[1] = f.y;
+          } else {
+            const uint2 a = __ldg(reinterpret_cast<const uint2*>(kc)), e = __ldg(reinterpret_cast<const uint2*>(vc));
+            kw[0] = a.x, kw[1] = a.y, vw[0] = e.x, vw[1] = e.y;
+            ks[0] = __ldg(kg);
+          }
+          const half2 v2 = u32_as_h2(__ldg(reinterpret_cast<const uint32_t*>(vb + (int64_t)page * (HD / 2)) + (slot >> 1)));
+          vs[0] = __low2float(v2), vs[1] = __high2float(v2);
+        }
+        uint4* ko = reinterpret_cast<uint4*>(k_out + ((int64_t)(t + kr) * C.nkv + h) * HD);
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          const half2 sc = u32_as_h2(ks[j >> 1]);
+          const float s = j & 1 ? __high2float(sc) : __low2float(sc);
+          uint32_t u[4];
+          unpack_int4x8(kw[j], u);
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(u32_as_h2(u[i]));
+            x[2 * i] = f.x * s;
+            x[2 * i + 1] = f.y * s;
+          }
+          if (keys) ko[4 * j + tq] = pack8(x);
+        }
+        // words 4 values x 2 positions: the low halves of the unpacked pairs are the even position's
+        float x[2][4 * G];
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          uint32_t u[4];
+          unpack_int4x8(vw[j], u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(u32_as_h2(u[i]));
+            x[0][4 * j + i] = f.x * vs[0];
+            x[1][4 * j + i] = f.y * vs[1];
+          }
+        }
+        for (int r = 0; r < n; ++r) {
+          uint4* vo = reinterpret_cast<uint4*>(v_out + ((int64_t)(t + r) * C.nkv + h) * HD) + l * (G / 2);
+          const bool odd = first + r;
+#pragma unroll
+          for (int j = 0; j < G / 2; ++j) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = odd ? x[1][8 * j + i] : x[0][8 * j + i];
+            vo[j] = pack8(y);
+          }
+        }
       }
     }
-    const int64_t o = ((int64_t)t * C.nkv + h) * kLanes + l;
-    reinterpret_cast<uint4*>(k_out)[o] = ko;
-    reinterpret_cast<uint4*>(v_out)[o] = vo;
   }
 }
 
 template <int HD, bool Q4>
 cudaError_t append_hd(const PagedAppendParams& P, cudaStream_t stream) {
-  constexpr int kRows = 256 / HD;
+  constexpr int kRows = 512 / HD;
   const int steps = (P.nq + kRows - 1) / kRows + 2 * ((P.nkv + kRows - 1) / kRows);
-  // few tokens: one step per warp, for latency; many: four, so that a warp's look-ups serve more rows
-  const bool wide = (int64_t)P.tokens * steps >= 148 * 64;
-  const int per_token = wide ? (steps + 3) / 4 : steps;
-  const unsigned ctas = (unsigned)(((int64_t)P.tokens * per_token + kWarps - 1) / kWarps);
-  return launch_ex(wide ? paged_append_kernel<HD, Q4, 4> : paged_append_kernel<HD, Q4, 1>, dim3(ctas),
-                   dim3(32 * kWarps), 0, stream, 1, true, P);
+  // as many steps per warp as still leave the GPU full of warps: a warp's look-ups then serve more rows
+  const int64_t all = (int64_t)P.tokens * steps;
+  int per = (int)(all / (148 * 32));
+  per = per < 1 ? 1 : per > steps ? steps : per;
+  const int64_t warps = (int64_t)P.tokens * ((steps + per - 1) / per);
+  return launch_ex(per > 1 ? paged_append_kernel<HD, Q4, 2> : paged_append_kernel<HD, Q4, 1>,
+                   dim3((unsigned)((warps + kWarps - 1) / kWarps)), dim3(32 * kWarps), 0, stream, 1, true, P, per);
 }
 
 }  // namespace
@@ -269,7 +365,7 @@ cudaError_t launch_paged_append(const PagedAppendParams& P, cudaStream_t stream)
 
 cudaError_t launch_paged_read(const PagedCache& C, const int32_t* cu, int seqs, int tokens, half* k_out, half* v_out,
                               cudaStream_t stream) {
-  const dim3 grid((unsigned)((tokens + kWarps - 1) / kWarps)), block(32 * kWarps);
+  const dim3 grid((unsigned)((tokens + 2 * kWarps - 1) / (2 * kWarps))), block(32 * kWarps);
   if (C.hd == 128)
     return launch_ex(C.q4 ? paged_read_kernel<128, true> : paged_read_kernel<128, false>, grid, block, 0, stream, 1,
                      true, C, cu, seqs, tokens, k_out, v_out);
