@@ -39,16 +39,29 @@ __device__ __forceinline__ int page_of(const PagedCache& c, int b, int pos) {
   return (id >= 0 && id < c.num_pages) ? id : -1;
 }
 
-// Sequence that owns packed row t: how many of cu[1..n] are <= t (all lanes get it; n = no sequence owns the row).
-__device__ __forceinline__ int owner_of(const int32_t* cu, int n, int t, int lane) {
-  int b = 0;
+// Sequence that owns packed row t (all lanes get it; n = no sequence owns the row), its first and last row, and x[its
+// index] where x is given.  Everything is loaded at once: what follows waits for one load, not for a chain.
+struct Owner {
+  int b, first, end, x;
+};
+__device__ __forceinline__ Owner owner_of(const int32_t* cu, int n, int t, int lane, const int32_t* x = nullptr) {
   for (int base = 0; base < n; base += 32) {
     const int i = base + lane;
-    const unsigned m = __ballot_sync(0xffffffffu, i < n && __ldg(cu + i + 1) <= t);
-    b += __popc(m);
-    if (m != 0xffffffffu) break;
+    int first = 0, end = 0x7fffffff, xi = 0;
+    if (i < n) {
+      first = __ldg(cu + i);
+      end = __ldg(cu + i + 1);
+      if (x) xi = __ldg(x + i);
+    }
+    const unsigned behind = __ballot_sync(0xffffffffu, i >= n || end > t);
+    if (behind) {
+      const int src = __ffs(behind) - 1;
+      if (base + src >= n) break;
+      return {base + src, __shfl_sync(0xffffffffu, first, src), __shfl_sync(0xffffffffu, end, src),
+              __shfl_sync(0xffffffffu, xi, src)};
+    }
   }
-  return b;
+  return {n, 0, 0, 0};
 }
 
 // fp16 scale of a group with largest magnitude amax (NaN and infinity stay what they are).
@@ -57,10 +70,28 @@ __device__ __forceinline__ half scale_of(float amax) {
   return __float2half_rn(s < kMinScale ? kMinScale : s);
 }
 
-// Code of x against the fp16 scale s: clamp(rint(x / s), -7, 7), 0 where the quotient is NaN.
-__device__ __forceinline__ int code_of(float x, float s) {
-  const float r = rintf(__fdiv_rn(x, s));
-  return r != r ? 0 : (int)fminf(fmaxf(r, -7.f), 7.f);
+// Codes of four values against the fp16 scale s (inv = 1 / s), first value in the lowest nibble: rint(x / s), which
+// needs no clamp since s is at least (1 - 2^-11) of the largest magnitude's seventh; a non-finite s gives zeros.  x * inv
+// is within 2^-23 |x / s| < 1e-6 of the quotient, so it rounds alike unless it lies that near to a half, where the division
+// decides.  An integer is rounded to by adding 1.5 * 2^23; the nibbles are summed up as exact fp32 (v + 8 in base 16).
+__device__ __forceinline__ uint32_t codes_of(float x0, float x1, float x2, float x3, float s, float inv) {
+  const float x[4] = {x0, x1, x2, x3};
+  constexpr float kRound = 12582912.f, kUnit[4] = {1.f, 16.f, 256.f, 4096.f};
+  float r[4], far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float y = __fmul_rn(x[i], inv);
+    r[i] = __fsub_rn(__fadd_rn(y, kRound), kRound);
+    far = fmaxf(far, fabsf(__fsub_rn(y, r[i])));
+  }
+  if (far > 0.499998f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = rintf(__fdiv_rn(x[i], s));
+  }
+  float v = 8388608.f + 8.f * (1.f + 16.f + 256.f + 4096.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v = fmaf(r[i], kUnit[i], v);
+  return s <= 65504.f ? (__float_as_uint(v) & 0xffffu) ^ 0x8888u : 0u;
 }
 
 // The larger magnitude, NaN if either is NaN.

@@ -27,14 +27,6 @@ __device__ __forceinline__ uint4 pack8(const float x[8]) {
   return u;
 }
 
-// Word of 8 codes in key order (value 2 i in nibble i, 2 i + 1 in nibble i + 4).
-__device__ __forceinline__ uint32_t key_word(const float x[8], float s) {
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w |= (uint32_t)(code_of(x[i], s) & 15) << (4 * ((i >> 1) + 4 * (i & 1)));
-  return w;
-}
-
 __device__ __forceinline__ float amax8(const float x[8]) {
   float a = 0.f;
 #pragma unroll
@@ -52,7 +44,9 @@ __device__ __forceinline__ void store_key_q4(uint8_t* block, int page, int slot,
     a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));  // the 4 lanes of a 32-value group
     a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
     const half sh = scale_of(a);
-    const uint32_t w = key_word(x[f], __half2float(sh));
+    const float s = __half2float(sh), inv = __fdiv_rn(1.f, s);
+    const uint32_t w = codes_of(x[f][0], x[f][2], x[f][4], x[f][6], s, inv) |
+                       codes_of(x[f][1], x[f][3], x[f][5], x[f][7], s, inv) << 16;
     if (!on) continue;
     const int j = f * (G / 2) + (l >> 2), t = l & 3;
     *reinterpret_cast<uint32_t*>(block + (int64_t)slot * (HD / 2) + 4 * (t * G + j)) = w;
@@ -67,12 +61,11 @@ __device__ __forceinline__ void store_value_q4(uint8_t* block, int page, int slo
 #pragma unroll
   for (int o = 1; o < HD / 16; o <<= 1) a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
   const half sh = scale_of(a);
-  const float s = __half2float(sh);
+  const float s = __half2float(sh), inv = __fdiv_rn(1.f, s);
 #pragma unroll
   for (int f = 0; f < 2; ++f) {
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i >> 2] |= (uint32_t)(code_of(x[f][i], s) & 15) << (4 * (i & 3));
+    const uint32_t w[2] = {codes_of(x[f][0], x[f][1], x[f][2], x[f][3], s, inv),
+                           codes_of(x[f][4], x[f][5], x[f][6], x[f][7], s, inv)};
     if (!on) continue;
     uint8_t* at = block + (int64_t)(slot >> 1) * HD + f * (HD / 2) + 8 * l + 2 * (slot & 1);
     *reinterpret_cast<uint16_t*>(at) = (uint16_t)w[0];
@@ -90,7 +83,7 @@ __device__ __forceinline__ void store_value_q4(uint8_t* block, int page, int slo
 //   rotate: y_i = x^_i c_i - x^_{i+h/2} s_i,  y_{i+h/2} = x^_{i+h/2} c_i + x^_i s_i
 // in fp32 with each operation rounded by itself, and one rounding to fp16 or to a code at the end.
 template <int HD, bool Q4, int R>
-__global__ void __launch_bounds__(32 * kWarps) paged_append_kernel(const PagedAppendParams P, const int per) {
+__global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const PagedAppendParams P, const int per) {
   constexpr int kLanes = HD / 16, kRows = 32 / kLanes;
   pdl_launch_dependents();
   pdl_wait();
@@ -118,15 +111,15 @@ __global__ void __launch_bounds__(32 * kWarps) paged_append_kernel(const PagedAp
 #pragma unroll
   for (int r = 0; r < R; ++r) load(s0 + r, raw[r]);
 
-  int b = t, at = 0;
-  if (P.cu) {
-    b = owner_of(P.cu, P.seqs, t, lane);
-    at = b < P.seqs ? t - __ldg(P.cu + b) : -1;
-  } else if (t >= P.seqs) {
-    at = -1;
-  }
+  int b = t;
   int64_t pos = -1;
-  if (at >= 0) pos = (int64_t)__ldg(P.start + b) + at;
+  if (P.cu) {
+    const Owner o = owner_of(P.cu, P.seqs, t, lane, P.start);
+    b = o.b;
+    if (b < P.seqs && t >= o.first) pos = (int64_t)o.x + (t - o.first);
+  } else if (t < P.seqs) {
+    pos = __ldg(P.start + t);
+  }
   const bool placed = pos >= 0 && pos < P.table_rows;  // a token of no sequence, or beyond the tables: zeros, no row
   const int page = 1 << P.cache.page_shift;
   int id = -1;
@@ -195,7 +188,12 @@ __global__ void __launch_bounds__(32 * kWarps) paged_append_kernel(const PagedAp
           for (int i = 0; i < 8; ++i) ss += (double)__fmul_rn(x[0][i], x[0][i]) + (double)__fmul_rn(x[1][i], x[1][i]);
 #pragma unroll
           for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          inv = (float)(1.0 / sqrt(ss / (double)HD + (double)P.eps));
+          // 1 / sqrt by Newton's iteration r += r (1 - a r^2) / 2 from the fp32 value: 2^-22 -> 2^-43 -> 64-bit rounding
+          const double a = ss * (1.0 / HD) + (double)P.eps;
+          double r = (double)rsqrtf((float)a);
+          r = fma(0.5 * r, fma(-a * r, r, 1.0), r);
+          r = fma(0.5 * r, fma(-a * r, r, 1.0), r);
+          inv = (float)r;
         }
 #pragma unroll
         for (int f = 0; f < 2; ++f)
@@ -241,14 +239,13 @@ __global__ void __launch_bounds__(32 * kWarps)
   if (t0 >= tokens) return;
   const int page = 1 << C.page_shift;
   const int64_t kbb = k_block_bytes(page, HD, Q4), vbb = v_block_bytes(page, HD, Q4);
-  int b = owner_of(cu, seqs, t0, lane);
   for (int t = t0, n; t < t0 + 2 && t < tokens; t += n) {
     n = 1;
-    if (t > t0) b = owner_of(cu, seqs, t, lane);
+    const Owner o = owner_of(cu, seqs, t, lane);
+    const int b = o.b, pos = t - o.first;
     if (b >= seqs) return;  // behind the last sequence: left as it was
-    const int pos = t - __ldg(cu + b);
     if (pos < 0) continue;
-    if (t == t0 && !(pos & 1) && t + 1 < tokens && t + 1 < __ldg(cu + b + 1)) n = 2;
+    if (t == t0 && !(pos & 1) && t + 1 < tokens && t + 1 < o.end) n = 2;
     const int slot = pos & (page - 1), id = page_of(C, b, pos);
     const uint8_t* k_base = C.k + (int64_t)id * C.nkv * kbb;
     const uint8_t* v_base = C.v + (int64_t)id * C.nkv * vbb;
@@ -351,6 +348,8 @@ cudaError_t append_hd(const PagedAppendParams& P, cudaStream_t stream) {
   const int64_t all = (int64_t)P.tokens * steps;
   int per = (int)(all / (148 * 32));
   per = per < 1 ? 1 : per > steps ? steps : per;
+  const int parts = (steps + per - 1) / per;
+  per = (steps + parts - 1) / parts;
   const int64_t warps = (int64_t)P.tokens * ((steps + per - 1) / per);
   return launch_ex(per > 1 ? paged_append_kernel<HD, Q4, 2> : paged_append_kernel<HD, Q4, 1>,
                    dim3((unsigned)((warps + kWarps - 1) / kWarps)), dim3(32 * kWarps), 0, stream, 1, true, P, per);

@@ -75,6 +75,26 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 operations at a time.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // A CTA's work: two query tiles of sequence rows q0.., keys k0.., kv head kvh.
 struct Work {
   int q0, lq, k0, lk, kvh;
@@ -342,11 +362,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 32; ++i)
             if (32 * c + i >= left) x[c][i] = 0xff800000u;  // -inf
       }
-      float top = -INFINITY;
+      float tops[8];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int i = 0; i < 8; ++i) tops[i] = __uint_as_float(x[0][i]);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[c][i]));
+      for (int i = 8; i < 128; ++i) tops[i & 7] = fmaxf(tops[i & 7], __uint_as_float(x[i >> 5][i & 31]));
+      float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
+                        fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
       top *= scale_log2;
       const bool move = top > m + kLazy;  // also the first finite maximum
       if (__any_sync(0xffffffffu, move)) {
@@ -355,32 +377,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         l *= f;
         if (j > 0) {
 #pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tc::ld32(o, O + 32 * c);
+          for (int c = 0; c < HD / 16; ++c) {
+            uint32_t o[16];
+            tc::ld16(o, O + 16 * c);
             tc::wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tc::st32(O + 32 * c, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tc::st16(O + 16 * c, o);
           }
         }
       }
       const float shift = m == -INFINITY ? 0.f : kLift - m;
-      float sum[2] = {0.f, 0.f};
+      const uint64_t scale2 = pack2(scale_log2, scale_log2), shift2 = pack2(shift, shift);
+      uint64_t sum2[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t p[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float a = ex2(fmaf(__uint_as_float(x[c][2 * i]), scale_log2, shift));
-          const float b = ex2(fmaf(__uint_as_float(x[c][2 * i + 1]), scale_log2, shift));
-          sum[0] += a;
-          sum[1] += b;
+          float a, b;
+          unpack2(fma2(pack2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), scale2, shift2), a, b);
+          a = ex2(a);
+          b = ex2(b);
+          sum2[i & 1] = add2(sum2[i & 1], pack2(a, b));
           p[i] = h2_as_u32(__floats2half2_rn(a, b));
         }
         tc::st16(S + 16 * c, p);
       }
-      l += sum[0] + sum[1];
+      float sa, sb;
+      unpack2(add2(sum2[0], sum2[1]), sa, sb);
+      l += sa + sb;
       tc::wait_st();
       tc::fence_before();
       mbar_arrive(&sh.p_full[s]);
