@@ -12,7 +12,7 @@
 //   warps 0-3, 4-7: the softmax of stage 0 / 1, one thread per row.
 //   warp 8: loads Q, then K and V tiles of 128 keys through a ring of four slots (TMA, 128-byte swizzle).  A last V tile
 //           with fewer keys has its other rows cleared: what lies behind a sequence may be anything, and 0 * NaN counts.
-//   warp 9: one thread issues the products in the order  S0(j) P1V(j-1) S1(j) P0V(j) -- while the tensor core works on one
+//   warp 9: issues the products in the order  S0(j) P1V(j-1) S1(j) P0V(j) -- while the tensor core works on one
 //           stage, the other stage's softmax runs.  Products of one thread run in order, so S(j+1) overwrites P(j) only
 //           after P(j) V has read it; a commit covers everything issued before it, so scores that have arrived say that
 //           the O before them is complete.
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_q = smem;                           // two tiles
   uint8_t* s_kv = smem + 2 * kTileBytes;         // kSlots tiles
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   pdl_launch_dependents();
   pdl_wait();
@@ -280,58 +280,60 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 9) {
     // ---------------------------------------------------------------- products
-    if (lane == 0) {
-      constexpr uint32_t kIdescS = tc::instr_desc(kTile, kTile, false), kIdescO = tc::instr_desc(kTile, HD, true);
-      bool ok = true;
+    constexpr uint32_t kIdescS = tc::instr_desc(kTile, kTile, false), kIdescO = tc::instr_desc(kTile, HD, true);
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
+    const int n0 = __shfl_sync(0xffffffffu, w.tiles[0], 0), n1 = __shfl_sync(0xffffffffu, w.tiles[1], 0);
+    const int n = n0 > n1 ? n0 : n1;
+    const uint32_t at_q = __shfl_sync(0xffffffffu, smem_u32(s_q), 0), at_kv = at_q + 2 * kTileBytes;
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, wait(sh, bar, parity)); };
+    bool ok = true;
+    if (n0 > 0) ok = wait_all(&sh.q_full[0], 0);
+    if (n1 > 0) ok = ok && wait_all(&sh.q_full[1], 0);
+    auto scores = [&](int s, int j) {          // S_s = Q_s K_j^T
+      const uint64_t a = tc::smem_desc(at_q + s * kTileBytes, 16, 1024);
+      const uint64_t b = tc::smem_desc(at_kv + (2 * j % kSlots) * kTileBytes, 16, 1024);
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (w.tiles[s] > 0) ok = ok && wait(sh, &sh.q_full[s], 0);
-      auto scores = [&](int s, int j) {          // S_s = Q_s K_j^T
-        const uint32_t a = smem_u32(s_q + s * kTileBytes), b = smem_u32(s_kv + (2 * j % kSlots) * kTileBytes);
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t at = (k / 4) * kBox + (k % 4) * 32;
-          tc::mma_ss(tmem + s * kTile, tc::smem_desc(a + at, 16, 1024), tc::smem_desc(b + at, 16, 1024), kIdescS, k > 0);
-        }
-        tc::commit(&sh.s_full[s]);
-      };
-      auto outputs = [&](int s, int j) {         // O_s (+)= P_s V_j
-        ok = ok && wait(sh, &sh.p_full[s], j & 1);
-        if (!ok) return;
-        tc::fence_after();
-        const uint32_t b = smem_u32(s_kv + ((2 * j + 1) % kSlots) * kTileBytes);
-#pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          tc::mma_ts(tmem + kO + s * HD, tmem + s * kTile + k * 8, tc::smem_desc(b + k * 2048, kBox, 1024), kIdescO,
-                     j > 0 || k > 0);
-        if (j == w.tiles[s] - 1) tc::commit(&sh.o_full[s]);
-      };
-      for (int j = 0; j <= steps && ok; ++j) {
-        if (j < steps) ok = wait(sh, &sh.kv_full[2 * j % kSlots], (2 * j / kSlots) & 1);
-        if (!ok) break;
-        tc::fence_after();
-        if (j < w.tiles[0]) scores(0, j);
-        if (j > 0) {
-          if (j - 1 < w.tiles[1]) {
-            ok = wait(sh, &sh.kv_full[(2 * j - 1) % kSlots], ((2 * j - 1) / kSlots) & 1);
-            if (ok) outputs(1, j - 1);
-            if (!ok) break;
-          }
-          tc::commit(&sh.kv_empty[(2 * j - 1) % kSlots]);
-        }
-        if (j == steps) break;
-        if (j < w.tiles[1]) scores(1, j);
-        tc::commit(&sh.kv_empty[2 * j % kSlots]);
-        if (j < w.tiles[0]) {
-          ok = wait(sh, &sh.kv_full[(2 * j + 1) % kSlots], ((2 * j + 1) / kSlots) & 1);
-          if (ok) outputs(0, j);
-        }
+      for (int k = 0; k < HD / 16; ++k) {
+        const uint32_t at = ((k / 4) * kBox + (k % 4) * 32) >> 4;
+        tc::mma_ss(base + s * kTile, a + at, b + at, kIdescS, k > 0);
       }
-      if (!ok) {  // let the products in flight end before the tensor memory is given back
-        tc::commit(&sh.drained);
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(&sh.drained, 0) && globaltimer_ns() - t0 < kTimeoutNs) {
+      tc::commit(&sh.s_full[s]);
+    };
+    auto outputs = [&](int s, int j, int last) {  // O_s (+)= P_s V_j
+      ok = ok && wait_all(&sh.p_full[s], j & 1);
+      if (!ok) return;
+      tc::fence_after();
+      const uint64_t b = tc::smem_desc(at_kv + ((2 * j + 1) % kSlots) * kTileBytes, kBox, 1024);
+#pragma unroll
+      for (int k = 0; k < kTile / 16; ++k)
+        tc::mma_ts(base + kO + s * HD, base + s * kTile + k * 8, b + k * (2048 >> 4), kIdescO, j > 0 || k > 0);
+      if (j == last) tc::commit(&sh.o_full[s]);
+    };
+    for (int j = 0; j <= n && ok; ++j) {
+      if (j < n) ok = wait_all(&sh.kv_full[2 * j % kSlots], (2 * j / kSlots) & 1);
+      if (!ok) break;
+      tc::fence_after();
+      if (j < n0) scores(0, j);
+      if (j > 0) {
+        if (j - 1 < n1) {
+          ok = wait_all(&sh.kv_full[(2 * j - 1) % kSlots], ((2 * j - 1) / kSlots) & 1);
+          if (ok) outputs(1, j - 1, n1 - 1);
+          if (!ok) break;
         }
+        tc::commit(&sh.kv_empty[(2 * j - 1) % kSlots]);
+      }
+      if (j == n) break;
+      if (j < n1) scores(1, j);
+      tc::commit(&sh.kv_empty[2 * j % kSlots]);
+      if (j < n0) {
+        ok = wait_all(&sh.kv_full[(2 * j + 1) % kSlots], ((2 * j + 1) / kSlots) & 1);
+        if (ok) outputs(0, j, n0 - 1);
+      }
+    }
+    if (!ok) {  // let the products in flight end before the tensor memory is given back
+      tc::commit(&sh.drained);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(&sh.drained, 0) && globaltimer_ns() - t0 < kTimeoutNs) {
       }
     }
     __syncwarp();

@@ -25,11 +25,14 @@ __host__ __device__ constexpr uint32_t instr_desc(int m, int n, bool b_rows_k) {
   return 1u << 4 | (b_rows_k ? 1u << 16 : 0u) | (uint32_t)(n / 8) << 17 | (uint32_t)(m / 16) << 24;
 }
 
+// The products and commits below are called by a whole warp with the same values and issued by its elected lane (the same
+// one every time): descriptors then stay in uniform registers.  From a single-lane branch each product took 90 cycles to
+// issue, more than the 64 that the tensor core needs for it.
 // D (+)= A B with A and B in shared memory.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.u32 p, %4, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
@@ -37,16 +40,18 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
 // D (+)= A B with A in tensor memory (two fp16 along the reduction per column).
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.u32 p, %4, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
 
-// Arrives on bar once every tcgen05 operation that this thread has issued is complete.
+// Arrives on bar once every tcgen05 operation that the elected lane has issued is complete.
 __device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+  asm volatile(
+      "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar))
+      : "memory");
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
