@@ -23,7 +23,7 @@
 // rows whose result is not finite are computed again one by one over exactly the keys they see.
 //
 // The grid holds one CTA per pair of tiles and kv head, an upper bound from the token counts (row bounds are read on the
-// device); within a sequence the longest rows come first, so that the short ones fill the end.
+// device).
 #include <cuda.h>
 
 #include "common.cuh"
@@ -36,16 +36,18 @@ namespace {
 
 constexpr int kTile = 128;            // query rows and keys per tile
 constexpr int kSlots = 4;             // K / V tiles in flight
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;         // 8 softmax warps, loads, products, two without work (register shares go by 4 warps)
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;  // 256 x 216 + 128 x 72 = 384 x 168, what the launch gets
 constexpr uint64_t kTimeoutNs = 1000000000ull;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;          // the maximum follows when exceeded by 2^8
+constexpr unsigned kFmaPairs = 0x22;  // which of 8 pairs of exponentials go to the fp32 pipe
 constexpr float kLift = 7.f;          // factor 2^7 on the probabilities
 
 __device__ int g_prefill_error;
 
 struct Shared {
-  uint64_t q_full[2], kv_full[kSlots], kv_empty[kSlots], v_landed, s_full[2], p_full[2], o_full[2], drained;
+  uint64_t q_full[2], kv_full[kSlots], kv_empty[kSlots], v_landed, s_full[2], p_full[2], p_half[2], o_full[2], drained;
   uint32_t tmem;
   int abort;
 };
@@ -75,6 +77,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Two fp32 operations at a time.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;
@@ -95,6 +103,27 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// 2^x of both halves on the fp32 pipe: x = n + f with n the nearest integer (added to 1.5 * 2^23, whose low bits then hold
+// it) and |f| <= 1/2, 2^f by a polynomial of degree 4 (least largest relative error, 2.7e-6, by exchange), 2^n added to the
+// exponent.  Below 2^-126: 0 or a subnormal.
+__device__ __forceinline__ void ex2_pair(uint64_t x2, float& a, float& b) {
+  constexpr float kRound = 12582912.f;
+  float x, y;
+  unpack2(x2, x, y);
+  x2 = pack2(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  const uint64_t t2 = add2(x2, pack2(kRound, kRound));
+  const uint64_t f2 = fma2(add2(t2, pack2(-kRound, -kRound)), pack2(-1.f, -1.f), x2);
+  uint64_t p2 = fma2(pack2(0.00957010220736f, 0.00957010220736f), f2, pack2(0.0559178590775f, 0.0559178590775f));
+  p2 = fma2(p2, f2, pack2(0.240247443318f, 0.240247443318f));
+  p2 = fma2(p2, f2, pack2(0.693121790886f, 0.693121790886f));
+  p2 = fma2(p2, f2, pack2(0.999999284744f, 0.999999284744f));
+  float t, u, p, q;
+  unpack2(t2, t, u);
+  unpack2(p2, p, q);
+  a = __int_as_float((__float_as_int(t) << 23) + __float_as_int(p));
+  b = __int_as_float((__float_as_int(u) << 23) + __float_as_int(q));
+}
+
 // A CTA's work: two query tiles of sequence rows q0.., keys k0.., kv head kvh.
 struct Work {
   int q0, lq, k0, lk, kvh;
@@ -102,39 +131,46 @@ struct Work {
 };
 
 // The pair of query tiles that blockIdx.x stands for (warp-wide; false: none).  Query tile t of a sequence and kv head
-// is head t % rep, rows (t / rep) * 128 ..; pairs run from the last to the first.
+// is head t % rep, rows (t / rep) * 128 ..; a sequence's pairs run from the last to the first, and of up to 32 sequences
+// those with more keys come first (more: as they are given), so that short work fills the end of the launch.
 __device__ __forceinline__ bool find_work(const PrefillParams& P, int lane, Work& w) {
   const int rep = P.nq / P.nkv;
   w.kvh = blockIdx.x % P.nkv;
-  const int want = blockIdx.x / P.nkv;
-  int before = 0;
+  int want = blockIdx.x / P.nkv;
   for (int base = 0; base < P.seqs; base += 32) {
     const int i = base + lane;
-    int q0 = 0, lq = 0;
+    int q0 = 0, lq = 0, k0 = 0, lk = 0;
     if (i < P.seqs) {
-      const int a = __ldg(P.cu_q + i), e = __ldg(P.cu_q + i + 1);
-      q0 = a < 0 ? 0 : a;
-      lq = (e > P.tokens_q ? P.tokens_q : e) - q0;
-      if (lq < 0) lq = 0;
+      const int a = __ldg(P.cu_q + i), e = __ldg(P.cu_q + i + 1), c = __ldg(P.cu_k + i), f = __ldg(P.cu_k + i + 1);
+      q0 = max(a, 0);
+      lq = max(min(e, P.tokens_q) - q0, 0);
+      k0 = max(c, 0);
+      lk = max(min(f, P.tokens_k) - k0, 0);
     }
     const int pairs = ((lq + kTile - 1) / kTile * rep + 1) / 2;
-    int sum = pairs;
+    int before = 0;
+    if (P.seqs <= 32) {
+      for (int o = 0; o < P.seqs; ++o) {
+        const int keys = __shfl_sync(0xffffffffu, lk, o), n = __shfl_sync(0xffffffffu, pairs, o);
+        if (keys > lk || (keys == lk && o < lane)) before += n;
+      }
+    } else {
+      before = pairs;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
+      }
+      before -= pairs;
     }
-    const int c = want - before;
-    const unsigned owns = __ballot_sync(0xffffffffu, c >= sum - pairs && c < sum);
+    const unsigned owns = __ballot_sync(0xffffffffu, want >= before && want < before + pairs);
     if (owns) {
-      const int src = __ffs(owns) - 1, b = base + src;
+      const int src = __ffs(owns) - 1;
       w.q0 = __shfl_sync(0xffffffffu, q0, src);
       w.lq = __shfl_sync(0xffffffffu, lq, src);
-      const int last = __shfl_sync(0xffffffffu, sum, src) - 1 - c;  // pairs from the sequence's end
-      const int ka = __ldg(P.cu_k + b), ke = __ldg(P.cu_k + b + 1);
-      w.k0 = ka < 0 ? 0 : ka;
-      w.lk = (ke > P.tokens_k ? P.tokens_k : ke) - w.k0;
-      if (w.lk < 0) w.lk = 0;
+      w.k0 = __shfl_sync(0xffffffffu, k0, src);
+      w.lk = __shfl_sync(0xffffffffu, lk, src);
+      const int last = __shfl_sync(0xffffffffu, pairs - 1 - (want - before), src);  // the pair, from the sequence's start
       const int tiles = (w.lq + kTile - 1) / kTile * rep;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -142,13 +178,12 @@ __device__ __forceinline__ bool find_work(const PrefillParams& P, int lane, Work
         w.row[s] = t / rep * kTile;
         w.head[s] = w.kvh * rep + t % rep;
         const int rows = w.lq - w.row[s] < kTile ? w.lq - w.row[s] : kTile;
-        int keys = w.row[s] + rows + w.lk - w.lq;  // what the tile's last row sees
-        keys = keys < 0 ? 0 : keys;
+        const int keys = max(w.row[s] + rows + w.lk - w.lq, 0);  // what the tile's last row sees
         w.tiles[s] = t < tiles ? (keys + kTile - 1) / kTile : -1;
       }
       return true;
     }
-    before += __shfl_sync(0xffffffffu, sum, 31);
+    want -= __reduce_add_sync(0xffffffffu, pairs);
   }
   return false;
 }
@@ -209,7 +244,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sh.q_full[s], 1);
       mbar_init(&sh.s_full[s], 1);
-      mbar_init(&sh.p_full[s], kTile);
+      mbar_init(&sh.p_full[s], 4);
+      mbar_init(&sh.p_half[s], 4);
       mbar_init(&sh.o_full[s], 1);
     }
     for (int i = 0; i < kSlots; ++i) {
@@ -226,7 +262,147 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after();
   const uint32_t tmem = sh.tmem;
 
-  if (warp == 8) {
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // ---------------------------------------------------------------- softmax
+    const int s = warp >> 2, r = threadIdx.x & (kTile - 1);
+    const int tiles = w.tiles[s], row = w.row[s] + r;
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+    const uint32_t S = lanes + s * kTile, O = lanes + kO + s * HD;
+    const bool valid = row < w.lq;
+    int limit = valid ? row + 1 + w.lk - w.lq : 0;  // keys this row sees
+    if (limit < 0) limit = 0;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < tiles && ok; ++j) {
+      ok = __all_sync(0xffffffffu, wait(sh, &sh.s_full[s], j & 1));
+      if (!ok) break;
+      tc::fence_after();
+      uint32_t x[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tc::ld32(x[c], S + 32 * c);
+      tc::wait_ld();
+      const int left = limit - j * kTile;
+      if (__any_sync(0xffffffffu, left < kTile)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * c + i >= left) x[c][i] = 0xff800000u;  // -inf
+      }
+      float tops[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) tops[i] = fmaxf(__uint_as_float(x[0][2 * i]), __uint_as_float(x[0][2 * i + 1]));
+#pragma unroll
+      for (int i = 16; i < 128; i += 2)
+        tops[(i >> 1) & 7] = max3(tops[(i >> 1) & 7], __uint_as_float(x[i >> 5][i & 31]), __uint_as_float(x[i >> 5][(i & 31) + 1]));
+      float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
+                        fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
+      top *= scale_log2;
+      const bool move = top > m + kLazy;  // also the first finite maximum
+      if (__any_sync(0xffffffffu, move)) {
+        const float f = move ? ex2(m - top) : 1.f;
+        if (move) m = top;
+        l *= f;
+        if (j > 0) {
+#pragma unroll
+          for (int c = 0; c < HD / 16; ++c) {
+            uint32_t o[16];
+            tc::ld16(o, O + 16 * c);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tc::st16(O + 16 * c, o);
+          }
+        }
+      }
+      const float shift = m == -INFINITY ? 0.f : kLift - m;
+      const uint64_t scale2 = pack2(scale_log2, scale_log2), shift2 = pack2(shift, shift);
+      uint64_t sum2[2] = {0, 0};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float a, b;
+          const uint64_t y2 = fma2(pack2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), scale2, shift2);
+          if (kFmaPairs >> (i & 7) & 1) {
+            ex2_pair(y2, a, b);
+          } else {
+            unpack2(y2, a, b);
+            a = ex2(a);
+            b = ex2(b);
+          }
+          sum2[i & 1] = add2(sum2[i & 1], pack2(a, b));
+          p[i] = h2_as_u32(__floats2half2_rn(a, b));
+        }
+        tc::st16(S + 16 * c, p);
+        if (c == 1) {  // the first 64 keys' probabilities are there
+          tc::wait_st();
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.p_half[s]);
+        }
+      }
+      float sa, sb;
+      unpack2(add2(sum2[0], sum2[1]), sa, sb);
+      l += sa + sb;
+      tc::wait_st();
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full[s]);
+    }
+    // the row's result
+    if (tiles >= 0 && ok) {
+      constexpr int kPieces = HD / 8;
+      uint4* stage = reinterpret_cast<uint4*>(s_q + s * kTileBytes + (warp & 3) * (32 * HD * 2));
+      bool good = true;
+      if (tiles > 0) {
+        ok = __all_sync(0xffffffffu, wait(sh, &sh.o_full[s], 0));
+        tc::fence_after();
+      }
+      if (ok) {
+        const float inv = limit > 0 ? 1.f / l : 0.f;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          if (tiles > 0) {
+            tc::ld32(o, O + 32 * c);
+            tc::wait_ld();
+          }
+          uint4 v[4];
+          uint32_t* h = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float a = 0.f, b = 0.f;
+            if (limit > 0) a = __uint_as_float(o[2 * i]) * inv, b = __uint_as_float(o[2 * i + 1]) * inv;
+            good = good && fabsf(a) <= 3.4e38f && fabsf(b) <= 3.4e38f;
+            h[i] = h2_as_u32(__floats2half2_rn(a, b));
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) stage[lane * kPieces + ((4 * c + i) ^ (lane & 7))] = v[i];
+        }
+        __syncwarp();
+        const int row0 = w.row[s] + (r & ~31);
+        uint4* out = reinterpret_cast<uint4*>(P.out + ((int64_t)(w.q0 + row0) * P.nq + w.head[s]) * HD);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int rr = (32 * i + lane) / kPieces, c = lane % kPieces;
+          if (row0 + rr < w.lq) out[(int64_t)rr * P.nq * kPieces + c] = stage[rr * kPieces + (c ^ (rr & 7))];
+        }
+        unsigned again = __ballot_sync(0xffffffffu, valid && !good);
+        while (again) {
+          const int src = __ffs(again) - 1, rr = w.row[s] + (r & ~31) + src;
+          again &= again - 1;
+          __syncwarp();
+          redo_row<HD>(P, P.q + (int64_t)(w.q0 + rr) * P.q_token + w.head[s] * P.q_head, w.k0, rr + 1 + w.lk - w.lq,
+                       w.kvh, P.out + ((int64_t)(w.q0 + rr) * P.nq + w.head[s]) * HD, scale_log2, lane);
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 8) {
     // ---------------------------------------------------------------- loads
     // Key tile j is ring entry 2 j, value tile j entry 2 j + 1.
     int issued = 0;
@@ -278,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         while (!mbar_try_wait(&sh.kv_full[e % kSlots], (e / kSlots) & 1) && globaltimer_ns() - t0 < kTimeoutNs) {
         }
     }
-  } else if (warp == 9) {
+    } else if (warp == 9) {
     // ---------------------------------------------------------------- products
     constexpr uint32_t kIdescS = tc::instr_desc(kTile, kTile, false), kIdescO = tc::instr_desc(kTile, HD, true);
     const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
@@ -300,13 +476,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::commit(&sh.s_full[s]);
     };
     auto outputs = [&](int s, int j, int last) {  // O_s (+)= P_s V_j
-      ok = ok && wait_all(&sh.p_full[s], j & 1);
-      if (!ok) return;
-      tc::fence_after();
       const uint64_t b = tc::smem_desc(at_kv + ((2 * j + 1) % kSlots) * kTileBytes, kBox, 1024);
 #pragma unroll
-      for (int k = 0; k < kTile / 16; ++k)
-        tc::mma_ts(base + kO + s * HD, base + s * kTile + k * 8, b + k * (2048 >> 4), kIdescO, j > 0 || k > 0);
+      for (int f = 0; f < 2; ++f) {
+        ok = ok && wait_all(f ? &sh.p_full[s] : &sh.p_half[s], j & 1);
+        if (!ok) return;
+        tc::fence_after();
+#pragma unroll
+        for (int k = 4 * f; k < 4 * f + 4; ++k)
+          tc::mma_ts(base + kO + s * HD, base + s * kTile + k * 8, b + k * (2048 >> 4), kIdescO, j > 0 || k > 0);
+      }
       if (j == last) tc::commit(&sh.o_full[s]);
     };
     for (int j = 0; j <= n && ok; ++j) {
@@ -337,121 +516,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else {
-    // ---------------------------------------------------------------- softmax
-    const int s = warp >> 2, r = threadIdx.x & (kTile - 1);
-    const int tiles = w.tiles[s], row = w.row[s] + r;
-    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
-    const uint32_t S = lanes + s * kTile, O = lanes + kO + s * HD;
-    const bool valid = row < w.lq;
-    int limit = valid ? row + 1 + w.lk - w.lq : 0;  // keys this row sees
-    if (limit < 0) limit = 0;
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int j = 0; j < tiles && ok; ++j) {
-      ok = __all_sync(0xffffffffu, wait(sh, &sh.s_full[s], j & 1));
-      if (!ok) break;
-      tc::fence_after();
-      uint32_t x[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tc::ld32(x[c], S + 32 * c);
-      tc::wait_ld();
-      const int left = limit - j * kTile;
-      if (__any_sync(0xffffffffu, left < kTile)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * c + i >= left) x[c][i] = 0xff800000u;  // -inf
-      }
-      float tops[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) tops[i] = __uint_as_float(x[0][i]);
-#pragma unroll
-      for (int i = 8; i < 128; ++i) tops[i & 7] = fmaxf(tops[i & 7], __uint_as_float(x[i >> 5][i & 31]));
-      float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
-                        fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
-      top *= scale_log2;
-      const bool move = top > m + kLazy;  // also the first finite maximum
-      if (__any_sync(0xffffffffu, move)) {
-        const float f = move ? ex2(m - top) : 1.f;
-        if (move) m = top;
-        l *= f;
-        if (j > 0) {
-#pragma unroll
-          for (int c = 0; c < HD / 16; ++c) {
-            uint32_t o[16];
-            tc::ld16(o, O + 16 * c);
-            tc::wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tc::st16(O + 16 * c, o);
-          }
-        }
-      }
-      const float shift = m == -INFINITY ? 0.f : kLift - m;
-      const uint64_t scale2 = pack2(scale_log2, scale_log2), shift2 = pack2(shift, shift);
-      uint64_t sum2[2] = {0, 0};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t p[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float a, b;
-          unpack2(fma2(pack2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), scale2, shift2), a, b);
-          a = ex2(a);
-          b = ex2(b);
-          sum2[i & 1] = add2(sum2[i & 1], pack2(a, b));
-          p[i] = h2_as_u32(__floats2half2_rn(a, b));
-        }
-        tc::st16(S + 16 * c, p);
-      }
-      float sa, sb;
-      unpack2(add2(sum2[0], sum2[1]), sa, sb);
-      l += sa + sb;
-      tc::wait_st();
-      tc::fence_before();
-      mbar_arrive(&sh.p_full[s]);
-    }
-    // the row's result
-    if (tiles >= 0 && ok) {
-      half* out = P.out + ((int64_t)(w.q0 + row) * P.nq + w.head[s]) * HD;
-      bool good = true;
-      if (tiles > 0) {
-        ok = __all_sync(0xffffffffu, wait(sh, &sh.o_full[s], 0));
-        tc::fence_after();
-      }
-      if (ok) {
-        const float inv = limit > 0 ? 1.f / l : 0.f;
-#pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t o[32];
-          if (tiles > 0) {
-            tc::ld32(o, O + 32 * c);
-            tc::wait_ld();
-          }
-          uint4 v[4];
-          uint32_t* h = reinterpret_cast<uint32_t*>(v);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float a = 0.f, b = 0.f;
-            if (limit > 0) a = __uint_as_float(o[2 * i]) * inv, b = __uint_as_float(o[2 * i + 1]) * inv;
-            good = good && fabsf(a) <= 3.4e38f && fabsf(b) <= 3.4e38f;
-            h[i] = h2_as_u32(__floats2half2_rn(a, b));
-          }
-          if (valid)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(out)[4 * c + i] = v[i];
-        }
-        unsigned again = __ballot_sync(0xffffffffu, valid && !good);
-        while (again) {
-          const int src = __ffs(again) - 1, rr = w.row[s] + (r & ~31) + src;
-          again &= again - 1;
-          __syncwarp();
-          redo_row<HD>(P, P.q + (int64_t)(w.q0 + rr) * P.q_token + w.head[s] * P.q_head, w.k0, rr + 1 + w.lk - w.lq,
-                       w.kvh, P.out + ((int64_t)(w.q0 + rr) * P.nq + w.head[s]) * HD, scale_log2, lane);
-        }
-      }
     }
   }
   tc::fence_before();
