@@ -155,9 +155,13 @@ def device_errors() -> int:
 def _call(fn_name: str, *args) -> None:
     status = getattr(lib(), fn_name)(*args)
     if status != 0:
-        msg = lib().soinfer_last_error().decode()
-        kind = lib().soinfer_status_string(status).decode()
-        raise RuntimeError(f"{msg} [{kind}]")
+        _raise(status)
+
+
+def _raise(status: int) -> None:
+    msg = lib().soinfer_last_error().decode()
+    kind = lib().soinfer_status_string(status).decode()
+    raise RuntimeError(f"{msg} [{kind}]")
 
 
 def _check(cond: bool, *msg) -> None:
@@ -886,7 +890,7 @@ def head_norm_rope(q, k, v, q_norm, k_norm, cos_vals, sin_vals, k_cache, v_cache
 _PAGED_CACHE = struct.Struct("PPPqqqqqqq")  # soinfer_paged_cache
 _ROWS = struct.Struct("Pqq")                # soinfer_rows
 PAGED_HEAD_DIMS = (64, 128)
-_F16, _U8, _I32 = torch.float16, torch.uint8, torch.int32
+_F16, _F32, _U8, _I32 = torch.float16, torch.float32, torch.uint8, torch.int32
 
 
 def _fail(*msg) -> None:
@@ -911,64 +915,72 @@ def paged_kv_alloc(num_pages: int, num_kv_heads: int, page_size: int, head_dim: 
 
 
 def _paged_cache(name: str, k_pages, v_pages, block_table, dev: int, head_dim: int | None = None):
-    """(the C form of a checked paged cache, its kv heads, its head_dim); dev: the device everything has to be on."""
-    if not (k_pages.is_cuda and v_pages.is_cuda and block_table.is_cuda):
-        _fail(name, ": pages and block_table must be CUDA tensors")
-    dtype = k_pages.dtype
-    if dtype != v_pages.dtype or (dtype != _F16 and dtype != _U8):
-        _fail(name, ": k_pages / v_pages must both be float16 or both uint8 (4 bits)")
-    ks, vs, ts = k_pages.shape, v_pages.shape, block_table.shape
-    if not (len(ks) == 4 and len(vs) == 4 and ks[:3] == vs[:3] and k_pages.is_contiguous() and v_pages.is_contiguous()):
+    """(the C form of a checked paged cache, its kv heads, head_dim, page size, sequences); dev: the device everything has
+    to be on."""
+    ks, vs, ts, table_stride, dtype = k_pages.shape, v_pages.shape, block_table.shape, block_table.stride(), k_pages.dtype
+    if (dev < 0 or k_pages.get_device() != dev or v_pages.get_device() != dev or block_table.get_device() != dev
+            or v_pages.dtype is not dtype or (dtype is not _F16 and dtype is not _U8) or len(ks) != 4 or len(vs) != 4
+            or not k_pages.is_contiguous() or not v_pages.is_contiguous()):
+        if not (k_pages.is_cuda and v_pages.is_cuda and block_table.is_cuda):
+            _fail(name, ": pages and block_table must be CUDA tensors")
+        if not (k_pages.get_device() == v_pages.get_device() == block_table.get_device() == dev):
+            _fail(name, ": all tensors must be on the same CUDA device")
+        if v_pages.dtype != dtype or dtype not in (_F16, _U8):
+            _fail(name, ": k_pages / v_pages must both be float16 or both uint8 (4 bits)")
         _fail(name, ": k_pages / v_pages must be contiguous [num_pages, num_kv_heads, page_size, width]")
     pages, nkv, page, wk = ks
-    if dtype == _F16:
-        bits, hd, fits = 16, wk, vs[3] == wk
+    if dtype is _F16:
+        bits, hd, wv = 16, wk, wk
     else:
         bits, hd = 4, wk * 16 // 9
-        fits = wk == hd // 2 + hd // 16 and vs[3] == hd // 2 + 2
-    if not fits or hd not in PAGED_HEAD_DIMS:
+        wv = hd // 2 + 2
+    if vs != (pages, nkv, page, wv) or hd not in PAGED_HEAD_DIMS or (bits == 4 and wk != hd // 2 + hd // 16):
+        if vs[:3] != ks[:3]:
+            _fail(name, ": k_pages / v_pages must agree in num_pages, num_kv_heads and page_size")
         _fail(name, ": page widths must be head_dim (64 or 128), or for 4 bits head_dim/2 + head_dim/16 and head_dim/2 + 2")
     if head_dim is not None and head_dim != hd:
         _fail(name, ": head_dim of the rows and of the pages disagree")
     if page < 16 or page > 1 << 16 or page & (page - 1):
         _fail(name, ": page_size must be a power of two in [16, 65536]")
-    if block_table.dtype != _I32 or len(ts) != 2 or (ts[1] > 1 and block_table.stride(1) != 1):
+    if block_table.dtype is not _I32 or len(ts) != 2 or (ts[1] > 1 and table_stride[1] != 1):
         _fail(name, ": block_table must be int32 [num_seqs, max_pages] with contiguous rows")
-    cols = ts[1] if ts[0] else 0
-    stride = block_table.stride(0) if ts[0] > 1 else cols
+    seqs = ts[0]
+    cols = ts[1] if seqs else 0
+    stride = table_stride[0] if seqs > 1 else cols
     if stride < cols:
         _fail(name, ": block_table rows must not overlap")
-    if not (k_pages.get_device() == v_pages.get_device() == block_table.get_device() == dev):
-        _fail(name, ": all tensors must be on the same CUDA device")
     return (_PAGED_CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), stride, cols, pages, nkv, page,
-                              hd, bits), nkv, hd)
+                              hd, bits), nkv, hd, page, seqs)
 
 
-def _rows(name: str, what: str, x):
-    """(the C form of checked rows [tokens, heads, head_dim], their shape)."""
-    if not x.is_cuda or x.dtype != _F16:
-        _fail(name, "(", what, "): must be a float16 CUDA tensor")
+def _rows(name: str, what: str, x, dev: int):
+    """(the C form of checked rows [tokens, heads, head_dim] on device dev, their shape)."""
     shape, stride, at = x.shape, x.stride(), x.data_ptr()
-    if len(shape) != 3 or stride[2] != 1:
-        _fail(name, "(", what, "): must be [tokens, heads, head_dim] with contiguous heads")
-    if stride[0] & 7 or stride[1] & 7 or at & 15:
+    if (x.dtype is not _F16 or dev < 0 or x.get_device() != dev or len(shape) != 3 or stride[2] != 1
+            or (stride[0] | stride[1]) & 7 or at & 15):
+        if not x.is_cuda or x.dtype != _F16:
+            _fail(name, "(", what, "): must be a float16 CUDA tensor")
+        if x.get_device() != dev:
+            _fail(name, ": all tensors must be on the same CUDA device")
+        if len(shape) != 3 or stride[2] != 1:
+            _fail(name, "(", what, "): must be [tokens, heads, head_dim] with contiguous heads")
         _fail(name, "(", what, "): needs 16-byte aligned rows (strides in multiples of 8 elements)")
     return _ROWS.pack(at, stride[0], stride[1]), shape
 
 
 def _int32(name: str, what: str, t, n: int, dev: int) -> int:
-    if not t.is_cuda or t.dtype != _I32 or t.dim() != 1 or t.size(0) != n or not t.is_contiguous():
+    """Address of a checked int32 vector of n elements on device dev."""
+    if t.dtype is not _I32 or t.get_device() != dev or t.shape != (n,) or not t.is_contiguous():
+        if t.is_cuda and t.get_device() != dev:
+            _fail(name, ": all tensors must be on the same CUDA device")
         _fail(name, "(", what, f"): must be a contiguous int32 CUDA tensor of {n} elements")
-    if t.get_device() != dev:
-        _fail(name, ": all tensors must be on the same CUDA device")
     return t.data_ptr()
 
 
 def _out_rows(name: str, out, like, shape) -> torch.Tensor:
     if out is None:
         return like.new_empty(shape, dtype=_F16)
-    if not (out.is_cuda and out.dtype == _F16 and tuple(out.shape) == shape and out.is_contiguous()
-            and out.data_ptr() % 16 == 0):
+    if not (out.is_cuda and out.dtype == _F16 and out.shape == shape and out.is_contiguous() and out.data_ptr() % 16 == 0):
         _fail(name, f": out must be a contiguous, 16-byte aligned float16 CUDA tensor of shape {shape}")
     if out.get_device() != like.get_device():
         _fail(name, ": all tensors must be on the same CUDA device")
@@ -978,7 +990,9 @@ def _out_rows(name: str, out, like, shape) -> torch.Tensor:
 def _call_on(dev: int, fn_name: str, *args) -> None:
     """_call with the device's current stream as the last argument and the device current."""
     if torch._C._cuda_getDevice() == dev:
-        _call(fn_name, *args, torch._C._cuda_getCurrentRawStream(dev))
+        status = getattr(_lib or lib(), fn_name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+        if status:
+            _raise(status)
     else:
         with torch.cuda.device(dev):
             _call(fn_name, *args, torch._C._cuda_getCurrentRawStream(dev))
@@ -987,61 +1001,62 @@ def _call_on(dev: int, fn_name: str, *args) -> None:
 def paged_kv_append(q, k, v, k_pages, v_pages, block_table, start, cos_table, sin_table, cu_seqlens=None, q_norm=None,
                     k_norm=None, eps: float = 1e-6, return_k: bool = False):
     name = "paged_kv_append"
-    rk, ks = _rows(name, "k", k)
-    rv, vs = _rows(name, "v", v)
-    T, nkv, hd = ks
     dev = k.get_device()
-    cache, heads, _ = _paged_cache(name, k_pages, v_pages, block_table, dev, hd)
+    rk, ks = _rows(name, "k", k, dev)
+    rv, vs = _rows(name, "v", v, dev)
+    T, nkv, hd = ks
+    cache, heads, _, _, B = _paged_cache(name, k_pages, v_pages, block_table, dev, hd)
     if ks != vs or nkv != heads:
         _fail(name, ": k / v must be [tokens, num_kv_heads, head_dim]")
     rq, nq, q_out, k_out = None, 0, None, None
     if q is not None:
-        rq, (tq, nq, hq) = _rows(name, "q", q)
+        rq, (tq, nq, hq) = _rows(name, "q", q, dev)
         if tq != T or hq != hd:
             _fail(name, ": q must be [tokens, num_q_heads, head_dim]")
-    B = block_table.size(0)
     start_at = _int32(name, "start", start, B, dev)
     cu_at = None
     if cu_seqlens is not None:
         cu_at = _int32(name, "cu_seqlens", cu_seqlens, B + 1, dev)
     elif T != B:
         _fail(name, ": without cu_seqlens there must be one token per sequence")
-    for t, what in ((cos_table, "cos_table"), (sin_table, "sin_table")):
-        if not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or t.size(1) != hd // 2:
-            _fail(name, f"({what}): must be a contiguous float32 CUDA tensor [max_pos, head_dim / 2]")
-    rows = cos_table.size(0)
-    if rows != sin_table.size(0):
-        _fail(name, ": cos_table and sin_table must have the same shape")
-    norms = [None, None]
-    for i, t in enumerate((q_norm, k_norm)):
-        if t is not None:
-            norms[i] = t.data_ptr()
-            if not t.is_cuda or t.dtype != _F16 or t.numel() != hd or not t.is_contiguous() or norms[i] % 16:
-                _fail(name, "(", ("q_norm", "k_norm")[i], "): must be a float16 CUDA tensor [head_dim], 16-byte aligned")
-    for t in (q, v, cos_table, sin_table, q_norm, k_norm):
-        if t is not None and t.get_device() != dev:
-            _fail(name, ": all tensors must be on the same CUDA device")
+    table = cos_table.shape
+    if (cos_table.dtype is not _F32 or sin_table.dtype is not _F32 or cos_table.get_device() != dev
+            or sin_table.get_device() != dev or len(table) != 2 or table[1] != hd // 2 or sin_table.shape != table
+            or not cos_table.is_contiguous() or not sin_table.is_contiguous()):
+        _fail(name, ": cos_table / sin_table must be contiguous float32 tensors [max_pos, head_dim / 2] on the same CUDA "
+                    "device")
+    q_norm_at = _norm_at(name, "q_norm", q_norm, hd, dev) if q_norm is not None else None
+    k_norm_at = _norm_at(name, "k_norm", k_norm, hd, dev) if k_norm is not None else None
+    q_at = k_at = None
     if q is not None:
         q_out = k.new_empty((T, nq, hd))
+        q_at = q_out.data_ptr()
     if return_k:
         k_out = k.new_empty((T, nkv, hd))
-    if T == 0:
-        return q_out, k_out
-    _call_on(dev, "soinfer_paged_kv_append", cache, rq, rk, rv, q_out.data_ptr() if nq else None,
-             k_out.data_ptr() if return_k else None, T, nq, B, cu_at, start_at, cos_table.data_ptr(), sin_table.data_ptr(),
-             rows, norms[0], norms[1], eps)
+        k_at = k_out.data_ptr()
+    if T:
+        _call_on(dev, "soinfer_paged_kv_append", cache, rq, rk, rv, q_at, k_at, T, nq, B, cu_at, start_at,
+                 cos_table.data_ptr(), sin_table.data_ptr(), table[0], q_norm_at, k_norm_at, eps)
     return q_out, k_out
+
+
+def _norm_at(name: str, what: str, t, hd: int, dev: int) -> int:
+    at = t.data_ptr()
+    if t.dtype is not _F16 or t.get_device() != dev or t.numel() != hd or not t.is_contiguous() or at & 15:
+        _fail(name, "(", what, "): must be a float16 tensor [head_dim] on the same CUDA device, 16-byte aligned")
+    return at
 
 
 def paged_kv_read(k_pages, v_pages, block_table, cu_seqlens, total: int, out=None):
     name = "paged_kv_read"
     dev = k_pages.get_device()
-    cache, nkv, hd = _paged_cache(name, k_pages, v_pages, block_table, dev)
-    B = block_table.size(0)
+    cache, nkv, hd, _, B = _paged_cache(name, k_pages, v_pages, block_table, dev)
     cu_at = _int32(name, "cu_seqlens", cu_seqlens, B + 1, dev)
     if total < 0:
         _fail(name, ": total must be >= 0")
-    ko, vo = (_out_rows(name, t, k_pages, (total, nkv, hd)) for t in (out if out is not None else (None, None)))
+    ko, vo = out if out is not None else (None, None)
+    ko = _out_rows(name, ko, k_pages, (total, nkv, hd))
+    vo = _out_rows(name, vo, k_pages, (total, nkv, hd))
     if total:
         _call_on(dev, "soinfer_paged_kv_read", cache, cu_at, B, total, ko.data_ptr(), vo.data_ptr())
     return ko, vo
@@ -1049,17 +1064,18 @@ def paged_kv_read(k_pages, v_pages, block_table, cu_seqlens, total: int, out=Non
 
 def paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, out=None) -> torch.Tensor:
     name = "paged_decode_attention"
-    rq, (B, nq, hd) = _rows(name, "q", q)
     dev = q.get_device()
-    cache, nkv, _ = _paged_cache(name, k_pages, v_pages, block_table, dev, hd)
+    rq, shape = _rows(name, "q", q, dev)
+    B, nq, hd = shape
+    cache, nkv, _, page, seqs = _paged_cache(name, k_pages, v_pages, block_table, dev, hd)
     if nkv < 1 or nq < 1 or nq % nkv:
         _fail(name, ": num_q_heads must be a multiple of num_kv_heads")
-    if block_table.size(0) != B:
+    if seqs != B:
         _fail(name, ": block_table must have one row per query")
     lens_at = _int32(name, "seq_lens", seq_lens, B, dev)
-    out = _out_rows(name, out, q, (B, nq, hd))
+    out = _out_rows(name, out, q, shape)
     if B:
-        nbytes = lib().soinfer_paged_decode_workspace_bytes(B, nq, nkv, hd, block_table.size(1) * k_pages.size(2))
+        nbytes = (_lib or lib()).soinfer_paged_decode_workspace_bytes(B, nq, nkv, hd, block_table.shape[1] * page)
         # a workspace of the call's own: two captured graphs or streams never share one
         ws = q.new_empty((nbytes // 2,)) if nbytes else None
         _call_on(dev, "soinfer_paged_decode_attention", cache, rq, out.data_ptr(), B, nq, lens_at,
@@ -1069,11 +1085,13 @@ def paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, out=None)
 
 def prefill_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None) -> torch.Tensor:
     name = "prefill_attention"
-    rq, (Tq, nq, hd) = _rows(name, "q", q)
-    rk, ks = _rows(name, "k", k)
-    rv, vs = _rows(name, "v", v)
-    Tk, nkv, _ = ks
-    if vs != ks or ks[2] != hd:
+    dev = q.get_device()
+    rq, qs = _rows(name, "q", q, dev)
+    rk, ks = _rows(name, "k", k, dev)
+    rv, vs = _rows(name, "v", v, dev)
+    Tq, nq, hd = qs
+    Tk, nkv, hk = ks
+    if vs != ks or hk != hd:
         _fail(name, ": k / v must be [tokens, num_kv_heads, head_dim]")
     if hd not in PAGED_HEAD_DIMS:
         _fail(name, ": head_dim must be 64 or 128")
@@ -1083,9 +1101,6 @@ def prefill_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None) -> torch
         # rows are loaded as boxes of a tensor map, which has no zero strides (an expanded dimension)
         if 0 in x.stride() and any(n > 1 and st == 0 for n, st in zip(x.shape, x.stride())):
             return prefill_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu_seqlens, cu_seqlens_k, out)
-    dev = q.get_device()
-    if k.get_device() != dev or v.get_device() != dev:
-        _fail(name, ": all tensors must be on the same CUDA device")
     n = cu_seqlens.numel()
     if n < 1:
         _fail(name, "(cu_seqlens): must be [num_seqs + 1]")
@@ -1096,7 +1111,7 @@ def prefill_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None) -> torch
         cu_k_at = cu_at
         if Tk != Tq:
             _fail(name, ": without cu_seqlens_k, q and k must have the same tokens")
-    out = _out_rows(name, out, q, (Tq, nq, hd))
+    out = _out_rows(name, out, q, qs)
     if Tq:
         _call_on(dev, "soinfer_prefill_attention", rq, rk, rv, out.data_ptr(), Tq, Tk, n - 1, cu_at, cu_k_at, nq, nkv, hd)
     return out
