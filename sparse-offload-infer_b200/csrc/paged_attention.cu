@@ -24,9 +24,11 @@
 //   order; a sequence of one chunk is finished in place.
 // A CTA has four warps, each with every fourth tile of the CTA's positions; they are joined in shared memory.
 //
-// Feeding: each warp has its own ring of tiles in shared memory, filled by bulk copies (one per run of positions inside a
-// page: codes and scales of a small page are one piece) and waited for on a barrier per tile, so loads run ahead and the
-// registers hold only what is being multiplied.  Waits are bounded.
+// Feeding: each warp has its own ring of tiles in shared memory, so loads run ahead and the registers hold only what is being
+// multiplied.  4 bits: bulk copies, one per run of positions inside a page and kind (codes and scales of a small page are
+// one piece), waited for on a barrier per tile (bounded).  fp16: 16-byte asynchronous copies, whose places are exchanged
+// within 128 bytes by row, since rows of 256 bytes end to end put the lanes of a load on the same banks (8 sequences of up
+// to 4096, 4 kv heads: bulk copies without exchange 15.5 us, a bulk copy per padded row 18.2, this @F16@).
 #include "launch.cuh"
 #include "paged_cache.cuh"
 
@@ -124,6 +126,26 @@ __device__ __forceinline__ void lds_words(uint32_t* d, const uint8_t* p) {
   }
 }
 
+// Where a tile of fp16 rows holds 16-byte piece c of key (value) row p: two neighbouring key rows, or four value rows two
+// apart, are read at a time.
+template <int HD>
+__device__ __forceinline__ int key_at(int p, int c) {
+  return p * (2 * HD) + ((c ^ (p & 1) << 2) << 4);
+}
+template <int HD>
+__device__ __forceinline__ int value_at(int p, int c) {
+  return p * (2 * HD) + ((c ^ (p & 6)) << 4);
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Scores of the 16 positions at slot0: D rows are positions g and g + 8, columns heads 2 t and 2 t + 1.
 template <int HD, bool Q4, int N>
 __device__ __forceinline__ void scores(float s[4], const Run<HD, Q4, N>& R, int slot0, const uint32_t (*qf)[4],
@@ -164,7 +186,7 @@ __device__ __forceinline__ void scores(float s[4], const Run<HD, Q4, N>& R, int 
     for (int j = 0; j < G; ++j) {
       uint32_t k[2][4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) lds_words<4>(k[r], R.k + (slot0 + g + 8 * r) * (2 * HD) + 64 * j + 16 * t);
+      for (int r = 0; r < 2; ++r) lds_words<4>(k[r], R.k + key_at<HD>(slot0 + g + 8 * r, 4 * j + t));
       const uint32_t a0[4] = {k[0][0], k[1][0], k[0][1], k[1][1]}, a1[4] = {k[0][2], k[1][2], k[0][3], k[1][3]};
       if (j == 0)
         mma_from(s, a0, qf[j][0], qf[j][1], 0.f, 0.f);
@@ -203,7 +225,7 @@ __device__ __forceinline__ void accumulate(float (*acc)[4], const Run<HD, Q4, N>
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int p = 2 * t + (r & 1) + 8 * (r >> 1);
-        lds_words<4>(v[r], R.v + (slot0 + p) * (2 * HD) + 128 * j + 16 * g);
+        lds_words<4>(v[r], R.v + value_at<HD>(slot0 + p, 8 * j + g));
         if (n_valid < 16 && p >= n_valid)
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[r][i] = 0;
@@ -317,18 +339,19 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
   const int p_begin = chunk * L, p_end = len - p_begin < L ? len : p_begin + L;
 
   // the ring: tile i of this warp starts at position p_begin + (warp + i kWarps) kTile and consists of runs of positions
-  // inside a page; lane c of the first lanes copies piece c % pieces of run c / pieces
+  // inside a page.  4 bits: lane c of the first lanes copies piece c % pieces of run c / pieces; fp16: one run, all lanes
   const int page = 1 << C.page_shift;
-  const bool whole = !Q4 || kRun == page;          // K (V) codes and scales of the run are one piece
-  const int pieces = whole ? 2 : 4, run = whole ? lane >> 1 : lane >> 2, piece = lane & (pieces - 1);
+  const bool whole = kRun == page;                 // 4-bit codes and scales of the run are one piece
+  const int pieces = whole ? 2 : 4, run = !Q4 ? 0 : whole ? lane >> 1 : lane >> 2, piece = lane & (pieces - 1);
   const int p_warp = p_begin + warp * kTile, stride = kWarps * kTile;
   const int tiles = p_warp < p_end ? (p_end - p_warp + stride - 1) / stride : 0;
-  // what this lane copies: from where in its page's block (bytes per slot), to where in the tile, how much
-  constexpr int kKeys = kRun * (Q4 ? HD / 2 + HD / 16 : 2 * HD), kCodes = kRun * (HD / 2);
-  int dst = run * kRunBytes + (piece & 1 ? kKeys : 0), src_step = Q4 ? 0 : 2 * HD;
-  int bytes = piece & 1 ? kRunBytes - kKeys : kKeys;
-  const uint8_t* src = piece & 1 ? C.v : C.k;
-  const int64_t block = piece & 1 ? v_block_bytes(page, HD, Q4) : k_block_bytes(page, HD, Q4);
+  const int64_t k_block = k_block_bytes(page, HD, Q4), v_block = v_block_bytes(page, HD, Q4);
+  // what this lane copies of 4-bit rows: from where in its page's block (bytes per slot), to where in the tile, how much
+  constexpr int kKeys = kRun * (HD / 2 + HD / 16), kCodes = kRun * (HD / 2);
+  const int64_t block = piece & 1 ? v_block : k_block;
+  const uint8_t* src = (piece & 1 ? C.v : C.k) + kvh * block;
+  int dst = (int)smem_u32(ring) + run * kRunBytes + (piece & 1 ? kKeys : 0);
+  int src_step = 0, bytes = piece & 1 ? kRunBytes - kKeys : kKeys;  // a whole page starts at its block
   if (!whole) {
     src_step = piece < 2 ? HD / 2 : piece == 2 ? HD / 16 : 2;
     bytes = kRun * src_step;
@@ -337,8 +360,6 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
       src += page * (HD / 2);
     }
   }
-  src += kvh * block;
-  dst += (int)smem_u32(ring);
   const int p_lane = p_warp + run * kRun;
   const bool copies = run < kRuns;
   auto page_id = [&](int i) {                      // page of this lane's run of tile i
@@ -347,27 +368,43 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
   };
   unsigned there = 0;                              // per ring slot, which runs hold data
   auto issue = [&](int i, int slot, int id) {
-    const unsigned on = __ballot_sync(0xffffffffu, id >= 0);
-    unsigned bits = on & 1u;  // (several runs: always two pieces each)
+    if constexpr (Q4) {
+      const unsigned on = __ballot_sync(0xffffffffu, id >= 0);
+      unsigned bits = on & 1u;                     // (several runs: always two pieces each)
 #pragma unroll
-    for (int r = 1; r < kRuns; ++r) bits |= (on >> (2 * r) & 1u) << r;
-    there = (there & ~(15u << (4 * slot))) | bits << (4 * slot);
-    if (lane == 0) mbar_arrive_expect_tx(&full[slot], __popc(bits) * kRunBytes);
-    __syncwarp();
-    if (id >= 0)
-      asm volatile(
-          "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + slot * kBytes),
-          "l"(src + (int64_t)id * C.nkv * block + ((p_lane + i * stride) & (page - 1)) * src_step), "r"(bytes),
-          "r"(smem_u32(&full[slot]))
-          : "memory");
+      for (int r = 1; r < kRuns; ++r) bits |= (on >> (2 * r) & 1u) << r;
+      there = (there & ~(15u << (4 * slot))) | bits << (4 * slot);
+      if (lane == 0) mbar_arrive_expect_tx(&full[slot], __popc(bits) * kRunBytes);
+      __syncwarp();
+      if (id >= 0)
+        asm volatile(
+            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                dst + slot * kBytes),
+            "l"(src + (int64_t)id * C.nkv * block + ((p_lane + i * stride) & (page - 1)) * src_step), "r"(bytes),
+            "r"(smem_u32(&full[slot]))
+            : "memory");
+    } else {
+      there = (there & ~(15u << (4 * slot))) | (id >= 0 ? 1u : 0u) << (4 * slot);
+      if (id >= 0) {
+        const int64_t at = ((int64_t)id * C.nkv + kvh) * k_block + ((p_lane + i * stride) & (page - 1)) * (2 * HD);
+        const uint32_t to = smem_u32(ring) + slot * kBytes;
+#pragma unroll
+        for (int o = lane; o < kTile * HD / 8; o += 32) {
+          copy16(to + key_at<HD>(o / (HD / 8), o % (HD / 8)), C.k + at + 16 * o);
+          copy16(to + kTile * 2 * HD + value_at<HD>(o / (HD / 8), o % (HD / 8)), C.v + at + 16 * o);
+        }
+      }
+    }
   };
   {
     int id[kStages];
 #pragma unroll
     for (int i = 0; i < kStages; ++i) id[i] = i < tiles ? page_id(i) : -1;
 #pragma unroll
-    for (int i = 0; i < kStages; ++i)
+    for (int i = 0; i < kStages; ++i) {
       if (i < tiles) issue(i, i, id[i]);
+      if (!Q4) copy_commit();
+    }
   }
   int next_id = kStages < tiles ? page_id(kStages) : -1;
 
@@ -404,13 +441,18 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
   int slot = 0;
   unsigned parity = 0;
   for (int i = 0; i < tiles; ++i) {
-    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[slot], parity, kTimeoutNs))) {
-      if (lane == 0) atomicOr(&g_paged_error, kErrCopyTimeout);
-      for (int o = 1; o < kStages && i + o < tiles; ++o) {  // the copies behind it, before the CTA may end
-        const int s = (slot + o) % kStages;
-        mbar_wait_bounded(&full[s], s < slot ? parity ^ 1 : parity, kTimeoutNs);
+    if constexpr (Q4) {
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[slot], parity, kTimeoutNs))) {
+        if (lane == 0) atomicOr(&g_paged_error, kErrCopyTimeout);
+        for (int o = 1; o < kStages && i + o < tiles; ++o) {  // the copies behind it, before the CTA may end
+          const int s = (slot + o) % kStages;
+          mbar_wait_bounded(&full[s], s < slot ? parity ^ 1 : parity, kTimeoutNs);
+        }
+        break;
       }
-      break;
+    } else {
+      copy_wait<kStages - 1>();
+      __syncwarp();
     }
     const int p0 = p_warp + i * stride;
     const unsigned held = there >> (4 * slot);
@@ -482,6 +524,7 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
       issue(i + kStages, slot, next_id);
       next_id = i + kStages + 1 < tiles ? page_id(i + kStages + 1) : -1;
     }
+    if (!Q4) copy_commit();
     if (++slot == kStages) slot = 0, parity ^= 1;
   }
 
