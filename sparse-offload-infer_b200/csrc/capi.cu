@@ -98,8 +98,6 @@ int soinfer_device_errors(int* flags) {
   *flags |= f;
   if (int st = cuda_result(read_and_clear_decode_fused_error(&f), "device_errors")) return st;
   *flags |= f;
-  if (int st = cuda_result(read_and_clear_paged_error(&f), "device_errors")) return st;
-  *flags |= f;
   if (int st = cuda_result(read_and_clear_prefill_error(&f), "device_errors")) return st;
   *flags |= f;
   return SOINFER_OK;

@@ -335,7 +335,6 @@ struct PagedDecodeParams {
 // Bytes for tables that name up to `positions` positions per sequence (0: none needed).
 int64_t paged_decode_workspace_bytes(int64_t seqs, int64_t nq, int64_t nkv, int64_t hd, int64_t positions);
 cudaError_t launch_paged_decode(const PagedDecodeParams& P, cudaStream_t stream);
-cudaError_t read_and_clear_paged_error(int* out);
 
 // Causal attention of packed prompts (prefill_attention.cu).
 struct PrefillParams {

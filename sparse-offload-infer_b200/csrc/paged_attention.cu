@@ -24,11 +24,10 @@
 //   order; a sequence of one chunk is finished in place.
 // A CTA has four warps, each with every fourth tile of the CTA's positions; they are joined in shared memory.
 //
-// Feeding: each warp has its own ring of tiles in shared memory, so loads run ahead and the registers hold only what is being
-// multiplied.  4 bits: bulk copies, one per run of positions inside a page and kind (codes and scales of a small page are
-// one piece), waited for on a barrier per tile (bounded).  fp16: 16-byte asynchronous copies, whose places are exchanged
-// within 128 bytes by row, since rows of 256 bytes end to end put the lanes of a load on the same banks (8 sequences of up
-// to 4096, 4 kv heads: bulk copies without exchange 15.5 us, a bulk copy per padded row 18.2, this @F16@).
+// Feeding: each warp has its own ring of tiles in shared memory, filled by 16-byte asynchronous copies, so loads run ahead and
+// the registers hold only what is being multiplied.  The pieces' places are exchanged within 128 bytes by row, since rows
+// that lie end to end put the lanes of a load on the same banks (fp16, 8 sequences of up to 4096, 4 kv heads: bulk copies
+// without exchange 15.5 us, a bulk copy per padded row 18.2, this 12.3).
 #include "launch.cuh"
 #include "paged_cache.cuh"
 
@@ -44,9 +43,6 @@ constexpr int kMostLen = 1 << 30;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;      // the running maximum follows when exceeded by 2^8 (it moves in a few tiles, not in half)
 constexpr float kLift = 7.f;      // factor 2^7 on the probabilities (it cancels)
-constexpr uint64_t kTimeoutNs = 1000000000ull;
-
-__device__ int g_paged_error;
 
 // Positions a warp takes at a time, tiles in its ring, CTAs that an SM holds (shared memory and registers).
 template <bool Q4>
@@ -57,9 +53,6 @@ struct Plan {
   static constexpr int kCtas = 148 * kPerSm;
   static constexpr int kMinChunk = kTile * kWarps;
 };
-template <int HD, bool Q4>
-constexpr int kTileBytes = Plan<Q4>::kTile * (Q4 ? HD / 2 + HD / 16 + HD / 2 + 2 : 4 * HD);
-
 // d = a b + c.
 __device__ __forceinline__ void mma_from(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1, float c0, float c1) {
   asm volatile(
@@ -106,11 +99,20 @@ __device__ __forceinline__ int chunk_len(const PagedDecodeParams& P, int units, 
   return (int)(c < kMin ? kMin : c > kMostLen ? kMostLen : c);
 }
 
-// A run of N positions of a tile in shared memory: 4 bits: K codes, K scales, V codes, V scales; fp16: K rows, V rows.
-template <int HD, bool Q4, int N>
-struct Run {
-  const uint8_t *k, *v;
-  __device__ __forceinline__ explicit Run(const uint8_t* at) : k(at), v(at + N * (Q4 ? HD / 2 + HD / 16 : 2 * HD)) {}
+// A tile in shared memory: key codes (rows), their scales, value codes (rows), their scales; where it holds 16-byte piece c
+// of a key row p and of a value row m (4 bits: a pair of positions): what a load of a quarter warp takes lies on all banks.
+template <int HD, bool Q4>
+struct Tile {
+  static constexpr int kTile = Plan<Q4>::kTile;
+  static constexpr int kKeyRow = Q4 ? HD / 2 : 2 * HD, kValueRow = Q4 ? HD : 2 * HD;
+  static constexpr int kScales = kTile * kKeyRow;  // offset of the key scales
+  static constexpr int kValues = kScales + (Q4 ? kTile * (HD / 16) : 0);
+  static constexpr int kValueScales = kValues + (Q4 ? kTile / 2 : kTile) * kValueRow;
+  static constexpr int kBytes = kValueScales + (Q4 ? 2 * kTile : 0);
+  static __device__ __forceinline__ int key(int p, int c) { return p * kKeyRow + ((Q4 ? c : c ^ (p & 1) << 2) << 4); }
+  static __device__ __forceinline__ int value(int m, int c) {
+    return kValues + m * kValueRow + ((c ^ (!Q4 ? m & 6 : HD == 128 ? (m & 3) << 1 : m & 2)) << 4);
+  }
 };
 
 template <int N>
@@ -126,17 +128,6 @@ __device__ __forceinline__ void lds_words(uint32_t* d, const uint8_t* p) {
   }
 }
 
-// Where a tile of fp16 rows holds 16-byte piece c of key (value) row p: two neighbouring key rows, or four value rows two
-// apart, are read at a time.
-template <int HD>
-__device__ __forceinline__ int key_at(int p, int c) {
-  return p * (2 * HD) + ((c ^ (p & 1) << 2) << 4);
-}
-template <int HD>
-__device__ __forceinline__ int value_at(int p, int c) {
-  return p * (2 * HD) + ((c ^ (p & 6)) << 4);
-}
-
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -147,9 +138,10 @@ __device__ __forceinline__ void copy_wait() {
 }
 
 // Scores of the 16 positions at slot0: D rows are positions g and g + 8, columns heads 2 t and 2 t + 1.
-template <int HD, bool Q4, int N>
-__device__ __forceinline__ void scores(float s[4], const Run<HD, Q4, N>& R, int slot0, const uint32_t (*qf)[4],
+template <int HD, bool Q4>
+__device__ __forceinline__ void scores(float s[4], const uint8_t* tile, int slot0, const uint32_t (*qf)[4],
                                        const float (*bias)[2], int g, int t) {
+  using T = Tile<HD, Q4>;
   constexpr int G = HD / 32;
   if constexpr (Q4) {
     const half2 k1032 = __floats2half2_rn(1032.f, 1032.f);
@@ -157,8 +149,8 @@ __device__ __forceinline__ void scores(float s[4], const Run<HD, Q4, N>& R, int 
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int p = slot0 + g + 8 * r;
-      lds_words<G>(k[r], R.k + p * (HD / 2) + t * (4 * G));
-      lds_words<G / 2>(ks[r], R.k + N * (HD / 2) + p * (2 * G));
+      lds_words<G>(k[r], tile + p * (HD / 2) + t * (4 * G));
+      lds_words<G / 2>(ks[r], tile + T::kScales + p * (2 * G));
     }
 #pragma unroll
     for (int j = 0; j < G; ++j) {
@@ -186,7 +178,7 @@ __device__ __forceinline__ void scores(float s[4], const Run<HD, Q4, N>& R, int 
     for (int j = 0; j < G; ++j) {
       uint32_t k[2][4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) lds_words<4>(k[r], R.k + key_at<HD>(slot0 + g + 8 * r, 4 * j + t));
+      for (int r = 0; r < 2; ++r) lds_words<4>(k[r], tile + T::key(slot0 + g + 8 * r, 4 * j + t));
       const uint32_t a0[4] = {k[0][0], k[1][0], k[0][1], k[1][1]}, a1[4] = {k[0][2], k[1][2], k[0][3], k[1][3]};
       if (j == 0)
         mma_from(s, a0, qf[j][0], qf[j][1], 0.f, 0.f);
@@ -199,16 +191,17 @@ __device__ __forceinline__ void scores(float s[4], const Run<HD, Q4, N>& R, int 
 
 // acc += V^T w.  w: weights of positions g, g + 8 (rows) for heads 2 t, 2 t + 1 (0 for positions that do not count);
 // n_valid positions of the 16 count: fp16 rows beyond them are taken as zeros.  acc[i] rows are values value_of(i, 0 / 1).
-template <int HD, bool Q4, int N>
-__device__ __forceinline__ void accumulate(float (*acc)[4], const Run<HD, Q4, N>& R, int slot0, const float w[4], int n_valid,
+template <int HD, bool Q4>
+__device__ __forceinline__ void accumulate(float (*acc)[4], const uint8_t* tile, int slot0, const float w[4], int n_valid,
                                            int g, int t) {
+  using T = Tile<HD, Q4>;
   uint32_t b[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) b[r] = transpose8x8(h2_as_u32(__floats2half2_rn(w[2 * r], w[2 * r + 1])));
   if constexpr (Q4) {
     uint32_t v[2][HD / 32];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) lds_words<HD / 32>(v[r], R.v + (slot0 / 2 + t + 4 * r) * HD + g * (HD / 8));
+    for (int r = 0; r < 2; ++r) lds_words<HD / 32>(v[r], tile + T::value(slot0 / 2 + t + 4 * r, g * (HD / 8) / 16) + g * (HD / 8) % 16);
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
       uint32_t x[2][4];  // values 4 i + (0..3) of the lane's, at position pairs t and t + 4
@@ -225,7 +218,7 @@ __device__ __forceinline__ void accumulate(float (*acc)[4], const Run<HD, Q4, N>
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int p = 2 * t + (r & 1) + 8 * (r >> 1);
-        lds_words<4>(v[r], R.v + value_at<HD>(slot0 + p, 8 * j + g));
+        lds_words<4>(v[r], tile + T::value(slot0 + p, 8 * j + g));
         if (n_valid < 16 && p >= n_valid)
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[r][i] = 0;
@@ -280,21 +273,13 @@ __device__ __forceinline__ float cluster_read(const float* p, int rank) {
 template <int HD, bool Q4, int kRuns, bool kJoined>
 __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
     paged_decode_kernel(const PagedDecodeParams P, const int groups, const float scale_log2) {
-  constexpr int G = HD / 32, kTile = Plan<Q4>::kTile, kSub = kTile / 16, kBytes = kTileBytes<HD, Q4>;
+  constexpr int G = HD / 32, kTile = Plan<Q4>::kTile, kSub = kTile / 16, kBytes = Tile<HD, Q4>::kBytes;
   constexpr int kStages = Plan<Q4>::kStages;
-  constexpr int kMin = Plan<Q4>::kMinChunk, kRun = kTile / kRuns, kRunBytes = kBytes / kRuns;
+  constexpr int kMin = Plan<Q4>::kMinChunk, kRun = kTile / kRuns;
   extern __shared__ __align__(128) uint8_t smem[];  // kWarps rings of kStages tiles, then the warps' results
-  __shared__ uint64_t s_full[kWarps][kStages];
   __shared__ float s_m[kWarps][kCols], s_l[kWarps][kCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  uint64_t* full = s_full[warp];
   uint8_t* ring = smem + warp * (kStages * kBytes);
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1);
-    fence_mbar_init();
-  }
-  __syncwarp();
   pdl_launch_dependents();
   pdl_wait();
   const PagedCache& C = P.cache;
@@ -339,59 +324,49 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
   const int p_begin = chunk * L, p_end = len - p_begin < L ? len : p_begin + L;
 
   // the ring: tile i of this warp starts at position p_begin + (warp + i kWarps) kTile and consists of runs of positions
-  // inside a page.  4 bits: lane c of the first lanes copies piece c % pieces of run c / pieces; fp16: one run, all lanes
+  // inside a page; lane r knows the page of run r
+  using T = Tile<HD, Q4>;
   const int page = 1 << C.page_shift;
-  const bool whole = kRun == page;                 // 4-bit codes and scales of the run are one piece
-  const int pieces = whole ? 2 : 4, run = !Q4 ? 0 : whole ? lane >> 1 : lane >> 2, piece = lane & (pieces - 1);
   const int p_warp = p_begin + warp * kTile, stride = kWarps * kTile;
   const int tiles = p_warp < p_end ? (p_end - p_warp + stride - 1) / stride : 0;
   const int64_t k_block = k_block_bytes(page, HD, Q4), v_block = v_block_bytes(page, HD, Q4);
-  // what this lane copies of 4-bit rows: from where in its page's block (bytes per slot), to where in the tile, how much
-  constexpr int kKeys = kRun * (HD / 2 + HD / 16), kCodes = kRun * (HD / 2);
-  const int64_t block = piece & 1 ? v_block : k_block;
-  const uint8_t* src = (piece & 1 ? C.v : C.k) + kvh * block;
-  int dst = (int)smem_u32(ring) + run * kRunBytes + (piece & 1 ? kKeys : 0);
-  int src_step = 0, bytes = piece & 1 ? kRunBytes - kKeys : kKeys;  // a whole page starts at its block
-  if (!whole) {
-    src_step = piece < 2 ? HD / 2 : piece == 2 ? HD / 16 : 2;
-    bytes = kRun * src_step;
-    if (piece & 2) {
-      dst += kCodes;
-      src += page * (HD / 2);
-    }
-  }
-  const int p_lane = p_warp + run * kRun;
-  const bool copies = run < kRuns;
-  auto page_id = [&](int i) {                      // page of this lane's run of tile i
-    const int p = p_lane + i * stride;
-    return copies && p < p_end ? page_of(C, b, p) : -1;
+  const uint32_t ring_at = smem_u32(ring);
+  auto page_id = [&](int i) {
+    const int p = p_warp + i * stride + lane * kRun;
+    return lane < kRuns && p < p_end ? page_of(C, b, p) : -1;
   };
   unsigned there = 0;                              // per ring slot, which runs hold data
-  auto issue = [&](int i, int slot, int id) {
-    if constexpr (Q4) {
-      const unsigned on = __ballot_sync(0xffffffffu, id >= 0);
-      unsigned bits = on & 1u;                     // (several runs: always two pieces each)
+  auto issue = [&](int i, int slot, int ids) {
+    const unsigned on = __ballot_sync(0xffffffffu, ids >= 0);
+    there = (there & ~(15u << (4 * slot))) | on << (4 * slot);
+    const uint32_t to = ring_at + slot * kBytes;
 #pragma unroll
-      for (int r = 1; r < kRuns; ++r) bits |= (on >> (2 * r) & 1u) << r;
-      there = (there & ~(15u << (4 * slot))) | bits << (4 * slot);
-      if (lane == 0) mbar_arrive_expect_tx(&full[slot], __popc(bits) * kRunBytes);
-      __syncwarp();
-      if (id >= 0)
-        asm volatile(
-            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                dst + slot * kBytes),
-            "l"(src + (int64_t)id * C.nkv * block + ((p_lane + i * stride) & (page - 1)) * src_step), "r"(bytes),
-            "r"(smem_u32(&full[slot]))
-            : "memory");
-    } else {
-      there = (there & ~(15u << (4 * slot))) | (id >= 0 ? 1u : 0u) << (4 * slot);
-      if (id >= 0) {
-        const int64_t at = ((int64_t)id * C.nkv + kvh) * k_block + ((p_lane + i * stride) & (page - 1)) * (2 * HD);
-        const uint32_t to = smem_u32(ring) + slot * kBytes;
+    for (int r = 0; r < kRuns; ++r) {
+      const int id = __shfl_sync(0xffffffffu, ids, r);
+      if (id < 0) continue;
+      const int slot0 = (p_warp + i * stride + r * kRun) & (page - 1);
+      const uint8_t* kb = C.k + ((int64_t)id * C.nkv + kvh) * k_block;
+      const uint8_t* vb = C.v + ((int64_t)id * C.nkv + kvh) * v_block;
+      const uint8_t* kc = kb + slot0 * T::kKeyRow;
+      const uint8_t* vc = vb + (Q4 ? slot0 / 2 : slot0) * T::kValueRow;
+      constexpr int kPieces = kRun * T::kKeyRow / 16, kKeyPieces = T::kKeyRow / 16, kValuePieces = T::kValueRow / 16;
+      static_assert(kPieces == (Q4 ? kRun / 2 : kRun) * kValuePieces, "keys and values have as many");
 #pragma unroll
-        for (int o = lane; o < kTile * HD / 8; o += 32) {
-          copy16(to + key_at<HD>(o / (HD / 8), o % (HD / 8)), C.k + at + 16 * o);
-          copy16(to + kTile * 2 * HD + value_at<HD>(o / (HD / 8), o % (HD / 8)), C.v + at + 16 * o);
+      for (int o0 = 0; o0 < kPieces; o0 += 32) {
+        const int o = o0 + lane;
+        copy16(to + T::key(r * kRun + o / kKeyPieces, o % kKeyPieces), kc + 16 * o);
+        copy16(to + T::value((Q4 ? r * kRun / 2 : r * kRun) + o / kValuePieces, o % kValuePieces), vc + 16 * o);
+      }
+      if constexpr (Q4) {
+        constexpr int kKeyScales = kRun * (HD / 16) / 16, kScales = kKeyScales + kRun * 2 / 16;
+        const uint8_t* ks = kb + page * (HD / 2) + slot0 * (HD / 16);
+        const uint8_t* vs = vb + page * (HD / 2) + slot0 * 2;
+#pragma unroll
+        for (int o0 = 0; o0 < kScales; o0 += 32) {
+          const int o = o0 + lane, n = o - kKeyScales;
+          if (o < kScales)
+            copy16(to + (n < 0 ? T::kScales + r * kRun * (HD / 16) + 16 * o : T::kValueScales + r * kRun * 2 + 16 * n),
+                   n < 0 ? ks + 16 * o : vs + 16 * n);
         }
       }
     }
@@ -403,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
       if (i < tiles) issue(i, i, id[i]);
-      if (!Q4) copy_commit();
+      copy_commit();
     }
   }
   int next_id = kStages < tiles ? page_id(kStages) : -1;
@@ -439,21 +414,9 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2 t, 2 t + 1
 
   int slot = 0;
-  unsigned parity = 0;
   for (int i = 0; i < tiles; ++i) {
-    if constexpr (Q4) {
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[slot], parity, kTimeoutNs))) {
-        if (lane == 0) atomicOr(&g_paged_error, kErrCopyTimeout);
-        for (int o = 1; o < kStages && i + o < tiles; ++o) {  // the copies behind it, before the CTA may end
-          const int s = (slot + o) % kStages;
-          mbar_wait_bounded(&full[s], s < slot ? parity ^ 1 : parity, kTimeoutNs);
-        }
-        break;
-      }
-    } else {
-      copy_wait<kStages - 1>();
-      __syncwarp();
-    }
+    copy_wait<kStages - 1>();
+    __syncwarp();
     const int p0 = p_warp + i * stride;
     const unsigned held = there >> (4 * slot);
     const uint8_t* tile = ring + slot * kBytes;
@@ -462,13 +425,11 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      const Run<HD, Q4, kRun> R(tile + 16 * u / kRun * kRunBytes);
-      const int slot0 = 16 * u % kRun;
-      scores<HD, Q4>(s[u], R, slot0, qf, bias, g, t);
+      scores<HD, Q4>(s[u], tile, 16 * u, qf, bias, g, t);
       if (Q4) {
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          sv[u][r] = __half2float(reinterpret_cast<const half*>(R.v + kRun * (HD / 2))[slot0 + g + 8 * r]);
+          sv[u][r] = __half2float(reinterpret_cast<const half*>(tile + T::kValueScales)[16 * u + g + 8 * r]);
       }
       if (!full_tile) {
 #pragma unroll
@@ -509,14 +470,13 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
     const float shift[2] = {m[0] == -INFINITY ? 0.f : kLift - m[0], m[1] == -INFINITY ? 0.f : kLift - m[1]};
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      const Run<HD, Q4, kRun> R(tile + 16 * u / kRun * kRunBytes);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[u][e] = ex2(fmaf(s[u][e], scale_log2, shift[e & 1]));
         l[e & 1] += s[u][e];
         if (Q4) s[u][e] *= sv[u][e >> 1];
       }
-      accumulate<HD, Q4>(acc, R, 16 * u % kRun, s[u], full_tile ? 16 : (held >> (16 * u / kRun) & 1) ? p_end - p0 - 16 * u : 0,
+      accumulate<HD, Q4>(acc, tile, 16 * u, s[u], full_tile ? 16 : (held >> (16 * u / kRun) & 1) ? p_end - p0 - 16 * u : 0,
                          g, t);
     }
     __syncwarp();  // every lane has read the tile
@@ -524,8 +484,8 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
       issue(i + kStages, slot, next_id);
       next_id = i + kStages + 1 < tiles ? page_id(i + kStages + 1) : -1;
     }
-    if (!Q4) copy_commit();
-    if (++slot == kStages) slot = 0, parity ^= 1;
+    copy_commit();
+    if (++slot == kStages) slot = 0;
   }
 
   // join the warps: lane (g, t) holds heads 2 t, 2 t + 1 and HD/8 of the values
@@ -657,7 +617,7 @@ template <int HD, bool Q4, int kRuns>
 cudaError_t decode_runs(const PagedDecodeParams& P, cudaStream_t stream) {
   const int groups = (int)head_groups(P.nq, P.cache.nkv), units = P.cache.nkv * groups;
   const float scale_log2 = (1.0f / sqrtf((float)HD)) * kLog2e;
-  constexpr int kSmem = kWarps * Plan<Q4>::kStages * kTileBytes<HD, Q4>;
+  constexpr int kSmem = kWarps * Plan<Q4>::kStages * Tile<HD, Q4>::kBytes;
   cudaError_t e;
   if (joined(P.cache.table_cols, P.cache.page_shift)) {
     if ((e = ensure_smem_attr<paged_decode_kernel<HD, Q4, kRuns, true>>(kSmem)) != cudaSuccess) return e;
@@ -695,13 +655,6 @@ int64_t paged_decode_workspace_bytes(int64_t seqs, int64_t nq, int64_t nkv, int6
 
 cudaError_t launch_paged_decode(const PagedDecodeParams& P, cudaStream_t stream) {
   return P.cache.hd == 128 ? decode_hd<128>(P, stream) : decode_hd<64>(P, stream);
-}
-
-cudaError_t read_and_clear_paged_error(int* out) {
-  cudaError_t e = cudaMemcpyFromSymbol(out, g_paged_error, sizeof(int));
-  if (e != cudaSuccess) return e;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(g_paged_error, &zero, sizeof(int));
 }
 
 }  // namespace soinfer
