@@ -280,8 +280,9 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
   __shared__ float s_m[kWarps][kCols], s_l[kWarps][kCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * (kStages * kBytes);
-  pdl_launch_dependents();
+  if (kJoined) pdl_launch_dependents();
   pdl_wait();
+  if (!kJoined) pdl_launch_dependents();  // not before the wait: the joining kernel reads the lengths as soon as it runs
   const PagedCache& C = P.cache;
   const int rep = P.nq / C.nkv, units = C.nkv * groups;
 
@@ -555,12 +556,10 @@ constexpr int kParts = 4;
 template <int HD, bool Q4>
 __global__ void __launch_bounds__(HD * kParts) paged_join_kernel(const PagedDecodeParams P, const int units) {
   __shared__ float s_num[kParts][HD], s_den[kParts];
-  pdl_launch_dependents();
-  pdl_wait();
   const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 31, part = threadIdx.x / HD, d = threadIdx.x % HD;
+  // the lengths are there: every CTA of the first kernel has waited for what came before it
   const int n = seq_len(P, b);
   const int L = chunk_len<Q4>(P, units, lane);
-  if (n <= L) return;  // finished by its only chunk
   int first = 0;
   for (int i = lane; i < b; i += 32) {
     const int x = seq_len(P, i);
@@ -568,6 +567,9 @@ __global__ void __launch_bounds__(HD * kParts) paged_join_kernel(const PagedDeco
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(0xffffffffu, first, o);
+  pdl_launch_dependents();
+  pdl_wait();
+  if (n <= L) return;  // finished by its only chunk
   const int count = (n + L - 1) / L, each = (count + kParts - 1) / kParts;
   const float* ws = P.ws + ((int64_t)first * P.nq + h) * (HD + 2);
   const int64_t step = (int64_t)P.nq * (HD + 2);
