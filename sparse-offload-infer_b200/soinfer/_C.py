@@ -890,6 +890,8 @@ def head_norm_rope(q, k, v, q_norm, k_norm, cos_vals, sin_vals, k_cache, v_cache
 _PAGED_CACHE = struct.Struct("PPPqqqqqqq")  # soinfer_paged_cache
 _ROWS = struct.Struct("Pqq")                # soinfer_rows
 PAGED_HEAD_DIMS = (64, 128)
+PAGED_CLUSTER_POSITIONS = 8192  # tables up to this many positions need no workspace (paged_attention.cu)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _F16, _F32, _U8, _I32 = torch.float16, torch.float32, torch.uint8, torch.int32
 
 
@@ -979,6 +981,8 @@ def _int32(name: str, what: str, t, n: int, dev: int) -> int:
 
 def _out_rows(name: str, out, like, shape) -> torch.Tensor:
     if out is None:
+        if like.shape == shape and like.is_contiguous() and like.dtype is _F16:
+            return torch.empty_like(like)
         return like.new_empty(shape, dtype=_F16)
     if not (out.is_cuda and out.dtype == _F16 and out.shape == shape and out.is_contiguous() and out.data_ptr() % 16 == 0):
         _fail(name, f": out must be a contiguous, 16-byte aligned float16 CUDA tensor of shape {shape}")
@@ -989,13 +993,13 @@ def _out_rows(name: str, out, like, shape) -> torch.Tensor:
 
 def _call_on(dev: int, fn_name: str, *args) -> None:
     """_call with the device's current stream as the last argument and the device current."""
-    if torch._C._cuda_getDevice() == dev:
-        status = getattr(_lib or lib(), fn_name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if _current_device() == dev:
+        status = getattr(_lib or lib(), fn_name)(*args, _raw_stream(dev))
         if status:
             _raise(status)
     else:
         with torch.cuda.device(dev):
-            _call(fn_name, *args, torch._C._cuda_getCurrentRawStream(dev))
+            _call(fn_name, *args, _raw_stream(dev))
 
 
 def paged_kv_append(q, k, v, k_pages, v_pages, block_table, start, cos_table, sin_table, cu_seqlens=None, q_norm=None,
@@ -1075,11 +1079,13 @@ def paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, out=None)
     lens_at = _int32(name, "seq_lens", seq_lens, B, dev)
     out = _out_rows(name, out, q, shape)
     if B:
-        nbytes = (_lib or lib()).soinfer_paged_decode_workspace_bytes(B, nq, nkv, hd, block_table.shape[1] * page)
-        # a workspace of the call's own: two captured graphs or streams never share one
-        ws = q.new_empty((nbytes // 2,)) if nbytes else None
-        _call_on(dev, "soinfer_paged_decode_attention", cache, rq, out.data_ptr(), B, nq, lens_at,
-                 ws.data_ptr() if nbytes else None, nbytes)
+        positions, nbytes, ws_at = block_table.shape[1] * page, 0, None
+        if positions > PAGED_CLUSTER_POSITIONS:
+            # a workspace of the call's own: two captured graphs or streams never share one
+            nbytes = lib().soinfer_paged_decode_workspace_bytes(B, nq, nkv, hd, positions)
+            ws = q.new_empty((nbytes // 2,))
+            ws_at = ws.data_ptr()
+        _call_on(dev, "soinfer_paged_decode_attention", cache, rq, out.data_ptr(), B, nq, lens_at, ws_at, nbytes)
     return out
 
 

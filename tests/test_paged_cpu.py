@@ -77,7 +77,9 @@ def test_read_decode_and_prefill_arguments():
     assert lib.soinfer_paged_kv_read(_cache(), P, 1, 0, None, None, None) == 0
     need = lib.soinfer_paged_decode_workspace_bytes(3, 8, 2, 128, 100_000)
     assert need >= 3 * 8 * 130 * 4 and lib.soinfer_paged_decode_workspace_bytes(3, 7, 2, 128, 100_000) == 0
-    assert lib.soinfer_paged_decode_workspace_bytes(3, 8, 2, 128, 64) == 0
+    # the front end asks for a workspace exactly where one is needed
+    assert lib.soinfer_paged_decode_workspace_bytes(3, 8, 2, 128, _C.PAGED_CLUSTER_POSITIONS) == 0
+    assert lib.soinfer_paged_decode_workspace_bytes(3, 8, 2, 128, _C.PAGED_CLUSTER_POSITIONS + 16) > 0
     d = lib.soinfer_paged_decode_attention
     long = dict(table_cols=10_000, table_stride=10_000)
     assert d(_cache(**long), _rows(), P, 3, 8, P, P, need - 1, None) == 1 and "workspace" in _err()
