@@ -70,28 +70,65 @@ __device__ __forceinline__ half scale_of(float amax) {
   return __float2half_rn(s < kMinScale ? kMinScale : s);
 }
 
-// Codes of four values against the fp16 scale s (inv = 1 / s), first value in the lowest nibble: rint(x / s), which
-// needs no clamp since s is at least (1 - 2^-11) of the largest magnitude's seventh; a non-finite s gives zeros.  x * inv
-// is within 2^-23 |x / s| < 1e-6 of the quotient, so it rounds alike unless it lies that near to a half, where the division
-// decides.  An integer is rounded to by adding 1.5 * 2^23; the nibbles are summed up as exact fp32 (v + 8 in base 16).
-__device__ __forceinline__ uint32_t codes_of(float x0, float x1, float x2, float x3, float s, float inv) {
-  const float x[4] = {x0, x1, x2, x3};
-  constexpr float kRound = 12582912.f, kUnit[4] = {1.f, 16.f, 256.f, 4096.f};
-  float r[4], far = 0.f;
+// Codes against the fp16 scale s (inv = 1 / s): rint(x / s), which needs no clamp since s is at least (1 - 2^-11) of the
+// largest magnitude's seventh.  x * inv is within 2^-23 |x / s| < 1e-6 of the quotient, so it rounds alike unless it lies
+// that near to a half, where the division decides.  An integer is rounded to by adding 1.5 * 2^23; digits r in base 16 are
+// summed up as exact fp32 numbers with 8 added to each, so that the low bits are the offset nibbles.
+constexpr float kDigits = 8388608.f + 8.f * (1.f + 16.f + 256.f + 4096.f);  // 2^23 + 0x8888
+
+// The rounded quotients of two values; far: the largest distance from an integer so far.
+__device__ __forceinline__ uint64_t quotients2(uint64_t x, uint64_t inv, float& far) {
+  const uint64_t y = mul2(x, inv);
+  const uint64_t r = add2(add2(y, both(12582912.f)), both(-12582912.f));
+  float d, e;
+  unpack2(fma2(r, both(-1.f), y), d, e);
+  far = fmaxf(far, fmaxf(fabsf(d), fabsf(e)));
+  return r;
+}
+__device__ __forceinline__ uint64_t divided2(uint64_t x, float s) {
+  float a, b;
+  unpack2(x, a, b);
+  return pack2(rintf(__fdiv_rn(a, s)), rintf(__fdiv_rn(b, s)));
+}
+// The four two's-complement nibbles whose digits v holds.
+__device__ __forceinline__ uint32_t nibbles(float v) { return (__float_as_uint(v) & 0xffffu) ^ 0x8888u; }
+
+// Key word of eight values x[4] (pairs of neighbours): value 2 i in nibble i, 2 i + 1 in nibble i + 4; a non-finite s gives
+// zeros.
+__device__ __forceinline__ uint32_t key_word(const uint64_t x[4], float s, float inv) {
+  constexpr float kUnit[4] = {1.f, 16.f, 256.f, 4096.f};
+  uint64_t r[4], v = both(kDigits);
+  float far = 0.f, lo, hi;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float y = __fmul_rn(x[i], inv);
-    r[i] = __fsub_rn(__fadd_rn(y, kRound), kRound);
-    far = fmaxf(far, fabsf(__fsub_rn(y, r[i])));
-  }
+  for (int i = 0; i < 4; ++i) r[i] = quotients2(x[i], both(inv), far);
   if (far > 0.499998f) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = rintf(__fdiv_rn(x[i], s));
+    for (int i = 0; i < 4; ++i) r[i] = divided2(x[i], s);
   }
-  float v = 8388608.f + 8.f * (1.f + 16.f + 256.f + 4096.f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v = fmaf(r[i], kUnit[i], v);
-  return s <= 65504.f ? (__float_as_uint(v) & 0xffffu) ^ 0x8888u : 0u;
+  for (int i = 0; i < 4; ++i) v = fma2(r[i], both(kUnit[i]), v);
+  unpack2(v, lo, hi);
+  return s <= 65504.f ? nibbles(lo) | nibbles(hi) << 16 : 0u;
+}
+
+// Value halves of eight values: the low 16 bits hold values 0..3 in order, the high ones values 4..7.
+__device__ __forceinline__ uint32_t value_word(const uint64_t x[4], float s, float inv) {
+  uint64_t r[4];
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = quotients2(x[i], both(inv), far);
+  if (far > 0.499998f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = divided2(x[i], s);
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float a, b;
+    unpack2(fma2(r[2 * i + 1], pack2(256.f, 4096.f), fma2(r[2 * i], pack2(1.f, 16.f), pack2(kDigits, 0.f))), a, b);
+    w[i] = nibbles(a + b);
+  }
+  return s <= 65504.f ? w[0] | w[1] << 16 : 0u;
 }
 
 // The larger magnitude, NaN if either is NaN.

@@ -9,16 +9,15 @@ namespace {
 
 constexpr int kWarps = 4;  // warps per CTA
 
-__device__ __forceinline__ void unpack8(const uint4& u, float x[8]) {
+// Eight fp16 values as pairs of fp32, and back.
+__device__ __forceinline__ void unpack8(const uint4& u, uint64_t x[4]) {
   const half2* p = reinterpret_cast<const half2*>(&u);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = __half22float2(p[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
+    x[i] = pack2(f.x, f.y);
   }
 }
-
 __device__ __forceinline__ uint4 pack8(const float x[8]) {
   uint4 u;
   half2* p = reinterpret_cast<half2*>(&u);
@@ -26,17 +25,27 @@ __device__ __forceinline__ uint4 pack8(const float x[8]) {
   for (int i = 0; i < 4; ++i) p[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
   return u;
 }
+__device__ __forceinline__ uint4 pack8(const uint64_t x[4]) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack2(x[i], f[2 * i], f[2 * i + 1]);
+  return pack8(f);
+}
 
-__device__ __forceinline__ float amax8(const float x[8]) {
+__device__ __forceinline__ float amax8(const uint64_t x[4]) {
   float a = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = amax_nan(a, x[i]);
+  for (int i = 0; i < 4; ++i) {
+    float f, g;
+    unpack2(x[i], f, g);
+    a = amax_nan(amax_nan(a, f), g);
+  }
   return a;
 }
 
 // Stores this lane's keys (x[half]: values half hd/2 + 8 l ..) of one position; the lanes of a row take part.
 template <int HD>
-__device__ __forceinline__ void store_key_q4(uint8_t* block, int page, int slot, int l, bool on, const float (*x)[8]) {
+__device__ __forceinline__ void store_key_q4(uint8_t* block, int page, int slot, int l, bool on, const uint64_t (*x)[4]) {
   constexpr int G = HD / kKGroup;
 #pragma unroll
   for (int f = 0; f < 2; ++f) {
@@ -44,9 +53,8 @@ __device__ __forceinline__ void store_key_q4(uint8_t* block, int page, int slot,
     a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));  // the 4 lanes of a 32-value group
     a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
     const half sh = scale_of(a);
-    const float s = __half2float(sh), inv = __fdiv_rn(1.f, s);
-    const uint32_t w = codes_of(x[f][0], x[f][2], x[f][4], x[f][6], s, inv) |
-                       codes_of(x[f][1], x[f][3], x[f][5], x[f][7], s, inv) << 16;
+    const float s = __half2float(sh);
+    const uint32_t w = key_word(x[f], s, __fdiv_rn(1.f, s));
     if (!on) continue;
     const int j = f * (G / 2) + (l >> 2), t = l & 3;
     *reinterpret_cast<uint32_t*>(block + (int64_t)slot * (HD / 2) + 4 * (t * G + j)) = w;
@@ -56,7 +64,7 @@ __device__ __forceinline__ void store_key_q4(uint8_t* block, int page, int slot,
 
 // Stores this lane's values of one position.
 template <int HD>
-__device__ __forceinline__ void store_value_q4(uint8_t* block, int page, int slot, int l, bool on, const float (*x)[8]) {
+__device__ __forceinline__ void store_value_q4(uint8_t* block, int page, int slot, int l, bool on, const uint64_t (*x)[4]) {
   float a = amax_nan(amax8(x[0]), amax8(x[1]));
 #pragma unroll
   for (int o = 1; o < HD / 16; o <<= 1) a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
@@ -64,12 +72,11 @@ __device__ __forceinline__ void store_value_q4(uint8_t* block, int page, int slo
   const float s = __half2float(sh), inv = __fdiv_rn(1.f, s);
 #pragma unroll
   for (int f = 0; f < 2; ++f) {
-    const uint32_t w[2] = {codes_of(x[f][0], x[f][1], x[f][2], x[f][3], s, inv),
-                           codes_of(x[f][4], x[f][5], x[f][6], x[f][7], s, inv)};
+    const uint32_t w = value_word(x[f], s, inv);
     if (!on) continue;
     uint8_t* at = block + (int64_t)(slot >> 1) * HD + f * (HD / 2) + 8 * l + 2 * (slot & 1);
-    *reinterpret_cast<uint16_t*>(at) = (uint16_t)w[0];
-    *reinterpret_cast<uint16_t*>(at + 4) = (uint16_t)w[1];
+    *reinterpret_cast<uint16_t*>(at) = (uint16_t)w;
+    *reinterpret_cast<uint16_t*>(at + 4) = (uint16_t)(w >> 16);
   }
   if (on && l == 0) reinterpret_cast<half*>(block + (int64_t)page * (HD / 2))[slot] = sh;
 }
@@ -129,15 +136,15 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
   uint8_t* k_base = P.cache.k + (int64_t)id * P.nkv * k_block;
   uint8_t* v_base = P.cache.v + (int64_t)id * P.nkv * v_block;
 
-  float c[8], sn[8];
+  uint64_t c[4], sn[4];  // pairs, as the rows'
   {
     const int64_t row = (placed ? pos : 0) * (HD / 2) + 8 * l;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float4 a = __ldg(reinterpret_cast<const float4*>(P.cos_t + row) + i);
       const float4 e = __ldg(reinterpret_cast<const float4*>(P.sin_t + row) + i);
-      c[4 * i] = a.x, c[4 * i + 1] = a.y, c[4 * i + 2] = a.z, c[4 * i + 3] = a.w;
-      sn[4 * i] = e.x, sn[4 * i + 1] = e.y, sn[4 * i + 2] = e.z, sn[4 * i + 3] = e.w;
+      c[2 * i] = pack2(a.x, a.y), c[2 * i + 1] = pack2(a.z, a.w);
+      sn[2 * i] = pack2(e.x, e.y), sn[2 * i + 1] = pack2(e.z, e.w);
     }
   }
 
@@ -145,7 +152,7 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
     uint4 cur[R][2];
 #pragma unroll
     for (int r = 0; r < R; ++r) cur[r][0] = raw[r][0], cur[r][1] = raw[r][1];
-    if (R > 1 && s1 + R < s_end)
+    if (s1 + R < s_end)
 #pragma unroll
       for (int r = 0; r < R; ++r) load(s1 + R + r, raw[r]);
 #pragma unroll
@@ -156,7 +163,8 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
       const int h = (is_q ? s : is_k ? s - q_steps : s - q_steps - kv_steps) * kRows + sub;
       const bool on = h < (is_q ? P.nq : P.nkv);
       const bool cached = on && id >= 0;
-      float x[2][8];
+      if (!placed) cur[r][0] = cur[r][1] = make_uint4(0, 0, 0, 0);
+      uint64_t x[2][4];
       unpack8(cur[r][0], x[0]);
       unpack8(cur[r][1], x[1]);
       if (!is_q && !is_k) {
@@ -172,20 +180,29 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
       }
       const half* w = is_q ? P.q_norm : P.k_norm;
       if (w) {
-        float inv, wf[2][8];
+        float inv;
+        uint64_t wf[2][4];
         unpack8(__ldg(reinterpret_cast<const uint4*>(w) + l), wf[0]);
         unpack8(__ldg(reinterpret_cast<const uint4*>(w) + kLanes + l), wf[1]);
         if (is_q) {
-          float ss = 0.f;
+          uint64_t ss2 = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) ss = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], ss));
+          for (int i = 0; i < 4; ++i) ss2 = fma2(x[0][i], x[0][i], fma2(x[1][i], x[1][i], ss2));
+          float ss, other;
+          unpack2(ss2, ss, other);
+          ss += other;
 #pragma unroll
           for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
           inv = rsqrtf(ss / (float)HD + P.eps);
         } else {
           double ss = 0.0;  // the squares are exact in fp32
 #pragma unroll
-          for (int i = 0; i < 8; ++i) ss += (double)__fmul_rn(x[0][i], x[0][i]) + (double)__fmul_rn(x[1][i], x[1][i]);
+          for (int i = 0; i < 4; ++i) {
+            float a, b, c2, d;
+            unpack2(mul2(x[0][i], x[0][i]), a, b);
+            unpack2(mul2(x[1][i], x[1][i]), c2, d);
+            ss += ((double)a + (double)b) + ((double)c2 + (double)d);
+          }
 #pragma unroll
           for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
           // 1 / sqrt by Newton's iteration r += r (1 - a r^2) / 2 from the fp32 value: 2^-22 -> 2^-43 -> 64-bit rounding
@@ -198,13 +215,19 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[f][i] = __fmul_rn(__fmul_rn(x[f][i], inv), wf[f][i]);
+          for (int i = 0; i < 4; ++i) x[f][i] = mul2(mul2(x[f][i], both(inv)), wf[f][i]);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float a = x[0][i], e = x[1][i];
-        x[0][i] = placed ? __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(e, sn[i])) : 0.f;
-        x[1][i] = placed ? __fadd_rn(__fmul_rn(e, c[i]), __fmul_rn(a, sn[i])) : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        // (sums one by one: products and sums of pairs may be contracted, which these must not be)
+        const uint64_t a = x[0][i], e = x[1][i];
+        float p0, p1, q0, q1;
+        unpack2(mul2(a, c[i]), p0, p1);
+        unpack2(mul2(e, sn[i]), q0, q1);
+        x[0][i] = pack2(__fsub_rn(p0, q0), __fsub_rn(p1, q1));
+        unpack2(mul2(e, c[i]), p0, p1);
+        unpack2(mul2(a, sn[i]), q0, q1);
+        x[1][i] = pack2(__fadd_rn(p0, q0), __fadd_rn(p1, q1));
       }
       const uint4 lo = pack8(x[0]), hi = pack8(x[1]);
       half* out = is_q ? P.q_out + ((int64_t)t * P.nq + h) * HD : P.k_out + ((int64_t)t * P.nkv + h) * HD;
@@ -351,7 +374,7 @@ cudaError_t append_hd(const PagedAppendParams& P, cudaStream_t stream) {
   const int parts = (steps + per - 1) / per;
   per = (steps + parts - 1) / parts;
   const int64_t warps = (int64_t)P.tokens * ((steps + per - 1) / per);
-  return launch_ex(per > 1 ? paged_append_kernel<HD, Q4, 2> : paged_append_kernel<HD, Q4, 1>,
+  return launch_ex(per > 1 && !Q4 ? paged_append_kernel<HD, Q4, 2> : paged_append_kernel<HD, Q4, 1>,
                    dim3((unsigned)((warps + kWarps - 1) / kWarps)), dim3(32 * kWarps), 0, stream, 1, true, P, per);
 }
 
