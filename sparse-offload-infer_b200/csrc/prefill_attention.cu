@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
     const uint32_t S = lanes + s * kTile, O = lanes + kO + s * HD;
     const bool valid = row < w.lq;
-    int limit = valid ? row + 1 + w.lk - w.lq : 0;  // keys this row sees
-    if (limit < 0) limit = 0;
+    // keys this row sees; a row behind the last one is worked on as that one (with none it would mask every tile) and dropped
+    const int limit = max(min(row, w.lq - 1) + 1 + w.lk - w.lq, 0);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < tiles && ok; ++j) {
@@ -277,9 +277,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (__any_sync(0xffffffffu, left < kTile)) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
+          if (__any_sync(0xffffffffu, left < 32 * c + 32)) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * c + i >= left) x[c][i] = 0xff800000u;  // -inf
+            for (int i = 0; i < 32; ++i)
+              if (32 * c + i >= left) x[c][i] = 0xff800000u;  // -inf
+          }
       }
       float tops[8];
 #pragma unroll
