@@ -31,9 +31,11 @@
 // Measured (8192 tokens, 40 / 8 heads, hd 128): products issued from a single lane's branch 832 us, maxima over eight chains
 // and packed pairs 685, products issued by a convergent warp 600, registers / halves / fp32 pipe / coalesced output 565 =
 // 1215 TFLOP/s, 0.75 of the measured burst rate of a library product and 0.88 of its sustained one, whose power limit this
-// kernel reaches too.  7 unequal prompts (3828 tokens, 16 / 8 heads): 32 us, the longest one's 12 steps of 1.9 us plus 6 us
-// of start and end.  One in eight / three in eight / half of the pairs on the fp32 pipe: 31.6 / 31.7 / 32.3 us against 31.2
-// there.
+// kernel reaches too.  7 unequal prompts (3828 tokens, 16 / 8 heads): 29 us, the longest one's 12 steps of 1.6 us plus 6 us
+// of start and end and a second round of CTAs.  One in eight / three in eight / half of the pairs on the fp32 pipe: 31.6 /
+// 31.7 / 32.3 us against 31.2 there.  hd 64, two chunks of 512 and 1000 rows over 4012 and 3047 keys, 32 / 4 heads: 73 us,
+// 192 CTAs in two rounds; P beside S in the tensor memory, so that scores run ahead, measured the same (the two warps of a
+// scheduler spend their exponentials' phases together).
 #include <cuda.h>
 
 #include "common.cuh"
