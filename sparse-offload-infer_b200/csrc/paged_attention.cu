@@ -435,24 +435,29 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
       scores<HD, Q4>(s[u], tile, 16 * u, qf, bias, g, t);
+      uint32_t scale[2];  // fp16 bits
       if (Q4) {
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          sv[u][r] = __half2float(reinterpret_cast<const half*>(tile + T::kValueScales)[16 * u + g + 8 * r]);
+          scale[r] = reinterpret_cast<const uint16_t*>(tile + T::kValueScales)[16 * u + g + 8 * r];
       }
       if (!full_tile) {
 #pragma unroll
         for (int r = 0; r < 2; ++r)
           if (!(p0 + 16 * u + g + 8 * r < p_end && (held >> (16 * u / kRun) & 1))) {
             s[u][2 * r] = s[u][2 * r + 1] = -INFINITY;
-            sv[u][r] = 1.f;
+            scale[r] = 0x3c00;
           }
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        // exponent of the scale, rounded up: scale * 2^-e < 1 (an integer put into a float's mantissa)
+        // exponent of the scale, rounded up: scale * 2^-e < 1 (an integer put into a float's mantissa); -14 for the scale 0 of
+        // zeroed pages, whose weights stay finite so
         float e = 0.f;
-        if (Q4) e = __uint_as_float(__float_as_uint(sv[u][r]) >> 23 | 0x4b000000u) - (8388608.f + 126.f);
+        if (Q4) {
+          e = __uint_as_float(scale[r] >> 10 | 0x4b000000u) - (8388608.f + 14.f);
+          sv[u][r] = __half2float(__ushort_as_half((unsigned short)scale[r]));
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], fmaf(s[u][2 * r + c], scale_log2, e));
       }

@@ -291,6 +291,24 @@ def test_decode_attention_over_missing_pages_and_odd_lengths(bits):
     assert torch.count_nonzero(got[1:3]) == 0
 
 
+@pytest.mark.parametrize("cols", [70, 640])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_decode_attention_over_pages_as_allocated(bits, cols):
+    """Zeroed pages hold zero keys and values (4 bits: with the scale 0), alone and next to written rows."""
+    lens, page, nq, nkv, hd = [1, 40, 1000], 16, 6, 2, 128
+    table, pages = _table([cols * page] * 3, page, 4)
+    pools = ops.paged_kv_alloc(pages, nkv, page, hd, bits, device=DEV)
+    q = torch.randn(3, nq, hd, generator=_gen(6)).half().to(DEV)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    assert torch.count_nonzero(ops.paged_decode_attention(q, *pools, table.to(DEV), lens_d)) == 0
+    k, v = (torch.randn(30, nkv, hd, generator=_gen(7)).half().to(DEV) for _ in range(2))
+    one = torch.ones(1000, hd // 2, device=DEV)
+    start = torch.tensor([0, 5, 500], dtype=torch.int32, device=DEV)
+    ops.paged_kv_append(None, k, v, *pools, table.to(DEV), start, one, 0 * one, cu_seqlens=_cum([0, 10, 20]))
+    got = ops.paged_decode_attention(q, *pools, table.to(DEV), lens_d)
+    _check_decode(got, q, pools, bits, table, lens, pages)
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_decode_attention_captured_replayed_and_repeatable(bits):
     """A captured call follows the lengths it finds at replay; two graphs on one pool do not share scratch; the same
