@@ -241,6 +241,11 @@ __device__ __forceinline__ void accumulate(float (*acc)[4], const uint8_t* tile,
   }
 }
 
+// The output.  Without positions the sum of weights is 0; else it is at least 2^(7 - 16) (the weight of the position whose
+// score and scale, below 2^16, set the maximum), or NaN: a NaN of the query or of a key never becomes the maximum, but its
+// weight is one.
+__device__ __forceinline__ half result(float num, float den) { return __float2half_rn(den == 0.f ? 0.f : num / den); }
+
 // Value index of row half r (0: row g, 1: row g + 8) of accumulator i.
 template <int HD, bool Q4>
 __device__ __forceinline__ int value_of(int i, int r, int g) {
@@ -544,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
         den = fmaf(f, cluster_read(row + HD + 1, r), den);
         num = fmaf(f, cluster_read(row + d, r), num);
       }
-      P.out[((int64_t)b * P.nq + qh0 + h) * HD + d] = __float2half_rn(M == -INFINITY ? 0.f : num / den);
+      P.out[((int64_t)b * P.nq + qh0 + h) * HD + d] = result(num, den);
     }
     cluster_sync();  // nobody leaves while its sums are read
   } else {
@@ -553,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
       float num, den, M;
       join_warps<HD>(s_acc, s_m, s_l, h, d, num, den, M);
       if (count == 1) {
-        P.out[((int64_t)b * P.nq + qh0 + h) * HD + d] = __float2half_rn(M == -INFINITY ? 0.f : num / den);
+        P.out[((int64_t)b * P.nq + qh0 + h) * HD + d] = result(num, den);
       } else {
         float* ws = P.ws + ((int64_t)blockIdx.y * P.nq + qh0 + h) * (HD + 2);
         ws[d] = num;
@@ -614,7 +619,7 @@ __global__ void __launch_bounds__(HD * kParts) paged_join_kernel(const PagedDeco
     num += s_num[i][d];
     den += s_den[i];
   }
-  P.out[((int64_t)b * P.nq + h) * HD + d] = __float2half_rn(M == -INFINITY ? 0.f : num / den);
+  P.out[((int64_t)b * P.nq + h) * HD + d] = result(num, den);
 }
 
 // Chunks of any lengths: sum over sequences of max(1, ceil(len / L)) with L >= total * units / CTAs.

@@ -309,6 +309,39 @@ def test_decode_attention_over_pages_as_allocated(bits, cols):
     _check_decode(got, q, pools, bits, table, lens, pages)
 
 
+@pytest.mark.parametrize("cols", [80, 640])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_decode_attention_with_nan(bits, cols):
+    """A NaN in a query makes its head NaN and no other; in a cached key the heads that read it, if it lies within."""
+    lens, page, nq, nkv, hd = [777, 1, 300, 300], 16, 6, 2, 128
+    table, pages = _table(lens, page, 4, cols=cols)
+    pools = _pools(pages, nkv, page, hd, bits)
+    T, g = sum(lens), _gen(16)
+    q = torch.randn(4, nq, hd, generator=g).half()
+    k, v = (torch.randn(T, nkv, hd, generator=g).half().to(DEV) for _ in range(2))
+    k[778 + 123, 1, 70] = k[1078 + 299, 0, 5] = float("nan")
+    one = torch.ones(800, hd // 2, device=DEV)
+    ops.paged_kv_append(None, k, v, *pools, table.to(DEV), torch.zeros(4, dtype=torch.int32, device=DEV), one, 0 * one,
+                        cu_seqlens=_cum(lens))
+    bad = q.clone()
+    bad[0, 1, 3] = bad[1, 5, 100] = float("nan")
+    seen = [777, 1, 300, 299]  # the last sequence's NaN lies behind
+    got = ops.paged_decode_attention(bad.to(DEV), *pools, table.to(DEV), torch.tensor(seen, dtype=torch.int32, device=DEV))
+    for b, h in ((0, [1]), (1, [5]), (2, [3, 4, 5])):
+        assert torch.isnan(got[b, h]).all(), (b, h)
+        got[b, h] = 0
+    assert torch.isfinite(got).all()
+    pools = [torch.where(torch.isnan(t), 0, t) if bits == 16 else t for t in pools]
+    if bits == 4:  # the groups that the NaN made unreadable
+        ks = pools[0].view(pages, nkv, -1)[:, :, page * hd // 2 :].view(torch.float16)
+        ks[torch.isnan(ks)] = 0
+    want = ops.paged_decode_attention(q.to(DEV), *pools, table.to(DEV), torch.tensor(seen, dtype=torch.int32, device=DEV))
+    _check_decode(want, q, pools, bits, table, seen, pages)
+    for b, h in ((0, [1]), (1, [5]), (2, [3, 4, 5])):
+        want[b, h] = 0
+    torch.testing.assert_close(got.float(), want.float(), rtol=4 * 2.0**-11, atol=4 * 2.0**-11)
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_decode_attention_captured_replayed_and_repeatable(bits):
     """A captured call follows the lengths it finds at replay; two graphs on one pool do not share scratch; the same
