@@ -89,12 +89,17 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// Largest value, NaN if any is NaN.
+__device__ __forceinline__ float max2(float a, float b) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // 2^x of both halves on the fp32 pipe: x = n + f with n the nearest integer (added to 1.5 * 2^23, whose low bits then hold
 // it) and |f| <= 1/2, 2^f by a polynomial of degree 4 (least largest relative error, 2.7e-6, by exchange), 2^n added to the
@@ -199,7 +204,7 @@ __device__ __noinline__ void redo_row(const PrefillParams& P, const half* q, int
 #pragma unroll
     for (int e = 0; e < E; ++e) s = fmaf(qf[e], __half2float(k[e]), s);
     s = warp_sum(s);
-    const float top = fmaxf(m, s), f = m == top ? 1.f : exp2f(m - top), p = exp2f(s - top);
+    const float top = fmaxf(m, s), f = m == top ? 1.f : exp2f(m - top), p = s == -INFINITY ? 0.f : exp2f(s - top);
     m = top;
     l = fmaf(l, f, p);
 #pragma unroll
@@ -265,7 +270,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool valid = row < w.lq;
     // keys this row sees; a row behind the last one is worked on as that one (with none it would mask every tile) and dropped
     const int limit = max(min(row, w.lq - 1) + 1 + w.lk - w.lq, 0);
-    float m = -INFINITY, l = 0.f;
+    // worst: the largest score of all, NaN if one is NaN (the polynomial loses them)
+    float m = -INFINITY, l = 0.f, worst = -INFINITY;
     bool ok = true;
     for (int j = 0; j < tiles && ok; ++j) {
       ok = __all_sync(0xffffffffu, wait(sh, &sh.s_full[s], j & 1));
@@ -287,13 +293,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float tops[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) tops[i] = fmaxf(__uint_as_float(x[0][2 * i]), __uint_as_float(x[0][2 * i + 1]));
+      for (int i = 0; i < 8; ++i) tops[i] = max2(__uint_as_float(x[0][2 * i]), __uint_as_float(x[0][2 * i + 1]));
 #pragma unroll
       for (int i = 16; i < 128; i += 2)
         tops[(i >> 1) & 7] = max3(tops[(i >> 1) & 7], __uint_as_float(x[i >> 5][i & 31]), __uint_as_float(x[i >> 5][(i & 31) + 1]));
-      float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
-                        fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
+      float top = max2(max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[4]), max3(tops[5], tops[6], tops[7]));
       top *= scale_log2;
+      worst = max2(worst, top);
       const bool move = top > m + kLazy;  // also the first finite maximum
       if (__any_sync(0xffffffffu, move)) {
         const float f = move ? ex2(m - top) : 1.f;
@@ -351,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tiles >= 0 && ok) {
       constexpr int kPieces = HD / 8;
       uint4* stage = reinterpret_cast<uint4*>(s_q + s * kTileBytes + (warp & 3) * (32 * HD * 2));
-      bool good = true;
+      bool good = limit == 0 || fabsf(worst) <= 3.4e38f;
       if (tiles > 0) {
         ok = __all_sync(0xffffffffu, wait(sh, &sh.o_full[s], 0));
         tc::fence_after();

@@ -556,6 +556,36 @@ def test_prefill_masked_places_do_not_count(bad):
     assert torch.isfinite(got[at:, 2:, 4:]).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_prefill_non_finite_scores(bad, hd):
+    """One non-finite key value or query value, at every place of a tile's columns: the rows that see it are what the
+    formula gives (NaN where a score is NaN or +inf, or all are -inf; a score of -inf alone has no weight)."""
+    n, count, nq, nkv = 40, 36, 4, 2
+    g = _gen(17)
+    q = torch.randn(n * count, nq, hd, generator=g).half()
+    k, v = (torch.randn(n * count, nkv, hd, generator=g).half() for _ in range(2))
+    kb, qb = k.clone(), q.clone()
+    for s in range(count):
+        kb[n * s + s, 0, s] = bad
+        qb[n * s + s, 3, s] = bad
+    vb = v.clone()
+    vb[n - 1 :: n, :, 7] = float("inf")  # what the last row of each sequence makes of it beside such keys
+    got = ops.prefill_attention(qb.to(DEV), kb.to(DEV), vb.to(DEV), _cum([n] * count)).cpu().numpy().astype(np.float64)
+    seen = np.tril(np.ones((n, n), bool))
+    for s in range(count):
+        at = slice(n * s, n * s + n)
+        with np.errstate(invalid="ignore"):
+            out, _, _ = oracle.attention(*(t[at].numpy().astype(np.float64) for t in (qb, kb, vb)), seen)
+        # magnitudes without the bad value: a key with the weight 0 adds nothing to the bound's sums
+        _, mag, dot = oracle.attention(*(t[at].numpy().astype(np.float64) for t in (q, k, v)), seen)
+        mag = np.maximum(mag, np.abs(v[at].numpy().astype(np.float64)).max())
+        fine = np.isfinite(out)
+        assert np.array_equal(got[at][~fine], out[~fine], equal_nan=True), s
+        err = np.abs(got[at][fine] - out[fine])
+        assert np.all(err <= oracle.attention_bound(np.where(fine, out, 0), mag, dot)[fine]), s
+
+
 def test_prefill_large_scores_and_equal_rows():
     """Scores of thousands (one key takes all) and all-equal keys (the mean of the values seen)."""
     n, hd = 260, 64
