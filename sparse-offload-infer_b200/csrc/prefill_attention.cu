@@ -489,6 +489,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (j == last) tc::commit(&sh.o_full[s]);
     };
+    // entry e may be overwritten; for the last ones nobody waits, and no arrival is left for after the CTA's end
+    auto release = [&](int e) {
+      if (e + kSlots < 2 * n) tc::commit(&sh.kv_empty[e % kSlots]);
+    };
     for (int j = 0; j <= n && ok; ++j) {
       if (j < n) ok = wait_all(&sh.kv_full[2 * j % kSlots], (2 * j / kSlots) & 1);
       if (!ok) break;
@@ -500,11 +504,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (ok) outputs(1, j - 1, n1 - 1);
           if (!ok) break;
         }
-        tc::commit(&sh.kv_empty[(2 * j - 1) % kSlots]);
+        release(2 * j - 1);
       }
       if (j == n) break;
       if (j < n1) scores(1, j);
-      tc::commit(&sh.kv_empty[2 * j % kSlots]);
+      release(2 * j);
       if (j < n0) {
         ok = wait_all(&sh.kv_full[(2 * j + 1) % kSlots], ((2 * j + 1) / kSlots) & 1);
         if (ok) outputs(0, j, n0 - 1);
