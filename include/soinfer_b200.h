@@ -579,9 +579,9 @@ int soinfer_paged_kv_read(const soinfer_paged_cache* cache, const int32_t* cu_se
  * table_cols * page_size; read on the device), grouped heads, scale
  * 1/sqrt(head_dim), fp32 softmax and sums: out [num_seqs, num_q_heads,
  * head_dim].  Positions without a page are skipped; a sequence without
- * positions gives zeros.  num_seqs <= 32768.  The workspace holds the
- * partial results of long sequences; its size (0: none needed, workspace may
- * be NULL) follows from max_positions = table_cols * page_size. */
+ * positions gives zeros.  num_seqs <= 32768.  The workspace holds partial
+ * results; its size (0: none needed, workspace may be NULL) follows from the
+ * sequences, the heads and max_positions = table_cols * page_size. */
 int64_t soinfer_paged_decode_workspace_bytes(int64_t num_seqs, int64_t num_q_heads, int64_t num_kv_heads,
                                              int64_t head_dim, int64_t max_positions);
 int soinfer_paged_decode_attention(const soinfer_paged_cache* cache, const soinfer_rows* q, soinfer_half* out,

@@ -330,7 +330,7 @@ struct PagedDecodeParams {
   half* out;              // [seqs, nq, hd]
   int seqs, nq;
   const int32_t* lens;    // [seqs]
-  float* ws;              // partial results of split sequences
+  float* ws;              // pieces of split sequences
 };
 // Bytes for tables that name up to `positions` positions per sequence (0: none needed).
 int64_t paged_decode_workspace_bytes(int64_t seqs, int64_t nq, int64_t nkv, int64_t hd, int64_t positions);

@@ -15,15 +15,19 @@
 //            once to fp16 (11 bits, down to 2^-21 of the largest).  fp16 rows: the same with the scale 1.
 // The softmax statistics and both sums are fp32.
 //
-// Work split, by the longest sequence the block table can name:
-//   up to kClusterMost positions: a sequence's kv head (and up to 8 of its query heads) is one cluster of eight CTAs, each
-//   an eighth of the positions; they join through distributed shared memory.  One launch, no workspace.  (8 unequal
-//   sequences of up to 4096 fp16 positions: 15.5 us against 19.3 by chunks; a single sequence uses 8 CTAs per kv head,
-//   which long ones outgrow.)
-//   beyond: positions of all sequences together are cut into chunks of equal length, about as many as the GPU holds CTAs,
-//   computed on the device from the lengths (no host read; a captured launch serves any lengths), one CTA each.  A
-//   sequence cut into several chunks leaves (m, l, acc) per chunk in the workspace and a second kernel joins them in
-//   order; a sequence of one chunk is finished in place.
+// Work split.  A sequence's kv head with up to 8 of its query heads is a unit.
+//   Few units (kClusterUnits) over tables that name few positions (kClusterMost): a unit is one cluster of eight CTAs, each
+//   an eighth of the positions; they join through distributed shared memory.  One launch, no workspace: 777 4-bit positions of
+//   8 kv heads 5.0 us against 7.8 by ranges; 8 unequal sequences of up to 4096 fp16 positions, 4 kv heads, 11.3 against 12.9.
+//   Beyond, a cluster's idle CTAs and the eight-fold start cost more than they bring (64 unequal sequences of up to 4000 4-bit
+//   positions 91 us against 58, 256 of 500 252 against 60; one of 8000 fp16 positions 14.3 against 11.7, 4-bit 11.0 against
+//   11.3).
+//   Else the positions of all units form one line that is cut into equal ranges, one per CTA that the GPU holds, computed on
+//   the device from the lengths (no host read; a captured launch serves any lengths).  A CTA works through the pieces of
+//   sequences in its range; a sequence inside one range is finished in place, the pieces (m, l, acc) of the others go to the
+//   workspace, whose size follows from the GPU, and a second kernel joins them in order.  (Chunks of equal length, as many as
+//   CTAs where that fits: 20 sequences of 50000 316 us against 222, 30 of 12000 141 against 94; two long ones 61.8 against
+//   62.4.)
 // A CTA has four warps, each with every fourth tile of the CTA's positions; they are joined in shared memory.
 //
 // Feeding: each warp has its own ring of tiles in shared memory, filled by 16-byte asynchronous copies, so loads run ahead and
@@ -35,6 +39,8 @@
 // measured copy rate), bound by issuing 294 instructions per 16 positions and kv head (integer pipe 47%, fp16 / fp32 pipe
 // 26%, tensor pipe 26% busy, DRAM 0.66); register tiles without a ring 96 us, 32-position tiles 81.  One sequence of 777
 // positions: 5.0 us in one launch, against 8.7 with a second kernel that joins.
+#include <algorithm>
+
 #include "launch.cuh"
 #include "paged_cache.cuh"
 
@@ -44,14 +50,15 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kCluster = 8;
-constexpr int64_t kClusterMost = 8192;
+constexpr int kClusterUnits = 148 * 2 / kCluster;  // one wave of CTAs
 constexpr int kCols = 8;          // query heads per CTA
 constexpr int kMostLen = 1 << 30;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;      // the running maximum follows when exceeded by 2^8 (it moves in a few tiles, not in half)
 constexpr float kLift = 7.f;      // factor 2^7 on the probabilities (it cancels)
 
-// Positions a warp takes at a time, tiles in its ring, CTAs that an SM holds (shared memory and registers).
+// Positions a warp takes at a time, tiles in its ring, CTAs that an SM holds (shared memory and registers), the split's limit
+// and units (see above and below).
 template <bool Q4>
 struct Plan {
   static constexpr int kTile = Q4 ? 64 : 16;
@@ -59,6 +66,8 @@ struct Plan {
   static constexpr int kPerSm = Q4 ? 3 : 2;
   static constexpr int kCtas = 148 * kPerSm;
   static constexpr int kMinChunk = kTile * kWarps;
+  static constexpr int kStart = Q4 ? 1 : 2;
+  static constexpr int64_t kClusterMost = Q4 ? 8192 : 4096;
 };
 
 // d = a b + c.
@@ -90,21 +99,113 @@ __device__ __forceinline__ int seq_len(const PagedDecodeParams& P, int b) {
   return n < 0 ? 0 : n > most ? most : n;
 }
 
-// Chunk length for the batch: a multiple of the smallest chunk that gives at most as many chunks x head groups as the GPU
-// holds CTAs, where the sequences are fewer than that (warp-wide).
+// The split by ranges: a sequence counts as its positions in units of kMinChunk and kStart units more, what beginning it
+// costs (without them 67 against 62 us in the file comment's case: the CTAs with two pieces were the last).  All sequences of
+// a head group follow one another, and the head groups; CTA i takes the units [i per, (i + 1) per) of that line, per =
+// ceil(all / CTAs).  Its range falls into pieces, one per sequence that it touches; a sequence that lies in one range is
+// finished by its CTA, the others' pieces go to the workspace: slot 2 i for a piece that begins the range, 2 i + 1 for one
+// that ends it.
+struct Piece {
+  int b, group, begin, end;        // sequence (-1: none), head group, positions
+  int slot;                        // workspace slot (-1: the whole sequence)
+  int later;                       // units that later CTAs do (-1: not the sequence's first piece)
+};
+struct Range {
+  long long left, per;             // units still to do, units of a range
+  int b, group, inside;            // where they begin: sequence, head group, units of the sequence before
+};
+// A split sequence, noted by the CTA that begins it: its pieces are slot first and slots 2 (first / 2 + 1) .. 2 last.
+struct Split {
+  int b, group, first, last;       // b -1: none
+};
+struct Workspace {
+  Split* splits;                   // per head group and sequence where those are fewer than the CTAs, else per CTA
+  float* pieces;                   // [2 CTAs][heads][hd + 2]: sums, maximum, sum of weights
+};
 template <bool Q4>
-__device__ __forceinline__ int chunk_len(const PagedDecodeParams& P, int units, int lane) {
-  constexpr int kMin = Plan<Q4>::kMinChunk;
+__device__ __forceinline__ Workspace workspace(const PagedDecodeParams& P) {
+  return {reinterpret_cast<Split*>(P.ws), P.ws + Plan<Q4>::kCtas * (sizeof(Split) / sizeof(float))};
+}
+
+template <bool Q4>
+__device__ __forceinline__ int units_of(int len) {
+  return (len + Plan<Q4>::kMinChunk - 1) / Plan<Q4>::kMinChunk + Plan<Q4>::kStart;
+}
+
+// The next piece of the range (one thread).
+template <bool Q4>
+__device__ __forceinline__ void next_piece(const PagedDecodeParams& P, Range& R, bool first, Piece& out) {
+  if (R.left <= 0) {
+    out.b = -1;
+    return;
+  }
+  constexpr int kMin = Plan<Q4>::kMinChunk, kStart = Plan<Q4>::kStart;
+  const int n = seq_len(P, R.b), rest = units_of<Q4>(n) - R.inside;
+  const int take = rest < R.left ? rest : (int)R.left;
+  const int from = max(R.inside - kStart, 0) * kMin, to = max(R.inside + take - kStart, 0) * kMin;
+  out.b = R.b;
+  out.group = R.group;
+  out.begin = from;
+  out.end = n < to ? n : to;
+  out.slot = R.inside == 0 && take == rest ? -1 : 2 * (int)blockIdx.x + (first ? 0 : 1);
+  out.later = R.inside == 0 ? rest - take : -1;
+  R.left -= take;
+  R.inside = 0;
+  if (++R.b == P.seqs) R.b = 0, ++R.group;
+}
+
+// Notes whether the sequence that this piece begins is split (one thread).
+template <bool Q4>
+__device__ __forceinline__ void note_split(const PagedDecodeParams& P, int groups_all, const Piece& piece, long long per) {
+  constexpr int kCtas = Plan<Q4>::kCtas;
+  const bool by_sequence = (long long)P.seqs * groups_all <= kCtas;
+  if (piece.later < 0 || (piece.later == 0 && !by_sequence)) return;
+  Split* at = workspace<Q4>(P).splits + (by_sequence ? piece.group * P.seqs + piece.b : (int)blockIdx.x);
+  if (piece.later == 0)
+    at->b = -1;
+  else
+    *at = {piece.b, piece.group, piece.slot, (int)(blockIdx.x + (piece.later + per - 1) / per)};
+}
+
+// This CTA's range and its first piece (one warp).
+template <bool Q4>
+__device__ __forceinline__ void first_piece(const PagedDecodeParams& P, int groups_all, int lane, Range& R, Piece& out) {
+  constexpr int kCtas = Plan<Q4>::kCtas;
   long long total = 0;
-  for (int b = lane; b < P.seqs; b += 32) total += seq_len(P, b);
+  for (int base = 0; base < P.seqs; base += 32)
+    total += __reduce_add_sync(0xffffffffu, base + lane < P.seqs ? (unsigned)units_of<Q4>(seq_len(P, base + lane)) : 0u);
+  const long long all = total * groups_all, per = (all + kCtas - 1) / kCtas, at = per * blockIdx.x;
+  long long want = at, group = 0;
+  if (at < all) {
+    group = all >> 31 ? at / total : (unsigned)at / (unsigned)total;
+    want -= group * total;
+  }
+  int b = 0, inside = 0;
+  for (int base = 0; at < all && base < P.seqs; base += 32) {
+    const int mine = base + lane < P.seqs ? units_of<Q4>(seq_len(P, base + lane)) : 0;
+    int sum = mine;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  // every sequence's last chunk is a partial one: room for those keeps the launch in one wave
-  const int slots = (Plan<Q4>::kCtas + units - 1) / units;
-  const int rest = P.seqs < slots / 2 ? slots - P.seqs : (slots + 1) / 2;
-  const long long want = (total + rest - 1) / rest;
-  const long long c = (want + kMin - 1) / kMin * kMin;
-  return (int)(c < kMin ? kMin : c > kMostLen ? kMostLen : c);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    const unsigned owns = __ballot_sync(0xffffffffu, want < sum);
+    if (owns) {
+      const int src = __ffs(owns) - 1;
+      b = base + src;
+      inside = (int)want - __shfl_sync(0xffffffffu, sum - mine, src);
+      break;
+    }
+    want -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (lane != 0) return;
+  R.per = per;
+  R.left = at + per < all ? per : at < all ? all - at : 0;
+  R.b = b;
+  R.group = (int)group;
+  R.inside = inside;
+  next_piece<Q4>(P, R, true, out);
+  if ((long long)P.seqs * groups_all > kCtas) workspace<Q4>(P).splits[blockIdx.x].b = -1;
 }
 
 // A tile in shared memory: key codes (rows), their scales, value codes (rows), their scales; where it holds 16-byte piece c
@@ -291,366 +392,346 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
   constexpr int kMin = Plan<Q4>::kMinChunk, kRun = kTile / kRuns;
   extern __shared__ __align__(128) uint8_t smem[];  // kWarps rings of kStages tiles, then the warps' results
   __shared__ float s_m[kWarps][kCols], s_l[kWarps][kCols];
+  __shared__ Range s_range;
+  __shared__ Piece s_piece[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * (kStages * kBytes);
-  if (kJoined) pdl_launch_dependents();
+  pdl_launch_dependents();
   pdl_wait();
-  if (!kJoined) pdl_launch_dependents();  // not before the wait: the joining kernel reads the lengths as soon as it runs
   const PagedCache& C = P.cache;
-  const int rep = P.nq / C.nkv, units = C.nkv * groups;
-
-  int b = -1, len = 0, chunk = 0, count = 0, L;
+  const int rep = P.nq / C.nkv;
+  Piece piece;
   if (kJoined) {
-    b = blockIdx.y;
-    chunk = blockIdx.z;  // the rank in the cluster
-    len = seq_len(P, b);
-    L = (len + kCluster * kMin - 1) / (kCluster * kMin) * kMin;
+    // an eighth of a sequence, by the rank in the cluster
+    const int len = seq_len(P, blockIdx.y), L = (len + kCluster * kMin - 1) / (kCluster * kMin) * kMin;
+    const int begin = blockIdx.z * L;
+    piece = {(int)blockIdx.y, (int)blockIdx.x, begin, len - begin < L ? len : begin + L, -1, -1};
   } else {
-    // which chunk of which sequence (every warp finds it for itself)
-    L = chunk_len<Q4>(P, units, lane);
-    for (int base = 0, before = 0; base < P.seqs; base += 32) {
-      const int i = base + lane;
-      const int n = i < P.seqs ? seq_len(P, i) : 0;
-      const int mine = i < P.seqs ? (n > L ? (n + L - 1) / L : 1) : 0;  // an empty sequence has one chunk: its zeros
-      int sum = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += x;
-      }
-      const int c = (int)blockIdx.y - before;
-      const unsigned owns = __ballot_sync(0xffffffffu, c >= sum - mine && c < sum);
-      if (owns) {
-        const int src = __ffs(owns) - 1;
-        b = base + src;
-        len = __shfl_sync(0xffffffffu, n, src);
-        count = __shfl_sync(0xffffffffu, mine, src);
-        chunk = c - __shfl_sync(0xffffffffu, sum - mine, src);
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    if (b < 0) return;
+    if (warp == 0) first_piece<Q4>(P, C.nkv * groups, lane, s_range, s_piece[0]);
+    __syncthreads();
+    piece = s_piece[0];
+    if (piece.b < 0) return;
   }
-  const int kvh = blockIdx.x / groups, h0 = (blockIdx.x - kvh * groups) * kCols;
-  const int heads = rep - h0 < kCols ? rep - h0 : kCols;
-  const int qh0 = kvh * rep + h0;
-  const int p_begin = chunk * L, p_end = len - p_begin < L ? len : p_begin + L;
+  for (int turn = 1;; ++turn) {
+    const int b = piece.b, kvh = piece.group / groups, h0 = (piece.group - kvh * groups) * kCols;
+    const int heads = rep - h0 < kCols ? rep - h0 : kCols;
+    const int qh0 = kvh * rep + h0;
+    const int p_begin = piece.begin, p_end = piece.end;
 
-  // the ring: tile i of this warp starts at position p_begin + (warp + i kWarps) kTile and consists of runs of positions
-  // inside a page; lane r knows the page of run r
-  using T = Tile<HD, Q4>;
-  const int page = 1 << C.page_shift;
-  const int p_warp = p_begin + warp * kTile, stride = kWarps * kTile;
-  const int tiles = p_warp < p_end ? (p_end - p_warp + stride - 1) / stride : 0;
-  const int64_t k_block = k_block_bytes(page, HD, Q4), v_block = v_block_bytes(page, HD, Q4);
-  const uint32_t ring_at = smem_u32(ring);
-  auto page_id = [&](int i) {
-    const int p = p_warp + i * stride + lane * kRun;
-    return lane < kRuns && p < p_end ? page_of(C, b, p) : -1;
-  };
-  unsigned there = 0;                              // per ring slot, which runs hold data
-  auto issue = [&](int i, int slot, int ids) {
-    const unsigned on = __ballot_sync(0xffffffffu, ids >= 0);
-    there = (there & ~(15u << (4 * slot))) | on << (4 * slot);
-    const uint32_t to = ring_at + slot * kBytes;
+    // the ring: tile i of this warp starts at position p_begin + (warp + i kWarps) kTile and consists of runs of positions
+    // inside a page; lane r knows the page of run r
+    using T = Tile<HD, Q4>;
+    const int page = 1 << C.page_shift;
+    const int p_warp = p_begin + warp * kTile, stride = kWarps * kTile;
+    const int tiles = p_warp < p_end ? (p_end - p_warp + stride - 1) / stride : 0;
+    const int64_t k_block = k_block_bytes(page, HD, Q4), v_block = v_block_bytes(page, HD, Q4);
+    const uint32_t ring_at = smem_u32(ring);
+    auto page_id = [&](int i) {
+      const int p = p_warp + i * stride + lane * kRun;
+      return lane < kRuns && p < p_end ? page_of(C, b, p) : -1;
+    };
+    unsigned there = 0;                              // per ring slot, which runs hold data
+    auto issue = [&](int i, int slot, int ids) {
+      const unsigned on = __ballot_sync(0xffffffffu, ids >= 0);
+      there = (there & ~(15u << (4 * slot))) | on << (4 * slot);
+      const uint32_t to = ring_at + slot * kBytes;
 #pragma unroll
-    for (int r = 0; r < kRuns; ++r) {
-      const int id = __shfl_sync(0xffffffffu, ids, r);
-      if (id < 0) continue;
-      const int slot0 = (p_warp + i * stride + r * kRun) & (page - 1);
-      const uint8_t* kb = C.k + ((int64_t)id * C.nkv + kvh) * k_block;
-      const uint8_t* vb = C.v + ((int64_t)id * C.nkv + kvh) * v_block;
-      const uint8_t* kc = kb + slot0 * T::kKeyRow;
-      const uint8_t* vc = vb + (Q4 ? slot0 / 2 : slot0) * T::kValueRow;
-      constexpr int kPieces = kRun * T::kKeyRow / 16, kKeyPieces = T::kKeyRow / 16, kValuePieces = T::kValueRow / 16;
-      static_assert(kPieces == (Q4 ? kRun / 2 : kRun) * kValuePieces, "keys and values have as many");
+      for (int r = 0; r < kRuns; ++r) {
+        const int id = __shfl_sync(0xffffffffu, ids, r);
+        if (id < 0) continue;
+        const int slot0 = (p_warp + i * stride + r * kRun) & (page - 1);
+        const uint8_t* kb = C.k + ((int64_t)id * C.nkv + kvh) * k_block;
+        const uint8_t* vb = C.v + ((int64_t)id * C.nkv + kvh) * v_block;
+        const uint8_t* kc = kb + slot0 * T::kKeyRow;
+        const uint8_t* vc = vb + (Q4 ? slot0 / 2 : slot0) * T::kValueRow;
+        constexpr int kPieces = kRun * T::kKeyRow / 16, kKeyPieces = T::kKeyRow / 16, kValuePieces = T::kValueRow / 16;
+        static_assert(kPieces == (Q4 ? kRun / 2 : kRun) * kValuePieces, "keys and values have as many");
 #pragma unroll
-      for (int o0 = 0; o0 < kPieces; o0 += 32) {
-        const int o = o0 + lane;
-        copy16(to + T::key(r * kRun + o / kKeyPieces, o % kKeyPieces), kc + 16 * o);
-        copy16(to + T::value((Q4 ? r * kRun / 2 : r * kRun) + o / kValuePieces, o % kValuePieces), vc + 16 * o);
-      }
-      if constexpr (Q4) {
-        constexpr int kKeyScales = kRun * (HD / 16) / 16, kScales = kKeyScales + kRun * 2 / 16;
-        const uint8_t* ks = kb + page * (HD / 2) + slot0 * (HD / 16);
-        const uint8_t* vs = vb + page * (HD / 2) + slot0 * 2;
-#pragma unroll
-        for (int o0 = 0; o0 < kScales; o0 += 32) {
-          const int o = o0 + lane, n = o - kKeyScales;
-          if (o < kScales)
-            copy16(to + (n < 0 ? T::kScales + r * kRun * (HD / 16) + 16 * o : T::kValueScales + r * kRun * 2 + 16 * n),
-                   n < 0 ? ks + 16 * o : vs + 16 * n);
+        for (int o0 = 0; o0 < kPieces; o0 += 32) {
+          const int o = o0 + lane;
+          copy16(to + T::key(r * kRun + o / kKeyPieces, o % kKeyPieces), kc + 16 * o);
+          copy16(to + T::value((Q4 ? r * kRun / 2 : r * kRun) + o / kValuePieces, o % kValuePieces), vc + 16 * o);
         }
-      }
-    }
-  };
-  {
-    int id[kStages];
+        if constexpr (Q4) {
+          constexpr int kKeyScales = kRun * (HD / 16) / 16, kScales = kKeyScales + kRun * 2 / 16;
+          const uint8_t* ks = kb + page * (HD / 2) + slot0 * (HD / 16);
+          const uint8_t* vs = vb + page * (HD / 2) + slot0 * 2;
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) id[i] = i < tiles ? page_id(i) : -1;
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) {
-      if (i < tiles) issue(i, i, id[i]);
-      copy_commit();
-    }
-  }
-  int next_id = kStages < tiles ? page_id(kStages) : -1;
-
-  // the queries as the product's column operand: head g, values 32 j + 8 t + (0..7)
-  uint32_t qf[G][4];
-  float bias[G][2];
-#pragma unroll
-  for (int j = 0; j < G; ++j) {
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (g < heads)
-      u = __ldg(reinterpret_cast<const uint4*>(P.q + b * P.q_token + (qh0 + g) * P.q_head) + 4 * j + t);
-    qf[j][0] = u.x, qf[j][1] = u.y, qf[j][2] = u.z, qf[j][3] = u.w;
-    if (Q4) {
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 1; i < 4; i += 2) {  // the values whose codes carry the 72
-        const float2 f = __half22float2(u32_as_h2(qf[j][i]));
-        sum += f.x + f.y;
-      }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      bias[j][0] = -72.f * __shfl_sync(0xffffffffu, sum, 8 * t);
-      bias[j][1] = -72.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-    }
-  }
-
-  float acc[HD / 16][4];
-#pragma unroll
-  for (int i = 0; i < HD / 16; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2 t, 2 t + 1
-
-  int slot = 0;
-  for (int i = 0; i < tiles; ++i) {
-    copy_wait<kStages - 1>();
-    __syncwarp();
-    const int p0 = p_warp + i * stride;
-    const unsigned held = there >> (4 * slot);
-    const uint8_t* tile = ring + slot * kBytes;
-    const bool full_tile = p0 + kTile <= p_end && (held & ((1u << kRuns) - 1)) == (1u << kRuns) - 1;
-    float s[kSub][4], sv[kSub][2];
-    float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int u = 0; u < kSub; ++u) {
-      scores<HD, Q4>(s[u], tile, 16 * u, qf, bias, g, t);
-      uint32_t scale[2];  // fp16 bits
-      if (Q4) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          scale[r] = reinterpret_cast<const uint16_t*>(tile + T::kValueScales)[16 * u + g + 8 * r];
-      }
-      if (!full_tile) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          if (!(p0 + 16 * u + g + 8 * r < p_end && (held >> (16 * u / kRun) & 1))) {
-            s[u][2 * r] = s[u][2 * r + 1] = -INFINITY;
-            scale[r] = 0x3c00;
+          for (int o0 = 0; o0 < kScales; o0 += 32) {
+            const int o = o0 + lane, n = o - kKeyScales;
+            if (o < kScales)
+              copy16(to + (n < 0 ? T::kScales + r * kRun * (HD / 16) + 16 * o : T::kValueScales + r * kRun * 2 + 16 * n),
+                     n < 0 ? ks + 16 * o : vs + 16 * n);
           }
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        // exponent of the scale, rounded up: scale * 2^-e < 1 (an integer put into a float's mantissa); -14 for the scale 0 of
-        // zeroed pages, whose weights stay finite so
-        float e = 0.f;
-        if (Q4) {
-          e = __uint_as_float(scale[r] >> 10 | 0x4b000000u) - (8388608.f + 14.f);
-          sv[u][r] = __half2float(__ushort_as_half((unsigned short)scale[r]));
         }
+      }
+    };
+    {
+      int id[kStages];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], fmaf(s[u][2 * r + c], scale_log2, e));
+      for (int i = 0; i < kStages; ++i) id[i] = i < tiles ? page_id(i) : -1;
+#pragma unroll
+      for (int i = 0; i < kStages; ++i) {
+        if (i < tiles) issue(i, i, id[i]);
+        copy_commit();
       }
     }
+    int next_id = kStages < tiles ? page_id(kStages) : -1;
+    if (!kJoined && threadIdx.x == 0) {
+      note_split<Q4>(P, C.nkv * groups, piece, s_range.per);
+      next_piece<Q4>(P, s_range, false, s_piece[turn & 1]);
+    }
+
+    // the queries as the product's column operand: head g, values 32 j + 8 t + (0..7)
+    uint32_t qf[G][4];
+    float bias[G][2];
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (g < heads)
+        u = __ldg(reinterpret_cast<const uint4*>(P.q + b * P.q_token + (qh0 + g) * P.q_head) + 4 * j + t);
+      qf[j][0] = u.x, qf[j][1] = u.y, qf[j][2] = u.z, qf[j][3] = u.w;
+      if (Q4) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 1; i < 4; i += 2) {  // the values whose codes carry the 72
+          const float2 f = __half22float2(u32_as_h2(qf[j][i]));
+          sum += f.x + f.y;
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        bias[j][0] = -72.f * __shfl_sync(0xffffffffu, sum, 8 * t);
+        bias[j][1] = -72.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      }
+    }
+
+    float acc[HD / 16][4];
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2 t, 2 t + 1
+
+    int slot = 0;
+    for (int i = 0; i < tiles; ++i) {
+      copy_wait<kStages - 1>();
+      __syncwarp();
+      const int p0 = p_warp + i * stride;
+      const unsigned held = there >> (4 * slot);
+      const uint8_t* tile = ring + slot * kBytes;
+      const bool full_tile = p0 + kTile <= p_end && (held & ((1u << kRuns) - 1)) == (1u << kRuns) - 1;
+      float s[kSub][4], sv[kSub][2];
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+        scores<HD, Q4>(s[u], tile, 16 * u, qf, bias, g, t);
+        uint32_t scale[2];  // fp16 bits
+        if (Q4) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            scale[r] = reinterpret_cast<const uint16_t*>(tile + T::kValueScales)[16 * u + g + 8 * r];
+        }
+        if (!full_tile) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            if (!(p0 + 16 * u + g + 8 * r < p_end && (held >> (16 * u / kRun) & 1))) {
+              s[u][2 * r] = s[u][2 * r + 1] = -INFINITY;
+              scale[r] = 0x3c00;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          // exponent of the scale, rounded up: scale * 2^-e < 1 (an integer put into a float's mantissa); -14 for the scale 0 of
+          // zeroed pages, whose weights stay finite so
+          float e = 0.f;
+          if (Q4) {
+            e = __uint_as_float(scale[r] >> 10 | 0x4b000000u) - (8388608.f + 14.f);
+            sv[u][r] = __half2float(__ushort_as_half((unsigned short)scale[r]));
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], fmaf(s[u][2 * r + c], scale_log2, e));
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+      }
+      if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
+        float f[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          top[c] = fmaxf(top[c], m[c]);
+          f[c] = m[c] == top[c] ? 1.f : ex2(m[c] - top[c]);
+          m[c] = top[c];
+          l[c] *= f[c];
+        }
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] *= f[e & 1];
+      }
+      const float shift[2] = {m[0] == -INFINITY ? 0.f : kLift - m[0], m[1] == -INFINITY ? 0.f : kLift - m[1]};
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[u][e] = ex2(fmaf(s[u][e], scale_log2, shift[e & 1]));
+          l[e & 1] += s[u][e];
+          if (Q4) s[u][e] *= sv[u][e >> 1];
+        }
+        accumulate<HD, Q4>(acc, tile, 16 * u, s[u], full_tile ? 16 : (held >> (16 * u / kRun) & 1) ? p_end - p0 - 16 * u : 0,
+                           g, t);
+      }
+      __syncwarp();  // every lane has read the tile
+      if (i + kStages < tiles) {
+        issue(i + kStages, slot, next_id);
+        next_id = i + kStages + 1 < tiles ? page_id(i + kStages + 1) : -1;
+      }
+      copy_commit();
+      if (++slot == kStages) slot = 0;
+    }
+
+    // join the warps: lane (g, t) holds heads 2 t, 2 t + 1 and HD/8 of the values
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-    }
-    if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
-      float f[2];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        top[c] = fmaxf(top[c], m[c]);
-        f[c] = m[c] == top[c] ? 1.f : ex2(m[c] - top[c]);
-        m[c] = top[c];
-        l[c] *= f[c];
+      for (int o = 4; o < 32; o <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], o);
+      if (g == 0) {
+        s_m[warp][2 * t + c] = m[c];
+        s_l[warp][2 * t + c] = l[c];
       }
-#pragma unroll
-      for (int j = 0; j < HD / 16; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[j][e] *= f[e & 1];
     }
-    const float shift[2] = {m[0] == -INFINITY ? 0.f : kLift - m[0], m[1] == -INFINITY ? 0.f : kLift - m[1]};
+    constexpr int kRow = HD + 4;
+    static_assert(kWarps * kCols * kRow * 4 <= kWarps * kStages * kBytes, "the results fit where the rings were");
+    float* s_acc = reinterpret_cast<float*>(smem);
+    __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kSub; ++u) {
+    for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[u][e] = ex2(fmaf(s[u][e], scale_log2, shift[e & 1]));
-        l[e & 1] += s[u][e];
-        if (Q4) s[u][e] *= sv[u][e >> 1];
+      for (int e = 0; e < 4; ++e)
+        s_acc[(warp * kCols + 2 * t + (e & 1)) * kRow + value_of<HD, Q4>(i, e >> 1, g)] = acc[i][e];
+    __syncthreads();
+    if constexpr (kJoined) {
+      // this CTA's sums, over the first warp's; then every CTA finishes an eighth of the cluster's values
+      for (int e = threadIdx.x; e < heads * HD; e += kThreads) {
+        const int h = e / HD, d = e - h * HD;
+        float num, den, M;
+        join_warps<HD>(s_acc, s_m, s_l, h, d, num, den, M);
+        s_acc[h * kRow + d] = num;
+        if (d == 0) s_acc[h * kRow + HD] = M, s_acc[h * kRow + HD + 1] = den;
       }
-      accumulate<HD, Q4>(acc, tile, 16 * u, s[u], full_tile ? 16 : (held >> (16 * u / kRun) & 1) ? p_end - p0 - 16 * u : 0,
-                         g, t);
-    }
-    __syncwarp();  // every lane has read the tile
-    if (i + kStages < tiles) {
-      issue(i + kStages, slot, next_id);
-      next_id = i + kStages + 1 < tiles ? page_id(i + kStages + 1) : -1;
-    }
-    copy_commit();
-    if (++slot == kStages) slot = 0;
-  }
-
-  // join the warps: lane (g, t) holds heads 2 t, 2 t + 1 and HD/8 of the values
+      cluster_sync();
+      for (int e = blockIdx.z * kThreads + threadIdx.x; e < heads * HD; e += kCluster * kThreads) {
+        const int h = e / HD, d = e - h * HD;
+        const float* row = s_acc + h * kRow;
+        float m8[kCluster], M = -INFINITY, num = 0.f, den = 0.f;
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+        for (int r = 0; r < kCluster; ++r) M = fmaxf(M, m8[r] = cluster_read(row + HD, r));
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], o);
-    if (g == 0) {
-      s_m[warp][2 * t + c] = m[c];
-      s_l[warp][2 * t + c] = l[c];
-    }
-  }
-  constexpr int kRow = HD + 4;
-  static_assert(kWarps * kCols * kRow * 4 <= kWarps * kStages * kBytes, "the results fit where the rings were");
-  float* s_acc = reinterpret_cast<float*>(smem);
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < HD / 16; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      s_acc[(warp * kCols + 2 * t + (e & 1)) * kRow + value_of<HD, Q4>(i, e >> 1, g)] = acc[i][e];
-  __syncthreads();
-  if constexpr (kJoined) {
-    // this CTA's sums, over the first warp's; then every CTA finishes an eighth of the cluster's values
-    for (int e = threadIdx.x; e < heads * HD; e += kThreads) {
-      const int h = e / HD, d = e - h * HD;
-      float num, den, M;
-      join_warps<HD>(s_acc, s_m, s_l, h, d, num, den, M);
-      s_acc[h * kRow + d] = num;
-      if (d == 0) s_acc[h * kRow + HD] = M, s_acc[h * kRow + HD + 1] = den;
-    }
-    cluster_sync();
-    for (int e = chunk * kThreads + threadIdx.x; e < heads * HD; e += kCluster * kThreads) {
-      const int h = e / HD, d = e - h * HD;
-      const float* row = s_acc + h * kRow;
-      float m8[kCluster], M = -INFINITY, num = 0.f, den = 0.f;
-#pragma unroll
-      for (int r = 0; r < kCluster; ++r) M = fmaxf(M, m8[r] = cluster_read(row + HD, r));
-#pragma unroll
-      for (int r = 0; r < kCluster; ++r) {
-        const float f = m8[r] == -INFINITY ? 0.f : ex2(m8[r] - M);
-        den = fmaf(f, cluster_read(row + HD + 1, r), den);
-        num = fmaf(f, cluster_read(row + d, r), num);
-      }
-      P.out[((int64_t)b * P.nq + qh0 + h) * HD + d] = result(num, den);
-    }
-    cluster_sync();  // nobody leaves while its sums are read
-  } else {
-    for (int e = threadIdx.x; e < heads * HD; e += kThreads) {
-      const int h = e / HD, d = e - h * HD;
-      float num, den, M;
-      join_warps<HD>(s_acc, s_m, s_l, h, d, num, den, M);
-      if (count == 1) {
+        for (int r = 0; r < kCluster; ++r) {
+          const float f = m8[r] == -INFINITY ? 0.f : ex2(m8[r] - M);
+          den = fmaf(f, cluster_read(row + HD + 1, r), den);
+          num = fmaf(f, cluster_read(row + d, r), num);
+        }
         P.out[((int64_t)b * P.nq + qh0 + h) * HD + d] = result(num, den);
-      } else {
-        float* ws = P.ws + ((int64_t)blockIdx.y * P.nq + qh0 + h) * (HD + 2);
-        ws[d] = num;
-        if (d == 0) ws[HD] = M, ws[HD + 1] = den;
       }
+      cluster_sync();  // nobody leaves while its sums are read
+    } else {
+      for (int e = threadIdx.x; e < heads * HD; e += kThreads) {
+        const int h = e / HD, d = e - h * HD;
+        float num, den, M;
+        join_warps<HD>(s_acc, s_m, s_l, h, d, num, den, M);
+        if (piece.slot < 0) {
+          P.out[((int64_t)b * P.nq + qh0 + h) * HD + d] = result(num, den);
+        } else {
+          float* ws = workspace<Q4>(P).pieces + (piece.slot * (rep < kCols ? rep : kCols) + h) * (HD + 2);
+          ws[d] = num;
+          if (d == 0) ws[HD] = M, ws[HD + 1] = den;
+        }
+      }
+      piece = s_piece[turn & 1];
+      if (piece.b < 0) return;
+      __syncthreads();  // the sums are read: their place becomes the rings' again
     }
+    if (kJoined) return;
   }
 }
 
-// Joins the chunks of a sequence that has several; one CTA per (sequence, query head), in kParts parts of the chunks that
-// are summed in order.  A lane looks at every 32nd chunk's maximum and sum; the rows' loads do not wait for one another.
-constexpr int kParts = 4;
+// Joins the pieces of a split sequence; one CTA per split and query head, in kParts parts of the pieces that are joined in
+// order.  The loads of a part's first pieces wait for nothing but the note of the split.
+constexpr int kParts = 4, kAtOnce = 8;
 template <int HD, bool Q4>
-__global__ void __launch_bounds__(HD * kParts) paged_join_kernel(const PagedDecodeParams P, const int units) {
-  __shared__ float s_num[kParts][HD], s_den[kParts];
-  const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 31, part = threadIdx.x / HD, d = threadIdx.x % HD;
-  // the lengths are there: every CTA of the first kernel has waited for what came before it
-  const int n = seq_len(P, b);
-  const int L = chunk_len<Q4>(P, units, lane);
-  int first = 0;
-  for (int i = lane; i < b; i += 32) {
-    const int x = seq_len(P, i);
-    first += x > L ? (x + L - 1) / L : 1;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(0xffffffffu, first, o);
+__global__ void __launch_bounds__(HD * kParts) paged_join_kernel(const PagedDecodeParams P, const int groups) {
+  __shared__ float s_num[kParts][HD], s_den[kParts], s_top[kParts];
+  const int part = threadIdx.x / HD, d = threadIdx.x % HD;
   pdl_launch_dependents();
   pdl_wait();
-  if (n <= L) return;  // finished by its only chunk
-  const int count = (n + L - 1) / L, each = (count + kParts - 1) / kParts;
-  const float* ws = P.ws + ((int64_t)first * P.nq + h) * (HD + 2);
-  const int64_t step = (int64_t)P.nq * (HD + 2);
-  float M = -INFINITY;
-  for (int c = lane; c < count; c += 32) M = fmaxf(M, ws[c * step + HD]);
-  M = warp_max(M);
-  float num = 0.f, den = 0.f;
-  const int end = (part + 1) * each < count ? (part + 1) * each : count;
-  for (int c0 = part * each; c0 < end; c0 += 32) {
-    const int c = c0 + lane;
-    float f = 0.f;
-    if (c < end) {
-      const float2 ml = *reinterpret_cast<const float2*>(ws + c * step + HD);
-      f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-      den = fmaf(f, ml.y, den);
+  const Workspace w = workspace<Q4>(P);
+  const Split split = w.splits[blockIdx.y];
+  if (split.b < 0) return;
+  const int rep = P.nq / P.cache.nkv, kvh = split.group / groups, h = (split.group - kvh * groups) * kCols + blockIdx.x;
+  if (h >= rep) return;
+  const int count = split.last - split.first / 2 + 1;
+  float M = -INFINITY, num = 0.f, den = 0.f;
+  for (int c0 = part * kAtOnce; c0 < count; c0 += kParts * kAtOnce) {
+    float x[kAtOnce];
+    float2 ml[kAtOnce];
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int c = c0 + i;
+      const float* at = w.pieces + ((c == 0 ? split.first : (split.first & ~1) + 2 * c) * gridDim.x + blockIdx.x) * (HD + 2);
+      x[i] = c < count ? at[d] : 0.f;
+      ml[i] = c < count ? *reinterpret_cast<const float2*>(at + HD) : make_float2(-INFINITY, 0.f);
     }
-    const int rows = end - c0 < 32 ? end - c0 : 32;
-    const float* row = ws + c0 * step + d;
-#pragma unroll 8
-    for (int i = 0; i < rows; ++i) num = fmaf(__shfl_sync(0xffffffffu, f, i), row[i * step], num);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, ml[i].x);
+    const float f = M == top ? 1.f : ex2(M - top);
+    num *= f, den *= f, M = top;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float fi = ml[i].x == -INFINITY ? 0.f : ex2(ml[i].x - M);
+      num = fmaf(fi, x[i], num);
+      den = fmaf(fi, ml[i].y, den);
+    }
   }
-  den = warp_sum(den);
   s_num[part][d] = num;
-  if (d == 0) s_den[part] = den;
+  if (d == 0) s_den[part] = den, s_top[part] = M;
   __syncthreads();
   if (part > 0) return;
 #pragma unroll
-  for (int i = 1; i < kParts; ++i) {
-    num += s_num[i][d];
-    den += s_den[i];
+  for (int i = 1; i < kParts; ++i) M = fmaxf(M, s_top[i]);
+  num = den = 0.f;
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) {
+    const float f = s_top[i] == -INFINITY ? 0.f : ex2(s_top[i] - M);
+    num = fmaf(f, s_num[i][d], num);
+    den = fmaf(f, s_den[i], den);
   }
-  P.out[((int64_t)b * P.nq + h) * HD + d] = result(num, den);
+  P.out[((int64_t)split.b * P.nq + kvh * rep + h) * HD + d] = result(num, den);
 }
-
-// Chunks of any lengths: sum over sequences of max(1, ceil(len / L)) with L >= total * units / CTAs.
-int64_t most_chunks(int64_t seqs, int64_t units, bool q4) {
-  const int64_t ctas = q4 ? Plan<true>::kCtas : Plan<false>::kCtas;
-  return seqs + (ctas + units - 1) / units;
-}
-
-// Whether a cluster of CTAs takes a whole sequence (see the file comment).
-bool joined(int64_t table_cols, int page_shift) { return (table_cols << page_shift) <= kClusterMost; }
 
 int64_t head_groups(int64_t nq, int64_t nkv) { return (nq / nkv + kCols - 1) / kCols; }
 
 template <int HD, bool Q4, int kRuns>
 cudaError_t decode_runs(const PagedDecodeParams& P, cudaStream_t stream) {
-  const int groups = (int)head_groups(P.nq, P.cache.nkv), units = P.cache.nkv * groups;
+  const int rep = P.nq / P.cache.nkv, groups = (int)head_groups(P.nq, P.cache.nkv), units = P.cache.nkv * groups;
   const float scale_log2 = (1.0f / sqrtf((float)HD)) * kLog2e;
-  constexpr int kSmem = kWarps * Plan<Q4>::kStages * Tile<HD, Q4>::kBytes;
+  constexpr int kSmem = kWarps * Plan<Q4>::kStages * Tile<HD, Q4>::kBytes, kCtas = Plan<Q4>::kCtas;
   cudaError_t e;
-  if (joined(P.cache.table_cols, P.cache.page_shift)) {
+  const int64_t all = (int64_t)P.seqs * units;
+  if (all <= kClusterUnits && (int64_t)P.cache.table_cols << P.cache.page_shift <= Plan<Q4>::kClusterMost) {
     if ((e = ensure_smem_attr<paged_decode_kernel<HD, Q4, kRuns, true>>(kSmem)) != cudaSuccess) return e;
     return launch_ex(paged_decode_kernel<HD, Q4, kRuns, true>, dim3((unsigned)units, (unsigned)P.seqs, kCluster),
                      dim3(kThreads), kSmem, stream, dim3(1, 1, kCluster), true, P, groups, scale_log2);
   }
   if ((e = ensure_smem_attr<paged_decode_kernel<HD, Q4, kRuns, false>>(kSmem)) != cudaSuccess) return e;
-  e = launch_ex(paged_decode_kernel<HD, Q4, kRuns, false>,
-                dim3((unsigned)units, (unsigned)most_chunks(P.seqs, units, Q4)), dim3(kThreads), kSmem, stream, 1, true, P,
-                groups, scale_log2);
+  e = launch_ex(paged_decode_kernel<HD, Q4, kRuns, false>, dim3(kCtas), dim3(kThreads), kSmem, stream, 1, true, P, groups,
+                scale_log2);
   if (e != cudaSuccess) return e;
-  return launch_ex(paged_join_kernel<HD, Q4>, dim3((unsigned)P.nq, (unsigned)P.seqs), dim3(HD * kParts), 0, stream, 1, true,
-                   P, units);
+  return launch_ex(paged_join_kernel<HD, Q4>, dim3((unsigned)(rep < kCols ? rep : kCols), (unsigned)(all < kCtas ? all : kCtas)),
+                   dim3(HD * kParts), 0, stream, 1, true, P, groups);
 }
 
 template <int HD>
@@ -667,10 +748,11 @@ cudaError_t decode_hd(const PagedDecodeParams& P, cudaStream_t stream) {
 }  // namespace
 
 int64_t paged_decode_workspace_bytes(int64_t seqs, int64_t nq, int64_t nkv, int64_t hd, int64_t positions) {
-  if (positions <= kClusterMost) return 0;
-  const int64_t units = nkv * head_groups(nq, nkv);
-  const int64_t a = most_chunks(seqs, units, true), b = most_chunks(seqs, units, false);
-  return (a > b ? a : b) * nq * (hd + 2) * (int64_t)sizeof(float);
+  // for either type of page
+  const int64_t most = std::min(Plan<true>::kClusterMost, Plan<false>::kClusterMost);
+  if (seqs * nkv * head_groups(nq, nkv) <= kClusterUnits && positions <= most) return 0;
+  const int64_t ctas = std::max(Plan<true>::kCtas, Plan<false>::kCtas), heads = std::min<int64_t>(nq / nkv, kCols);
+  return ctas * (int64_t)(sizeof(Split) + 2 * heads * (hd + 2) * sizeof(float));
 }
 
 cudaError_t launch_paged_decode(const PagedDecodeParams& P, cudaStream_t stream) {

@@ -890,7 +890,8 @@ def head_norm_rope(q, k, v, q_norm, k_norm, cos_vals, sin_vals, k_cache, v_cache
 _PAGED_CACHE = struct.Struct("PPPqqqqqqq")  # soinfer_paged_cache
 _ROWS = struct.Struct("Pqq")                # soinfer_rows
 PAGED_HEAD_DIMS = (64, 128)
-PAGED_CLUSTER_POSITIONS = 8192  # tables up to this many positions need no workspace (paged_attention.cu)
+# no workspace up to this many positions in a table row and kv heads x sequences (paged_attention.cu)
+PAGED_CLUSTER_POSITIONS, PAGED_CLUSTER_UNITS = 4096, 37
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _F16, _F32, _U8, _I32 = torch.float16, torch.float32, torch.uint8, torch.int32
 
@@ -1080,7 +1081,7 @@ def paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, out=None)
     out = _out_rows(name, out, q, shape)
     if B:
         positions, nbytes, ws_at = block_table.shape[1] * page, 0, None
-        if positions > PAGED_CLUSTER_POSITIONS:
+        if positions > PAGED_CLUSTER_POSITIONS or B * nkv * -(-nq // (8 * nkv)) > PAGED_CLUSTER_UNITS:
             # a workspace of the call's own: two captured graphs or streams never share one
             nbytes = lib().soinfer_paged_decode_workspace_bytes(B, nq, nkv, hd, positions)
             ws = q.new_empty((nbytes // 2,))

@@ -80,6 +80,11 @@ def test_read_decode_and_prefill_arguments():
     # the front end asks for a workspace exactly where one is needed
     assert lib.soinfer_paged_decode_workspace_bytes(3, 8, 2, 128, _C.PAGED_CLUSTER_POSITIONS) == 0
     assert lib.soinfer_paged_decode_workspace_bytes(3, 8, 2, 128, _C.PAGED_CLUSTER_POSITIONS + 16) > 0
+    most = _C.PAGED_CLUSTER_UNITS  # sequences x kv heads (x groups of 8 query heads of a kv head)
+    for seqs, nq, nkv in ((most, 8, 1), (most // 2, 2, 2), (most // 3, 17, 1)):
+        assert lib.soinfer_paged_decode_workspace_bytes(seqs, nq, nkv, 64, 64) == 0
+    for seqs, nq, nkv in ((most + 1, 8, 1), (most // 2 + 1, 2, 2), (most // 3 + 1, 17, 1)):
+        assert lib.soinfer_paged_decode_workspace_bytes(seqs, nq, nkv, 64, 64) > 0
     d = lib.soinfer_paged_decode_attention
     long = dict(table_cols=10_000, table_stride=10_000)
     assert d(_cache(**long), _rows(), P, 3, 8, P, P, need - 1, None) == 1 and "workspace" in _err()

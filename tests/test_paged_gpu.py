@@ -274,6 +274,19 @@ def test_decode_attention_with_wide_tables(lens, page, nq, nkv, hd, bits):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("lens,page,nq,nkv,hd", [
+    ([30 + i * 37 % 300 for i in range(60)] + [0] * 20 + [7000] + [5] * 45, 16, 4, 4, 64),  # more units than CTAs
+    ([100] * 298 + [101, 99], 16, 2, 1, 128),
+    ([5000, 0, 40, 3000], 32, 24, 2, 128),  # 12 heads a group: two column groups, split sequences
+    ([0] * 50, 64, 8, 8, 64),
+    ([257, 64, 65, 1024, 256] * 4 + [0, 1], 64, 10, 2, 64),
+])
+def test_decode_attention_of_batches(lens, page, nq, nkv, hd, bits):
+    """Ranges over many sequences: several to a CTA, some over many CTAs, empty ones, units noted per sequence or CTA."""
+    test_decode_attention_with_wide_tables(lens, page, nq, nkv, hd, bits)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
 def test_decode_attention_over_missing_pages_and_odd_lengths(bits):
     """Pages that are not there are skipped; lengths below zero and beyond the table are cut."""
     lens, page, nq, nkv, hd = [700, 64, 90, 33], 32, 4, 2, 128
