@@ -379,8 +379,11 @@ cudaError_t append_hd(const PagedAppendParams& P, cudaStream_t stream) {
   const int parts = (steps + per - 1) / per;
   per = (steps + parts - 1) / parts;
   const int64_t warps = (int64_t)P.tokens * ((steps + per - 1) / per);
-  return launch_ex(per > 1 && !Q4 ? paged_append_kernel<HD, Q4, 2> : paged_append_kernel<HD, Q4, 1>,
-                   dim3((unsigned)((warps + kWarps - 1) / kWarps)), dim3(32 * kWarps), 0, stream, 1, true, P, per);
+  const dim3 grid((unsigned)((warps + kWarps - 1) / kWarps)), block(32 * kWarps);
+  if constexpr (!Q4) {
+    if (per > 1) return launch_ex(paged_append_kernel<HD, Q4, 2>, grid, block, 0, stream, 1, true, P, per);
+  }
+  return launch_ex(paged_append_kernel<HD, Q4, 1>, grid, block, 0, stream, 1, true, P, per);
 }
 
 }  // namespace
