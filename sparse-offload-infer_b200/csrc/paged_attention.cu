@@ -20,14 +20,14 @@
 //   an eighth of the positions; they join through distributed shared memory.  One launch, no workspace: 777 4-bit positions of
 //   8 kv heads 5.0 us against 7.8 by ranges; 8 unequal sequences of up to 4096 fp16 positions, 4 kv heads, 11.3 against 12.9.
 //   Beyond, a cluster's idle CTAs and the eight-fold start cost more than they bring (64 unequal sequences of up to 4000 4-bit
-//   positions 91 us against 58, 256 of 500 252 against 60; one of 8000 fp16 positions 14.3 against 11.7, 4-bit 11.0 against
+//   positions 91 us against 56, 256 of 500 252 against 58; one of 8000 fp16 positions 14.3 against 11.3, 4-bit 11.0 against
 //   11.3).
 //   Else the positions of all units form one line that is cut into equal ranges, one per CTA that the GPU holds, computed on
 //   the device from the lengths (no host read; a captured launch serves any lengths).  A CTA works through the pieces of
 //   sequences in its range; a sequence inside one range is finished in place, the pieces (m, l, acc) of the others go to the
 //   workspace, whose size follows from the GPU, and a second kernel joins them in order.  (Chunks of equal length, as many as
-//   CTAs where that fits: 20 sequences of 50000 316 us against 222, 30 of 12000 141 against 94; two long ones 61.8 against
-//   62.4.)
+//   CTAs where that fits: 20 sequences of 50000 316 us against 219, 30 of 12000 141 against 93; two long ones 61.8 against
+//   61.4.)
 // A CTA has four warps, each with every fourth tile of the CTA's positions; they are joined in shared memory.
 //
 // Feeding: each warp has its own ring of tiles in shared memory, filled by 16-byte asynchronous copies, so loads run ahead and
@@ -167,9 +167,9 @@ __device__ __forceinline__ void note_split(const PagedDecodeParams& P, int group
     *at = {piece.b, piece.group, piece.slot, (int)(blockIdx.x + (piece.later + per - 1) / per)};
 }
 
-// This CTA's range and its first piece (one warp).
+// This CTA's range and its first two pieces (one warp).
 template <bool Q4>
-__device__ __forceinline__ void first_piece(const PagedDecodeParams& P, int groups_all, int lane, Range& R, Piece& out) {
+__device__ __forceinline__ void first_piece(const PagedDecodeParams& P, int groups_all, int lane, Range& R, Piece* out) {
   constexpr int kCtas = Plan<Q4>::kCtas;
   long long total = 0;
   for (int base = 0; base < P.seqs; base += 32)
@@ -204,7 +204,8 @@ __device__ __forceinline__ void first_piece(const PagedDecodeParams& P, int grou
   R.b = b;
   R.group = (int)group;
   R.inside = inside;
-  next_piece<Q4>(P, R, true, out);
+  next_piece<Q4>(P, R, true, out[0]);
+  next_piece<Q4>(P, R, false, out[1]);
   if ((long long)P.seqs * groups_all > kCtas) workspace<Q4>(P).splits[blockIdx.x].b = -1;
 }
 
@@ -310,7 +311,8 @@ __device__ __forceinline__ void accumulate(float (*acc)[4], const uint8_t* tile,
   if constexpr (Q4) {
     uint32_t v[2][HD / 32];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) lds_words<HD / 32>(v[r], tile + T::value(slot0 / 2 + t + 4 * r, g * (HD / 8) / 16) + g * (HD / 8) % 16);
+    for (int r = 0; r < 2; ++r)
+      lds_words<HD / 32>(v[r], tile + T::value(slot0 / 2 + t + 4 * r, g * (HD / 8) / 16) + g * (HD / 8) % 16);
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
       uint32_t x[2][4];  // values 4 i + (0..3) of the lane's, at position pairs t and t + 4
@@ -353,8 +355,8 @@ __device__ __forceinline__ int value_of(int i, int r, int g) {
   return Q4 ? g * (HD / 8) + 2 * i + r : 64 * (i >> 2) + 8 * g + 2 * (i & 3) + r;
 }
 
-// The four warps' sums of head h, value d.
-template <int HD>
+// The four warps' sums of head h, value d; a warp's lie kStride floats behind the one's before.
+template <int HD, int kStride>
 __device__ __forceinline__ void join_warps(const float* s_acc, const float (*s_m)[kCols], const float (*s_l)[kCols], int h,
                                            int d, float& num, float& den, float& M) {
   M = -INFINITY;
@@ -365,7 +367,7 @@ __device__ __forceinline__ void join_warps(const float* s_acc, const float (*s_m
   for (int w = 0; w < kWarps; ++w) {
     const float f = s_m[w][h] == -INFINITY ? 0.f : ex2(s_m[w][h] - M);
     den = fmaf(f, s_l[w][h], den);
-    num = fmaf(f, s_acc[(w * kCols + h) * (HD + 4) + d], num);
+    num = fmaf(f, s_acc[w * kStride + h * (HD + 4) + d], num);
   }
 }
 
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
   extern __shared__ __align__(128) uint8_t smem[];  // kWarps rings of kStages tiles, then the warps' results
   __shared__ float s_m[kWarps][kCols], s_l[kWarps][kCols];
   __shared__ Range s_range;
-  __shared__ Piece s_piece[2];
+  __shared__ Piece s_piece[3];  // this one, the next, the one after
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * (kStages * kBytes);
   pdl_launch_dependents();
@@ -407,79 +409,89 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
     const int begin = blockIdx.z * L;
     piece = {(int)blockIdx.y, (int)blockIdx.x, begin, len - begin < L ? len : begin + L, -1, -1};
   } else {
-    if (warp == 0) first_piece<Q4>(P, C.nkv * groups, lane, s_range, s_piece[0]);
+    if (warp == 0) first_piece<Q4>(P, C.nkv * groups, lane, s_range, s_piece);
     __syncthreads();
     piece = s_piece[0];
     if (piece.b < 0) return;
   }
-  for (int turn = 1;; ++turn) {
-    const int b = piece.b, kvh = piece.group / groups, h0 = (piece.group - kvh * groups) * kCols;
-    const int heads = rep - h0 < kCols ? rep - h0 : kCols;
-    const int qh0 = kvh * rep + h0;
-    const int p_begin = piece.begin, p_end = piece.end;
 
-    // the ring: tile i of this warp starts at position p_begin + (warp + i kWarps) kTile and consists of runs of positions
-    // inside a page; lane r knows the page of run r
-    using T = Tile<HD, Q4>;
-    const int page = 1 << C.page_shift;
-    const int p_warp = p_begin + warp * kTile, stride = kWarps * kTile;
-    const int tiles = p_warp < p_end ? (p_end - p_warp + stride - 1) / stride : 0;
-    const int64_t k_block = k_block_bytes(page, HD, Q4), v_block = v_block_bytes(page, HD, Q4);
-    const uint32_t ring_at = smem_u32(ring);
-    auto page_id = [&](int i) {
-      const int p = p_warp + i * stride + lane * kRun;
-      return lane < kRuns && p < p_end ? page_of(C, b, p) : -1;
-    };
-    unsigned there = 0;                              // per ring slot, which runs hold data
-    auto issue = [&](int i, int slot, int ids) {
-      const unsigned on = __ballot_sync(0xffffffffu, ids >= 0);
-      there = (there & ~(15u << (4 * slot))) | on << (4 * slot);
-      const uint32_t to = ring_at + slot * kBytes;
+  // the ring: tile i of this warp starts at position p_warp + i kWarps kTile and consists of runs of positions inside a page;
+  // lane r knows the page of run r
+  using T = Tile<HD, Q4>;
+  constexpr int stride = kWarps * kTile;
+  const int page = 1 << C.page_shift;
+  const int64_t k_block = k_block_bytes(page, HD, Q4), v_block = v_block_bytes(page, HD, Q4);
+  const uint32_t ring_at = smem_u32(ring);
+  int b, kvh, heads, qh0, p_end, p_warp, tiles;
+  unsigned there;                                // per ring slot, which runs hold data
+  auto take = [&] {
+    b = piece.b, kvh = piece.group / groups;
+    const int h0 = (piece.group - kvh * groups) * kCols;
+    heads = rep - h0 < kCols ? rep - h0 : kCols;
+    qh0 = kvh * rep + h0;
+    p_end = piece.end;
+    p_warp = piece.begin + warp * kTile;
+    tiles = p_warp < p_end ? (p_end - p_warp + stride - 1) / stride : 0;
+    there = 0;
+  };
+  auto page_id = [&](int i) {
+    const int p = p_warp + i * stride + lane * kRun;
+    return i < tiles && lane < kRuns && p < p_end ? page_of(C, b, p) : -1;
+  };
+  auto issue = [&](int i, int slot, int ids) {
+    const unsigned on = __ballot_sync(0xffffffffu, ids >= 0);
+    there = (there & ~(15u << (4 * slot))) | on << (4 * slot);
+    const uint32_t to = ring_at + slot * kBytes;
 #pragma unroll
-      for (int r = 0; r < kRuns; ++r) {
-        const int id = __shfl_sync(0xffffffffu, ids, r);
-        if (id < 0) continue;
-        const int slot0 = (p_warp + i * stride + r * kRun) & (page - 1);
-        const uint8_t* kb = C.k + ((int64_t)id * C.nkv + kvh) * k_block;
-        const uint8_t* vb = C.v + ((int64_t)id * C.nkv + kvh) * v_block;
-        const uint8_t* kc = kb + slot0 * T::kKeyRow;
-        const uint8_t* vc = vb + (Q4 ? slot0 / 2 : slot0) * T::kValueRow;
-        constexpr int kPieces = kRun * T::kKeyRow / 16, kKeyPieces = T::kKeyRow / 16, kValuePieces = T::kValueRow / 16;
-        static_assert(kPieces == (Q4 ? kRun / 2 : kRun) * kValuePieces, "keys and values have as many");
+    for (int r = 0; r < kRuns; ++r) {
+      const int id = __shfl_sync(0xffffffffu, ids, r);
+      if (id < 0) continue;
+      const int slot0 = (p_warp + i * stride + r * kRun) & (page - 1);
+      const uint8_t* kb = C.k + ((int64_t)id * C.nkv + kvh) * k_block;
+      const uint8_t* vb = C.v + ((int64_t)id * C.nkv + kvh) * v_block;
+      const uint8_t* kc = kb + slot0 * T::kKeyRow;
+      const uint8_t* vc = vb + (Q4 ? slot0 / 2 : slot0) * T::kValueRow;
+      constexpr int kPieces = kRun * T::kKeyRow / 16, kKeyPieces = T::kKeyRow / 16, kValuePieces = T::kValueRow / 16;
+      static_assert(kPieces == (Q4 ? kRun / 2 : kRun) * kValuePieces, "keys and values have as many");
 #pragma unroll
-        for (int o0 = 0; o0 < kPieces; o0 += 32) {
-          const int o = o0 + lane;
-          copy16(to + T::key(r * kRun + o / kKeyPieces, o % kKeyPieces), kc + 16 * o);
-          copy16(to + T::value((Q4 ? r * kRun / 2 : r * kRun) + o / kValuePieces, o % kValuePieces), vc + 16 * o);
-        }
-        if constexpr (Q4) {
-          constexpr int kKeyScales = kRun * (HD / 16) / 16, kScales = kKeyScales + kRun * 2 / 16;
-          const uint8_t* ks = kb + page * (HD / 2) + slot0 * (HD / 16);
-          const uint8_t* vs = vb + page * (HD / 2) + slot0 * 2;
-#pragma unroll
-          for (int o0 = 0; o0 < kScales; o0 += 32) {
-            const int o = o0 + lane, n = o - kKeyScales;
-            if (o < kScales)
-              copy16(to + (n < 0 ? T::kScales + r * kRun * (HD / 16) + 16 * o : T::kValueScales + r * kRun * 2 + 16 * n),
-                     n < 0 ? ks + 16 * o : vs + 16 * n);
-          }
-        }
+      for (int o0 = 0; o0 < kPieces; o0 += 32) {
+        const int o = o0 + lane;
+        copy16(to + T::key(r * kRun + o / kKeyPieces, o % kKeyPieces), kc + 16 * o);
+        copy16(to + T::value((Q4 ? r * kRun / 2 : r * kRun) + o / kValuePieces, o % kValuePieces), vc + 16 * o);
       }
-    };
-    {
-      int id[kStages];
+      if constexpr (Q4) {
+        constexpr int kKeyScales = kRun * (HD / 16) / 16, kScales = kKeyScales + kRun * 2 / 16;
+        const uint8_t* ks = kb + page * (HD / 2) + slot0 * (HD / 16);
+        const uint8_t* vs = vb + page * (HD / 2) + slot0 * 2;
 #pragma unroll
-      for (int i = 0; i < kStages; ++i) id[i] = i < tiles ? page_id(i) : -1;
-#pragma unroll
-      for (int i = 0; i < kStages; ++i) {
-        if (i < tiles) issue(i, i, id[i]);
-        copy_commit();
+        for (int o0 = 0; o0 < kScales; o0 += 32) {
+          const int o = o0 + lane, n = o - kKeyScales;
+          if (o < kScales)
+            copy16(to + (n < 0 ? T::kScales + r * kRun * (HD / 16) + 16 * o : T::kValueScales + r * kRun * 2 + 16 * n),
+                   n < 0 ? ks + 16 * o : vs + 16 * n);
+        }
       }
     }
-    int next_id = kStages < tiles ? page_id(kStages) : -1;
+  };
+  int id[kStages];
+  auto look_up = [&] {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) id[i] = page_id(i);
+  };
+  auto start = [&](int i) {
+    if (i < tiles) issue(i, i, id[i]);
+    copy_commit();
+  };
+  take();
+  look_up();
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) start(i);
+  for (int turn = 1;; turn = turn == 2 ? 0 : turn + 1) {  // turn: where the next piece is
+    start(kStages - 1);
+    int next_id = page_id(kStages);
     if (!kJoined && threadIdx.x == 0) {
       note_split<Q4>(P, C.nkv * groups, piece, s_range.per);
-      next_piece<Q4>(P, s_range, false, s_piece[turn & 1]);
+      next_piece<Q4>(P, s_range, false, s_piece[turn == 2 ? 0 : turn + 1]);
     }
 
     // the queries as the product's column operand: head g, values 32 j + 8 t + (0..7)
@@ -541,8 +553,8 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          // exponent of the scale, rounded up: scale * 2^-e < 1 (an integer put into a float's mantissa); -14 for the scale 0 of
-          // zeroed pages, whose weights stay finite so
+          // exponent of the scale, rounded up: scale * 2^-e < 1 (an integer put into a float's mantissa); -14 for the scale 0
+          // of zeroed pages, whose weights stay finite so
           float e = 0.f;
           if (Q4) {
             e = __uint_as_float(scale[r] >> 10 | 0x4b000000u) - (8388608.f + 14.f);
@@ -586,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
       __syncwarp();  // every lane has read the tile
       if (i + kStages < tiles) {
         issue(i + kStages, slot, next_id);
-        next_id = i + kStages + 1 < tiles ? page_id(i + kStages + 1) : -1;
+        next_id = page_id(i + kStages + 1);
       }
       copy_commit();
       if (++slot == kStages) slot = 0;
@@ -602,59 +614,70 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
         s_l[warp][2 * t + c] = l[c];
       }
     }
-    constexpr int kRow = HD + 4;
-    static_assert(kWarps * kCols * kRow * 4 <= kWarps * kStages * kBytes, "the results fit where the rings were");
-    float* s_acc = reinterpret_cast<float*>(smem);
-    __syncthreads();
+    // each warp's sums where its last ring slot was; the next piece's first tiles are on their way to the others meanwhile
+    constexpr int kRow = HD + 4, kStride = kStages * kBytes / 4;
+    static_assert(kCols * kRow * 4 <= kBytes, "the results fit into a ring slot");
+    float* s_acc = reinterpret_cast<float*>(smem + (kStages - 1) * kBytes);
+    const int64_t row = (int64_t)b * P.nq + qh0;
+    const int done_heads = heads, done_slot = piece.slot;
+    if (!kJoined) {
+      piece = s_piece[turn];
+      if (piece.b >= 0) {
+        take();
+        look_up();
+      }
+    }
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        s_acc[(warp * kCols + 2 * t + (e & 1)) * kRow + value_of<HD, Q4>(i, e >> 1, g)] = acc[i][e];
+        s_acc[warp * kStride + (2 * t + (e & 1)) * kRow + value_of<HD, Q4>(i, e >> 1, g)] = acc[i][e];
+    if (!kJoined && piece.b >= 0) {
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i) start(i);
+    }
     __syncthreads();
     if constexpr (kJoined) {
       // this CTA's sums, over the first warp's; then every CTA finishes an eighth of the cluster's values
-      for (int e = threadIdx.x; e < heads * HD; e += kThreads) {
+      for (int e = threadIdx.x; e < done_heads * HD; e += kThreads) {
         const int h = e / HD, d = e - h * HD;
         float num, den, M;
-        join_warps<HD>(s_acc, s_m, s_l, h, d, num, den, M);
+        join_warps<HD, kStride>(s_acc, s_m, s_l, h, d, num, den, M);
         s_acc[h * kRow + d] = num;
         if (d == 0) s_acc[h * kRow + HD] = M, s_acc[h * kRow + HD + 1] = den;
       }
       cluster_sync();
-      for (int e = blockIdx.z * kThreads + threadIdx.x; e < heads * HD; e += kCluster * kThreads) {
+      for (int e = blockIdx.z * kThreads + threadIdx.x; e < done_heads * HD; e += kCluster * kThreads) {
         const int h = e / HD, d = e - h * HD;
-        const float* row = s_acc + h * kRow;
+        const float* sums = s_acc + h * kRow;
         float m8[kCluster], M = -INFINITY, num = 0.f, den = 0.f;
 #pragma unroll
-        for (int r = 0; r < kCluster; ++r) M = fmaxf(M, m8[r] = cluster_read(row + HD, r));
+        for (int r = 0; r < kCluster; ++r) M = fmaxf(M, m8[r] = cluster_read(sums + HD, r));
 #pragma unroll
         for (int r = 0; r < kCluster; ++r) {
           const float f = m8[r] == -INFINITY ? 0.f : ex2(m8[r] - M);
-          den = fmaf(f, cluster_read(row + HD + 1, r), den);
-          num = fmaf(f, cluster_read(row + d, r), num);
+          den = fmaf(f, cluster_read(sums + HD + 1, r), den);
+          num = fmaf(f, cluster_read(sums + d, r), num);
         }
-        P.out[((int64_t)b * P.nq + qh0 + h) * HD + d] = result(num, den);
+        P.out[(row + h) * HD + d] = result(num, den);
       }
       cluster_sync();  // nobody leaves while its sums are read
     } else {
-      for (int e = threadIdx.x; e < heads * HD; e += kThreads) {
+      for (int e = threadIdx.x; e < done_heads * HD; e += kThreads) {
         const int h = e / HD, d = e - h * HD;
         float num, den, M;
-        join_warps<HD>(s_acc, s_m, s_l, h, d, num, den, M);
-        if (piece.slot < 0) {
-          P.out[((int64_t)b * P.nq + qh0 + h) * HD + d] = result(num, den);
+        join_warps<HD, kStride>(s_acc, s_m, s_l, h, d, num, den, M);
+        if (done_slot < 0) {
+          P.out[(row + h) * HD + d] = result(num, den);
         } else {
-          float* ws = workspace<Q4>(P).pieces + (piece.slot * (rep < kCols ? rep : kCols) + h) * (HD + 2);
+          float* ws = workspace<Q4>(P).pieces + (done_slot * (rep < kCols ? rep : kCols) + h) * (HD + 2);
           ws[d] = num;
           if (d == 0) ws[HD] = M, ws[HD + 1] = den;
         }
       }
-      piece = s_piece[turn & 1];
-      if (piece.b < 0) return;
-      __syncthreads();  // the sums are read: their place becomes the rings' again
     }
-    if (kJoined) return;
+    if (kJoined || piece.b < 0) return;
+    __syncthreads();  // the sums are read: their place becomes a ring slot again
   }
 }
 
