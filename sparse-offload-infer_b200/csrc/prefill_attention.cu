@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
     const uint32_t S = lanes + s * kTile, O = lanes + kO + s * HD;
     const bool valid = row < w.lq;
+    const bool idle = w.row[s] + (r & ~31) >= w.lq;  // no row of the warp exists: whatever its P is stays in its rows
     // keys this row sees; a row behind the last one is worked on as that one (with none it would mask every tile) and dropped
     const int limit = max(min(row, w.lq - 1) + 1 + w.lk - w.lq, 0);
     // worst: the largest score of all, NaN if one is NaN (the polynomial loses them)
@@ -276,6 +277,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int j = 0; j < tiles && ok; ++j) {
       ok = __all_sync(0xffffffffu, wait(sh, &sh.s_full[s], j & 1));
       if (!ok) break;
+      if (idle) {
+        if (lane == 0) {
+          mbar_arrive(&sh.p_half[s]);
+          mbar_arrive(&sh.p_full[s]);
+        }
+        continue;
+      }
       tc::fence_after();
       uint32_t x[4][32];
 #pragma unroll
@@ -354,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&sh.p_full[s]);
     }
     // the row's result
-    if (tiles >= 0 && ok) {
+    if (tiles >= 0 && ok && !idle) {
       constexpr int kPieces = HD / 8;
       uint4* stage = reinterpret_cast<uint4*>(s_q + s * kTileBytes + (warp & 3) * (32 * HD * 2));
       bool good = limit == 0 || fabsf(worst) <= 3.4e38f;
@@ -364,6 +372,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (ok) {
         const float inv = limit > 0 ? 1.f / l : 0.f;
+        const bool zero = __any_sync(0xffffffffu, limit == 0);
+        uint64_t zeros = 0;                      // 0 * value: NaN where one is not finite
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t o[32];
@@ -375,14 +385,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t* h = reinterpret_cast<uint32_t*>(v);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float a = 0.f, b = 0.f;
-            if (limit > 0) a = __uint_as_float(o[2 * i]) * inv, b = __uint_as_float(o[2 * i + 1]) * inv;
-            good = good && fabsf(a) <= 3.4e38f && fabsf(b) <= 3.4e38f;
+            const uint64_t y = mul2(pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), both(inv));
+            float a, b;
+            zeros = fma2(y, 0, zeros);
+            unpack2(y, a, b);
             h[i] = h2_as_u32(__floats2half2_rn(a, b));
           }
+          if (zero && limit == 0)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) h[i] = 0;
 #pragma unroll
           for (int i = 0; i < 4; ++i) stage[lane * kPieces + ((4 * c + i) ^ (lane & 7))] = v[i];
         }
+        float a, b;
+        unpack2(zeros, a, b);
+        good = limit == 0 || (good && a + b == 0.f);
         __syncwarp();
         const int row0 = w.row[s] + (r & ~31);
         uint4* out = reinterpret_cast<uint4*>(P.out + ((int64_t)(w.q0 + row0) * P.nq + w.head[s]) * HD);
