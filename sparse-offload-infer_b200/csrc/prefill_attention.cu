@@ -7,9 +7,10 @@
 // core 2 x 512 cycles and the exponential unit (16 per cycle and SM) 1024, so both bound it and have to overlap; at hd = 64
 // the exponentials alone do.
 //
-// A CTA holds two tiles of 128 query rows that share a kv head (stages 0 and 1: two heads of the group, or two row
-// tiles).  Their scores S (fp32, 128 columns each) and outputs O (fp32, hd columns each) lie in the tensor memory; the
-// probabilities P (fp16) overwrite the scores they come from and feed the second product from there.
+// A CTA holds two tiles of 128 query rows that share a kv head (stages 0 and 1: two heads of the group, or two row tiles; a
+// tile's rows are tokens of one head, or tokens x heads where the sequences are short).  Their scores S (fp32, 128 columns
+// each) and outputs O (fp32, hd columns each) lie in the tensor memory; the probabilities P (fp16) overwrite the scores they
+// come from and feed the second product from there.
 //   warps 0-3, 4-7: the softmax of stage 0 / 1, one thread per row (two threads per row: 716 against 685 us in the case
 //           below).  P is handed over in two halves, so that the second product starts after the first 64 keys, and one in
 //           four pairs of exponentials is computed on the fp32 pipe.  These warps take most of the CTA's registers.
@@ -37,6 +38,8 @@
 // 192 CTAs in two rounds; P beside S in the tensor memory, so that scores run ahead, measured the same (the two warps of a
 // scheduler spend their exponentials' phases together).
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -122,17 +125,25 @@ __device__ __forceinline__ void ex2_pair(uint64_t x2, float& a, float& b) {
   b = __int_as_float((__float_as_int(u) << 23) + __float_as_int(q));
 }
 
+// A query tile's heads of a kv head, its rows of the sequence (128 / heads), the kv head's groups of that many heads; inv:
+// 2^16 / heads, rounded up (a tile row's number times that, shifted back, is the quotient).
+struct TileHeads {
+  int heads, rows, groups, inv;
+};
+
 // A CTA's work: two query tiles of sequence rows q0.., keys k0.., kv head kvh.
 struct Work {
   int q0, lq, k0, lk, kvh;
-  int row[2], head[2], tiles[2];  // first row in the sequence, query head, key tiles (0: nothing to do)
+  int row[2], head[2], tiles[2];  // first row in the sequence, first query head, key tiles (0: nothing to do)
 };
 
-// The pair of query tiles that blockIdx.x stands for (warp-wide; false: none).  Query tile t of a sequence and kv head
-// is head t % rep, rows (t / rep) * 128 ..; a sequence's pairs run from the last to the first, and of up to 32 sequences
+// The pair of query tiles that blockIdx.x stands for (warp-wide; false: none).  Tile t of a sequence and kv head is head
+// group t % groups, rows t / groups * rows ..  A sequence's pairs run from the last to the first, and of up to 32 sequences
 // those with more keys come first (more: as they are given), so that short work fills the end of the launch.
-__device__ __forceinline__ bool find_work(const PrefillParams& P, int lane, Work& w) {
-  const int rep = P.nq / P.nkv;
+template <bool kPacked>
+__device__ __forceinline__ bool find_work(const PrefillParams& P, const TileHeads& H, int lane, Work& w) {
+  const int rows_tile = kPacked ? H.rows : kTile;
+  auto tiles_of = [&](int n) { return (n + rows_tile - 1) / rows_tile * H.groups; };
   w.kvh = blockIdx.x % P.nkv;
   int want = blockIdx.x / P.nkv;
   for (int base = 0; base < P.seqs; base += 32) {
@@ -145,7 +156,7 @@ __device__ __forceinline__ bool find_work(const PrefillParams& P, int lane, Work
       k0 = max(c, 0);
       lk = max(min(f, P.tokens_k) - k0, 0);
     }
-    const int pairs = ((lq + kTile - 1) / kTile * rep + 1) / 2;
+    const int pairs = (tiles_of(lq) + 1) / 2;
     int before = 0;
     if (P.seqs <= 32) {
       for (int o = 0; o < P.seqs; ++o) {
@@ -169,13 +180,14 @@ __device__ __forceinline__ bool find_work(const PrefillParams& P, int lane, Work
       w.k0 = __shfl_sync(0xffffffffu, k0, src);
       w.lk = __shfl_sync(0xffffffffu, lk, src);
       const int last = __shfl_sync(0xffffffffu, pairs - 1 - (want - before), src);  // the pair, from the sequence's start
-      const int tiles = (w.lq + kTile - 1) / kTile * rep;
+      const int tiles = tiles_of(w.lq);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int t = 2 * last + s;
-        w.row[s] = t / rep * kTile;
-        w.head[s] = w.kvh * rep + t % rep;
-        const int rows = w.lq - w.row[s] < kTile ? w.lq - w.row[s] : kTile;
+        const int q = t / H.groups;
+        w.row[s] = q * rows_tile;
+        w.head[s] = (w.kvh * H.groups + t - q * H.groups) * (kPacked ? H.heads : 1);
+        const int rows = w.lq - w.row[s] < rows_tile ? w.lq - w.row[s] : rows_tile;
         const int keys = max(w.row[s] + rows + w.lk - w.lq, 0);  // what the tile's last row sees
         w.tiles[s] = t < tiles ? (keys + kTile - 1) / kTile : -1;
       }
@@ -214,10 +226,11 @@ __device__ __noinline__ void redo_row(const PrefillParams& P, const half* q, int
   for (int e = 0; e < E; ++e) out[lane * E + e] = __float2half_rn(acc[e] / l);
 }
 
-template <int HD>
+// kPacked: a tile holds several heads.
+template <int HD, bool kPacked>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                   const __grid_constant__ CUtensorMap v_map, const PrefillParams P, const float scale_log2) {
+                   const __grid_constant__ CUtensorMap v_map, const PrefillParams P, const TileHeads H, const float scale_log2) {
   constexpr int kBox = kTile * 128;              // bytes of a TMA box: 128 rows of 64 fp16
   constexpr int kBoxes = HD / 64;
   constexpr int kTileBytes = kBoxes * kBox;
@@ -233,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
   Work w;
-  if (!find_work(P, lane, w)) return;            // the same for every warp
+  if (!find_work<kPacked>(P, H, lane, w)) return;           // the same for every warp
   const int steps = w.tiles[0] > w.tiles[1] ? w.tiles[0] : w.tiles[1];
 
   if (warp == 9) {
@@ -264,11 +277,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---------------------------------------------------------------- softmax
     const int s = warp >> 2, r = threadIdx.x & (kTile - 1);
-    const int tiles = w.tiles[s], row = w.row[s] + r;
+    const int tiles = w.tiles[s], token = kPacked ? r * H.inv >> 16 : r, row = w.row[s] + token;
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
     const uint32_t S = lanes + s * kTile, O = lanes + kO + s * HD;
-    const bool valid = row < w.lq;
-    const bool idle = w.row[s] + (r & ~31) >= w.lq;  // no row of the warp exists: whatever its P is stays in its rows
+    const bool valid = row < w.lq && (!kPacked || token < H.rows);
+    const bool idle = !__any_sync(0xffffffffu, valid);  // whatever its P is stays in its rows
     // keys this row sees; a row behind the last one is worked on as that one (with none it would mask every tile) and dropped
     const int limit = max(min(row, w.lq - 1) + 1 + w.lk - w.lq, 0);
     // worst: the largest score of all, NaN if one is NaN (the polynomial loses them)
@@ -401,20 +414,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         unpack2(zeros, a, b);
         good = limit == 0 || (good && a + b == 0.f);
         __syncwarp();
-        const int row0 = w.row[s] + (r & ~31);
-        uint4* out = reinterpret_cast<uint4*>(P.out + ((int64_t)(w.q0 + row0) * P.nq + w.head[s]) * HD);
+        const unsigned write = __ballot_sync(0xffffffffu, valid);
+        uint4* out = reinterpret_cast<uint4*>(P.out + ((int64_t)(w.q0 + w.row[s]) * P.nq + w.head[s]) * HD);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-          const int rr = (32 * i + lane) / kPieces, c = lane % kPieces;
-          if (row0 + rr < w.lq) out[(int64_t)rr * P.nq * kPieces + c] = stage[rr * kPieces + (c ^ (rr & 7))];
+          const int rr = (32 * i + lane) / kPieces, c = lane % kPieces, tr = (r & ~31) + rr;
+          // the row's place behind the tile's first
+          const int to = kPacked ? (tr * H.inv >> 16) * (P.nq - H.heads) + tr : tr * P.nq;
+          if (write >> rr & 1) out[(int64_t)to * kPieces + c] = stage[rr * kPieces + (c ^ (rr & 7))];
         }
         unsigned again = __ballot_sync(0xffffffffu, valid && !good);
         while (again) {
-          const int src = __ffs(again) - 1, rr = w.row[s] + (r & ~31) + src;
+          const int src = __ffs(again) - 1, rr = __shfl_sync(0xffffffffu, row, src);
+          const int h = w.head[s] + (kPacked ? (r & ~31) + src - (rr - w.row[s]) * H.heads : 0);
           again &= again - 1;
           __syncwarp();
-          redo_row<HD>(P, P.q + (int64_t)(w.q0 + rr) * P.q_token + w.head[s] * P.q_head, w.k0, rr + 1 + w.lk - w.lq,
-                       w.kvh, P.out + ((int64_t)(w.q0 + rr) * P.nq + w.head[s]) * HD, scale_log2, lane);
+          redo_row<HD>(P, P.q + (int64_t)(w.q0 + rr) * P.q_token + h * P.q_head, w.k0, rr + 1 + w.lk - w.lq, w.kvh,
+                       P.out + ((int64_t)(w.q0 + rr) * P.nq + h) * HD, scale_log2, lane);
         }
       }
     }
@@ -432,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int s = 0; s < 2; ++s)
         if (w.tiles[s] > 0) {
-          mbar_arrive_expect_tx(&sh.q_full[s], kTileBytes);
+          mbar_arrive_expect_tx(&sh.q_full[s], kBoxes * (kPacked ? H.rows * H.heads : kTile) * 128);
           for (int x = 0; x < kBoxes; ++x)
             tc::tma_load_3d(s_q + s * kTileBytes + x * kBox, &q_map, 64 * x, w.head[s], w.q0 + w.row[s], &sh.q_full[s]);
         }
@@ -564,9 +580,9 @@ EncodeTiled encoder() {
   return fn;
 }
 
-// Map of rows [tokens, heads, hd] with boxes of 64 values x 1 head x 128 tokens.
+// Map of rows [tokens, heads, hd] with boxes of 64 values x box_heads x 128 / box_heads tokens.
 cudaError_t make_map(CUtensorMap* map, const half* data, int64_t tokens, int64_t heads, int hd, int64_t token_stride,
-                     int64_t head_stride) {
+                     int64_t head_stride, int box_heads) {
   const EncodeTiled encode = encoder();
   if (!encode) return cudaErrorNotSupported;
   // a dimension of one entry may have any stride
@@ -574,32 +590,52 @@ cudaError_t make_map(CUtensorMap* map, const half* data, int64_t tokens, int64_t
   if (tokens == 1) token_stride = heads * hd;
   const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)tokens};
   const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
-  const cuuint32_t box[3] = {64, 1, kTile}, ones[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)(kTile / box_heads)}, ones[3] = {1, 1, 1};
   const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<half*>(data), dims, strides, box, ones,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// Query heads per tile: all of a kv head's where that takes at most 7/8 of the tiles for sequences of the average length (a
+// few tokens each: 16 tokens of 4 heads fill half a tile, not an eighth of four), else one.  32 / 8 heads: 128 sequences of
+// one token over 2001 453 against 214 us, 256 of 20 tokens 368 against 140, 64 of 200 135.9 against 131.0 (7/8 of the tiles);
+// 100 of 10 to 910 573 against 597 (15/16 of them, and a few rows' last step is masked as a whole tile's).
+TileHeads heads_per_tile(const PrefillParams& P) {
+  const int64_t rep = P.nq / P.nkv, length = (P.tokens_q + P.seqs - 1) / P.seqs;
+  int heads = 1;
+  if (rep <= kTile) {
+    const int64_t rows = kTile / rep;
+    if (8 * ((length + rows - 1) / rows) <= 7 * ((length + kTile - 1) / kTile * rep)) heads = (int)rep;
+  }
+  return {heads, kTile / heads, (int)rep / heads, (65536 + heads - 1) / heads};
+}
+
 template <int HD>
 cudaError_t prefill_hd(const PrefillParams& P, cudaStream_t stream) {
   CUtensorMap q, k, v;
-  cudaError_t e = make_map(&q, P.q, P.tokens_q, P.nq, HD, P.q_token, P.q_head);
+  const TileHeads H = heads_per_tile(P);
+  cudaError_t e = make_map(&q, P.q, P.tokens_q, P.nq, HD, P.q_token, P.q_head, H.heads);
   if (e != cudaSuccess) return e;
   k = v = q;  // no keys: never read
   if (P.tokens_k > 0) {
-    if ((e = make_map(&k, P.k, P.tokens_k, P.nkv, HD, P.k_token, P.k_head)) != cudaSuccess) return e;
-    if ((e = make_map(&v, P.v, P.tokens_k, P.nkv, HD, P.v_token, P.v_head)) != cudaSuccess) return e;
+    if ((e = make_map(&k, P.k, P.tokens_k, P.nkv, HD, P.k_token, P.k_head, 1)) != cudaSuccess) return e;
+    if ((e = make_map(&v, P.v, P.tokens_k, P.nkv, HD, P.v_token, P.v_head, 1)) != cudaSuccess) return e;
   }
-  const int smem = (2 + kSlots) * kTile * HD * 2 + 1024;
-  if ((e = ensure_smem_attr<prefill_kernel<HD>>(smem)) != cudaSuccess) return e;
-  // sum over sequences of ceil(rep ceil(lq / 128) / 2) <= (rep (tokens / 128 + seqs') + seqs') / 2, seqs' of them not empty
-  const int64_t rep = P.nq / P.nkv, seqs = P.seqs < P.tokens_q ? P.seqs : P.tokens_q;
-  const int64_t pairs = (rep * (P.tokens_q / kTile + seqs) + seqs + 1) / 2;
+  // sum over sequences of ceil(n ceil(lq / rows) / 2) <= (n (tokens / rows + seqs') + seqs') / 2, seqs' of them not empty
+  const int64_t n = H.groups, seqs = P.seqs < P.tokens_q ? P.seqs : P.tokens_q;
+  const int64_t pairs = (n * (P.tokens_q / H.rows + seqs) + seqs + 1) / 2;
   if (pairs * P.nkv > 0x7fffffff) return cudaErrorInvalidValue;
   const float scale_log2 = (1.0f / sqrtf((float)HD)) * kLog2e;
-  return launch_ex(prefill_kernel<HD>, dim3((unsigned)(pairs * P.nkv)), dim3(kThreads), (size_t)smem, stream, 1, true, q,
-                   k, v, P, scale_log2);
+  const int smem = (2 + kSlots) * kTile * HD * 2 + 1024;
+  auto launch = [&](auto packed) {
+    constexpr auto kernel = prefill_kernel<HD, decltype(packed)::value>;
+    const cudaError_t error = ensure_smem_attr<kernel>(smem);
+    if (error != cudaSuccess) return error;
+    return launch_ex(kernel, dim3((unsigned)(pairs * P.nkv)), dim3(kThreads), (size_t)smem, stream, 1, true, q, k, v, P, H,
+                     scale_log2);
+  };
+  return H.heads > 1 ? launch(std::true_type{}) : launch(std::false_type{});
 }
 
 }  // namespace

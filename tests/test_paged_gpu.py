@@ -509,6 +509,14 @@ def test_prefill_attention(new, past, nq, nkv, hd):
         assert torch.equal(same, out[: sum(new)])
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rep,nkv", [(2, 4), (3, 1), (5, 2), (12, 1), (40, 2), (128, 1), (130, 1)])
+def test_prefill_of_few_tokens_each(rep, nkv, hd):
+    """A tile holds all query heads of a kv head for a few rows: groups that fill it and that do not, contexts, rows behind."""
+    new, past = [1, 0, 7, 26, 3, 1, 60], [0, 300, 130, 5, 125, 128, 0]
+    test_prefill_attention(new, past, rep * nkv, nkv, hd)
+
+
 def test_prefill_of_many_sequences_longest_anywhere():
     """More sequences than a warp has lanes, and a few with the longest in the middle."""
     g = _gen(21)
