@@ -8,7 +8,7 @@
 // the exponentials alone do.
 //
 // A CTA holds two tiles of 128 query rows that share a kv head (stages 0 and 1: two heads of the group, or two row tiles; a
-// tile's rows are tokens of one head, or tokens x heads where the sequences are short).  Their scores S (fp32, 128 columns
+// tile's rows are tokens x heads, or tokens of one head).  Their scores S (fp32, 128 columns
 // each) and outputs O (fp32, hd columns each) lie in the tensor memory; the probabilities P (fp16) overwrite the scores they
 // come from and feed the second product from there.
 //   warps 0-3, 4-7: the softmax of stage 0 / 1, one thread per row (two threads per row: 716 against 685 us in the case
@@ -597,16 +597,16 @@ cudaError_t make_map(CUtensorMap* map, const half* data, int64_t tokens, int64_t
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-// Query heads per tile: all of a kv head's where that takes at most 7/8 of the tiles for sequences of the average length (a
-// few tokens each: 16 tokens of 4 heads fill half a tile, not an eighth of four), else one.  32 / 8 heads: 128 sequences of
-// one token over 2001 453 against 214 us, 256 of 20 tokens 368 against 140, 64 of 200 135.9 against 131.0 (7/8 of the tiles);
-// 100 of 10 to 910 573 against 597 (15/16 of them, and a few rows' last step is masked as a whole tile's).
+// Query heads per tile: all of a kv head's unless that takes more tiles for sequences of the average length (5 heads leave 3
+// of 128 rows empty), which also lets a tile's rows see keys that differ less.  32 / 8 heads, one against all heads a tile:
+// 128 sequences of one token over 2001 450 against 210 us, 256 of 20 tokens 340 against 165, 64 of 200 135.6 against 126.8,
+// 100 of 10 to 910 580 against 535, 16 of 1000 196.9 against 197.0; 64 / 8 heads, 20 of 450 194 against 176.
 TileHeads heads_per_tile(const PrefillParams& P) {
   const int64_t rep = P.nq / P.nkv, length = (P.tokens_q + P.seqs - 1) / P.seqs;
   int heads = 1;
   if (rep <= kTile) {
     const int64_t rows = kTile / rep;
-    if (8 * ((length + rows - 1) / rows) <= 7 * ((length + kTile - 1) / kTile * rep)) heads = (int)rep;
+    if ((length + rows - 1) / rows <= (length + kTile - 1) / kTile * rep) heads = (int)rep;
   }
   return {heads, kTile / heads, (int)rep / heads, (65536 + heads - 1) / heads};
 }
