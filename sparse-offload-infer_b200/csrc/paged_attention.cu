@@ -36,8 +36,8 @@
 // without exchange 15.5 us, a bulk copy per padded row 18.2, this 12.3).
 //
 // Measured (GPU time): 4 bits, two sequences of 131072 and 100003, 40 / 8 heads: 61 us for 255 MB = 4.2 TB/s (0.64 of the
-// measured copy rate), bound by issuing 294 instructions per 16 positions and kv head (integer pipe 47%, fp16 / fp32 pipe
-// 26%, tensor pipe 26% busy, DRAM 0.66); register tiles without a ring 96 us, 32-position tiles 81.  One sequence of 777
+// measured copy rate), bound by issuing 303 instructions per 16 positions and kv head (integer pipe 47%, fp16 / fp32 pipe
+// 25%, tensor pipe 25% busy); register tiles without a ring 96 us, 32-position tiles 81.  One sequence of 777
 // positions: 5.0 us in one launch, against 8.7 with a second kernel that joins.
 #include <algorithm>
 

@@ -8,12 +8,13 @@
 // the exponentials alone do.
 //
 // A CTA holds two tiles of 128 query rows that share a kv head (stages 0 and 1: two heads of the group, or two row tiles; a
-// tile's rows are tokens x heads, or tokens of one head).  Their scores S (fp32, 128 columns
-// each) and outputs O (fp32, hd columns each) lie in the tensor memory; the probabilities P (fp16) overwrite the scores they
-// come from and feed the second product from there.
+// tile's rows are tokens x heads, or tokens of one head).  Their scores S (fp32, 128 columns each) and outputs O (fp32, hd
+// columns each) lie in the tensor memory; the probabilities P (fp16) overwrite the scores they come from and feed the second
+// product from there.
 //   warps 0-3, 4-7: the softmax of stage 0 / 1, one thread per row (two threads per row: 716 against 685 us in the case
-//           below).  P is handed over in two halves, so that the second product starts after the first 64 keys, and one in
-//           four pairs of exponentials is computed on the fp32 pipe.  These warps take most of the CTA's registers.
+//           below; the first half's probabilities with the old maximum, beside the search for the new one: 570 against 553).
+//           P is handed over in two halves, so that the second product starts after the first 64 keys, and one in four
+//           pairs of exponentials is computed on the fp32 pipe.  These warps take most of the CTA's registers.
 //   warp 8: loads Q, then K and V tiles of 128 keys through a ring of four slots (TMA, 128-byte swizzle).  A last V tile
 //           with fewer keys has its other rows cleared: what lies behind a sequence may be anything, and 0 * NaN counts.
 //   warp 9: issues the products in the order  S0(j) P1V(j-1) S1(j) P0V(j) -- while the tensor core works on one
@@ -24,17 +25,17 @@
 // probabilities carry a factor 2^7 and are rounded once to fp16, which keeps 11 bits down to 2^-21 of the largest; the sum
 // is fp32 over the unrounded ones and the factor cancels.
 // A masked score is selected away, but a non-finite V in a masked place of a shared tile would still reach the product:
-// rows whose result is not finite are computed again one by one over exactly the keys they see.
+// rows whose scores or result are not finite are computed again one by one over exactly the keys they see.
 //
 // The grid holds one CTA per pair of tiles and kv head, an upper bound from the token counts (row bounds are read on the
 // device).
 //
 // Measured (8192 tokens, 40 / 8 heads, hd 128): products issued from a single lane's branch 832 us, maxima over eight chains
-// and packed pairs 685, products issued by a convergent warp 600, registers / halves / fp32 pipe / coalesced output 565 =
-// 1215 TFLOP/s, 0.75 of the measured burst rate of a library product and 0.88 of its sustained one, whose power limit this
+// and packed pairs 685, products issued by a convergent warp 600, registers / halves / fp32 pipe / coalesced output 555 =
+// 1238 TFLOP/s, 0.77 of the measured burst rate of a library product and 0.90 of its sustained one, whose power limit this
 // kernel reaches too.  7 unequal prompts (3828 tokens, 16 / 8 heads): 29 us, the longest one's 12 steps of 1.6 us plus 6 us
 // of start and end and a second round of CTAs.  One in eight / three in eight / half of the pairs on the fp32 pipe: 31.6 /
-// 31.7 / 32.3 us against 31.2 there.  hd 64, two chunks of 512 and 1000 rows over 4012 and 3047 keys, 32 / 4 heads: 73 us,
+// 31.7 / 32.3 us against 31.2 there.  hd 64, two chunks of 512 and 1000 rows over 4012 and 3047 keys, 32 / 4 heads: 68 us,
 // 192 CTAs in two rounds; P beside S in the tensor memory, so that scores run ahead, measured the same (the two warps of a
 // scheduler spend their exponentials' phases together).
 #include <cuda.h>
