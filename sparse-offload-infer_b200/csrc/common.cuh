@@ -148,6 +148,38 @@ __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
 
 __device__ __forceinline__ void fence_mbar_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 
+// All threads of the cluster arrive and wait (warp-wide).
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// What lies at this CTA's shared-memory address p, in CTA `rank` of the cluster.
+__device__ __forceinline__ float cluster_read(const float* p, int rank) {
+  float v;
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}"
+               : "=f"(v)
+               : "r"(smem_u32(p)), "r"(rank)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 cluster_read(const float2* p, int rank) {
+  float2 v;
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %2, %3;\n ld.shared::cluster.v2.f32 {%0, %1}, [a];\n}"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(smem_u32(p)), "r"(rank)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_read(const float4* p, int rank) {
+  float4 v;
+  asm volatile(
+      "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %4, %5;\n ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(smem_u32(p)), "r"(rank)
+      : "memory");
+  return v;
+}
+
 // Order this thread's earlier generic-proxy shared-memory accesses before
 // subsequent async-proxy (bulk copy) writes to shared memory.
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }

@@ -371,20 +371,6 @@ __device__ __forceinline__ void join_warps(const float* s_acc, const float (*s_m
   }
 }
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
-}
-
-// The float at this CTA's shared-memory address p, in CTA `rank` of the cluster.
-__device__ __forceinline__ float cluster_read(const float* p, int rank) {
-  float v;
-  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}"
-               : "=f"(v)
-               : "r"(smem_u32(p)), "r"(rank)
-               : "memory");
-  return v;
-}
-
 // kRuns: a tile's runs (more than one where a page is smaller than a 4-bit tile).
 template <int HD, bool Q4, int kRuns, bool kJoined>
 __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)

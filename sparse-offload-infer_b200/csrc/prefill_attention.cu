@@ -28,7 +28,9 @@
 // rows whose scores or result are not finite are computed again one by one over exactly the keys they see.
 //
 // The grid holds one CTA per pair of tiles and kv head, an upper bound from the token counts (row bounds are read on the
-// device).
+// device).  Where those leave at least half of the SMs idle and the contexts are long, a cluster of two, four or eight CTAs
+// shares a pair's keys and joins its sums through distributed shared memory: 32 / 8 heads, 512 tokens over 8000 107 -> 69 us
+// and over 30000 382 -> 228, 128 over 32000 383 -> 116, four times 5 over 16000 182 -> 56, 64 over 1000 20.0 -> 19.8.
 //
 // Measured (8192 tokens, 40 / 8 heads, hd 128): products issued from a single lane's branch 832 us, maxima over eight chains
 // and packed pairs 685, products issued by a convergent warp 600, registers / halves / fp32 pipe / coalesced output 555 =
@@ -59,6 +61,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;          // the maximum follows when exceeded by 2^8
 constexpr unsigned kFmaPairs = 0x22;  // which of 8 pairs of exponentials go to the fp32 pipe (see above)
 constexpr float kLift = 7.f;          // factor 2^7 on the probabilities
+constexpr int64_t kSplitKeys = 512;   // keys that a CTA of a cluster has at least
 
 __device__ int g_prefill_error;
 
@@ -127,9 +130,10 @@ __device__ __forceinline__ void ex2_pair(uint64_t x2, float& a, float& b) {
 }
 
 // A query tile's heads of a kv head, its rows of the sequence (128 / heads), the kv head's groups of that many heads; inv:
-// 2^16 / heads, rounded up (a tile row's number times that, shifted back, is the quotient).
-struct TileHeads {
-  int heads, rows, groups, inv;
+// 2^16 / heads, rounded up (a tile row's number times that, shifted back, is the quotient).  ranks: CTAs that share the keys
+// of a pair of tiles.
+struct Layout {
+  int heads, rows, groups, inv, ranks;
 };
 
 // A CTA's work: two query tiles of sequence rows q0.., keys k0.., kv head kvh.
@@ -138,15 +142,15 @@ struct Work {
   int row[2], head[2], tiles[2];  // first row in the sequence, first query head, key tiles (0: nothing to do)
 };
 
-// The pair of query tiles that blockIdx.x stands for (warp-wide; false: none).  Tile t of a sequence and kv head is head
+// The pair of query tiles with this index (warp-wide; false: none).  Tile t of a sequence and kv head is head
 // group t % groups, rows t / groups * rows ..  A sequence's pairs run from the last to the first, and of up to 32 sequences
 // those with more keys come first (more: as they are given), so that short work fills the end of the launch.
 template <bool kPacked>
-__device__ __forceinline__ bool find_work(const PrefillParams& P, const TileHeads& H, int lane, Work& w) {
+__device__ __forceinline__ bool find_work(const PrefillParams& P, const Layout& H, int index, int lane, Work& w) {
   const int rows_tile = kPacked ? H.rows : kTile;
   auto tiles_of = [&](int n) { return (n + rows_tile - 1) / rows_tile * H.groups; };
-  w.kvh = blockIdx.x % P.nkv;
-  int want = blockIdx.x / P.nkv;
+  w.kvh = index % P.nkv;
+  int want = index / P.nkv;
   for (int base = 0; base < P.seqs; base += 32) {
     const int i = base + lane;
     int q0 = 0, lq = 0, k0 = 0, lk = 0;
@@ -227,11 +231,11 @@ __device__ __noinline__ void redo_row(const PrefillParams& P, const half* q, int
   for (int e = 0; e < E; ++e) out[lane * E + e] = __float2half_rn(acc[e] / l);
 }
 
-// kPacked: a tile holds several heads.
-template <int HD, bool kPacked>
+// kPacked: a tile holds several heads.  kSplit: the CTAs of a cluster share the keys.
+template <int HD, bool kPacked, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                   const __grid_constant__ CUtensorMap v_map, const PrefillParams P, const TileHeads H, const float scale_log2) {
+                   const __grid_constant__ CUtensorMap v_map, const PrefillParams P, const Layout H, const float scale_log2) {
   constexpr int kBox = kTile * 128;              // bytes of a TMA box: 128 rows of 64 fp16
   constexpr int kBoxes = HD / 64;
   constexpr int kTileBytes = kBoxes * kBox;
@@ -247,7 +251,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
   Work w;
-  if (!find_work<kPacked>(P, H, lane, w)) return;           // the same for every warp
+  const int rank = kSplit ? blockIdx.x % H.ranks : 0;
+  if (!find_work<kPacked>(P, H, kSplit ? blockIdx.x / H.ranks : blockIdx.x, lane, w)) return;  // alike for the whole cluster
+  int first = 0;                                 // this CTA's first key tile
+  if (kSplit) {
+    const int each = (max(max(w.tiles[0], w.tiles[1]), 0) + H.ranks - 1) / H.ranks;
+    first = rank * each;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (w.tiles[s] >= 0) w.tiles[s] = min(max(w.tiles[s] - first, 0), each);
+  }
   const int steps = w.tiles[0] > w.tiles[1] ? w.tiles[0] : w.tiles[1];
 
   if (warp == 9) {
@@ -284,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool valid = row < w.lq && (!kPacked || token < H.rows);
     const bool idle = !__any_sync(0xffffffffu, valid);  // whatever its P is stays in its rows
     // keys this row sees; a row behind the last one is worked on as that one (with none it would mask every tile) and dropped
-    const int limit = max(min(row, w.lq - 1) + 1 + w.lk - w.lq, 0);
+    const int limit = max(min(row, w.lq - 1) + 1 + w.lk - w.lq - first * kTile, 0);  // (from this CTA's first key)
     // worst: the largest score of all, NaN if one is NaN (the polynomial loses them)
     float m = -INFINITY, l = 0.f, worst = -INFINITY;
     bool ok = true;
@@ -318,7 +331,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < 8; ++i) tops[i] = max2(__uint_as_float(x[0][2 * i]), __uint_as_float(x[0][2 * i + 1]));
 #pragma unroll
       for (int i = 16; i < 128; i += 2)
-        tops[(i >> 1) & 7] = max3(tops[(i >> 1) & 7], __uint_as_float(x[i >> 5][i & 31]), __uint_as_float(x[i >> 5][(i & 31) + 1]));
+        tops[(i >> 1) & 7] =
+            max3(tops[(i >> 1) & 7], __uint_as_float(x[i >> 5][i & 31]), __uint_as_float(x[i >> 5][(i & 31) + 1]));
       float top = max2(max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[4]), max3(tops[5], tops[6], tops[7]));
       top *= scale_log2;
       worst = max2(worst, top);
@@ -375,8 +389,105 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.p_full[s]);
     }
-    // the row's result
-    if (tiles >= 0 && ok && !idle) {
+    if constexpr (kSplit) {
+      // The CTAs' sums, maxima and sums of weights (NaN: a score that is not finite), where the tiles were, which no product
+      // and no load needs any more; every CTA then finishes its share of the 256 rows.
+      float4* sums = reinterpret_cast<float4*>(smem);
+      float2* stats = reinterpret_cast<float2*>(smem + 2 * kTile * HD * 4);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (w.tiles[x] > 0) ok = ok && __all_sync(0xffffffffu, wait(sh, &sh.o_full[x], 0));
+      tc::fence_after();
+      if (ok && tiles >= 0 && !idle) {
+        if (tiles > 0) {
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            tc::ld32(o, O + 32 * c);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              sums[(s * kTile + r) * (HD / 4) + ((8 * c + i) ^ (r & 7))] =
+                  make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                              __uint_as_float(o[4 * i + 3]));
+          }
+        }
+        stats[s * kTile + r] = make_float2(m, worst <= 3.4e38f ? l : __int_as_float(0x7fffffff));
+      }
+      __syncwarp();
+      cluster_sync();
+      // kRows rows at a time, two CTAs' sums at a time: their loads wait for one another only there
+      constexpr int kLanes = HD / 4, kStep = 2 * kTile / kLanes, kRows = HD / 32;  // threads of a row, rows of all threads
+      const int c = threadIdx.x % kLanes;
+      for (int i0 = threadIdx.x / kLanes; ok && i0 < 2 * kTile / H.ranks; i0 += kStep * kRows) {
+        float M[kRows], L[kRows], v[kRows][4];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) M[u] = -INFINITY, L[u] = v[u][0] = v[u][1] = v[u][2] = v[u][3] = 0.f;
+        int at[kRows], heads_at[kRows];          // the rows' places in the sequence (-1: no such row) and heads
+        bool any = false;
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+          const int x = (i0 + u * kStep) * H.ranks + rank, xr = x % kTile, xt = kPacked ? xr * H.inv >> 16 : xr;
+          const bool second = x >= kTile;
+          at[u] = (second ? w.row[1] : w.row[0]) + xt;
+          heads_at[u] = (second ? w.head[1] : w.head[0]) + (kPacked ? xr - xt * H.heads : 0);
+          if ((second ? w.tiles[1] : w.tiles[0]) < 0 || at[u] >= w.lq || (kPacked && xt >= H.rows)) at[u] = -1;
+          any = any || at[u] >= 0;
+        }
+        if (!__any_sync(0xffffffffu, any)) continue;
+        for (int k = 0; k < H.ranks; k += 2) {
+          float2 ml[kRows][2];
+          float4 o[kRows][2];
+#pragma unroll
+          for (int u = 0; u < kRows; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int x = (i0 + u * kStep) * H.ranks + rank;
+              ml[u][e] = cluster_read(stats + x, k + e);
+              o[u][e] = cluster_read(sums + x * (HD / 4) + (c ^ (x & 7)), k + e);
+            }
+#pragma unroll
+          for (int u = 0; u < kRows; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 t = ml[u][e];
+              const float top = fmaxf(M[u], t.x), f = M[u] == top ? 1.f : ex2(M[u] - top);
+              const float g = t.x == -INFINITY ? 0.f : ex2(t.x - top);
+              const float4 y = t.x == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f) : o[u][e];  // (else never written)
+              M[u] = top;
+              L[u] = fmaf(g, t.y, L[u] * f);
+              v[u][0] = fmaf(g, y.x, v[u][0] * f), v[u][1] = fmaf(g, y.y, v[u][1] * f);
+              v[u][2] = fmaf(g, y.z, v[u][2] * f), v[u][3] = fmaf(g, y.w, v[u][3] * f);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+          bool bad = false;
+          if (at[u] >= 0) {
+            const float inv = 1.f / L[u];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              v[u][e] *= inv;
+              bad = bad || !(fabsf(v[u][e]) <= 3.4e38f);
+            }
+            if (at[u] + 1 + w.lk - w.lq <= 0) v[u][0] = v[u][1] = v[u][2] = v[u][3] = 0.f, bad = false;
+            *reinterpret_cast<uint2*>(P.out + ((int64_t)(w.q0 + at[u]) * P.nq + heads_at[u]) * HD + 4 * c) =
+                make_uint2(h2_as_u32(__floats2half2_rn(v[u][0], v[u][1])), h2_as_u32(__floats2half2_rn(v[u][2], v[u][3])));
+          }
+          unsigned again = __ballot_sync(0xffffffffu, bad);
+          while (again) {
+            const int src = (__ffs(again) - 1) / kLanes * kLanes;  // the first lane of the row
+            again &= ~(kLanes == 32 ? 0xffffffffu : 0xffffu << src);
+            const int rr = __shfl_sync(0xffffffffu, at[u], src), h = __shfl_sync(0xffffffffu, heads_at[u], src);
+            __syncwarp();
+            redo_row<HD>(P, P.q + (int64_t)(w.q0 + rr) * P.q_token + h * P.q_head, w.k0, rr + 1 + w.lk - w.lq, w.kvh,
+                         P.out + ((int64_t)(w.q0 + rr) * P.nq + h) * HD, scale_log2, lane);
+          }
+        }
+      }
+      __syncwarp();
+      cluster_sync();  // nobody leaves while its sums are read
+    } else if (tiles >= 0 && ok && !idle) {  // the row's result
       constexpr int kPieces = HD / 8;
       uint4* stage = reinterpret_cast<uint4*>(s_q + s * kTileBytes + (warp & 3) * (32 * HD * 2));
       bool good = limit == 0 || fabsf(worst) <= 3.4e38f;
@@ -460,13 +571,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       uint8_t* dst = s_kv + slot * kTileBytes;
-      const int rows = w.lk - j * kTile;         // valid rows of the tile
+      const int rows = w.lk - (first + j) * kTile;  // valid rows of the tile
       const bool clear = (e & 1) && rows < kTile;
       uint64_t* bar = clear ? &sh.v_landed : &sh.kv_full[slot];
       if (lane == 0) {
         mbar_arrive_expect_tx(bar, kTileBytes);
         for (int x = 0; x < kBoxes; ++x)
-          tc::tma_load_3d(dst + x * kBox, e & 1 ? &v_map : &k_map, 64 * x, w.kvh, w.k0 + j * kTile, bar);
+          tc::tma_load_3d(dst + x * kBox, e & 1 ? &v_map : &k_map, 64 * x, w.kvh, w.k0 + (first + j) * kTile, bar);
       }
       ++issued;
       if (clear) {                               // at most once: the sequence's last tile
@@ -556,6 +667,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
     }
+    if (kSplit) {
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
   }
   tc::fence_before();
   __syncthreads();
@@ -602,20 +718,27 @@ cudaError_t make_map(CUtensorMap* map, const half* data, int64_t tokens, int64_t
 // of 128 rows empty), which also lets a tile's rows see keys that differ less.  32 / 8 heads, one against all heads a tile:
 // 128 sequences of one token over 2001 450 against 210 us, 256 of 20 tokens 340 against 165, 64 of 200 135.6 against 126.8,
 // 100 of 10 to 910 580 against 535, 16 of 1000 196.9 against 197.0; 64 / 8 heads, 20 of 450 194 against 176.
-TileHeads heads_per_tile(const PrefillParams& P) {
+Layout layout_of(const PrefillParams& P) {
   const int64_t rep = P.nq / P.nkv, length = (P.tokens_q + P.seqs - 1) / P.seqs;
   int heads = 1;
   if (rep <= kTile) {
     const int64_t rows = kTile / rep;
     if ((length + rows - 1) / rows <= (length + kTile - 1) / kTile * rep) heads = (int)rep;
   }
-  return {heads, kTile / heads, (int)rep / heads, (65536 + heads - 1) / heads};
+  return {heads, kTile / heads, (int)rep / heads, (65536 + heads - 1) / heads, 1};
+}
+
+// CTAs that share the keys of a pair of tiles: as many as the GPU has to spare, with at least kSplitKeys keys each.
+int ranks_for(int64_t ctas, int64_t keys) {
+  int ranks = 1;
+  while (ranks < 8 && ctas * ranks * 2 <= 148 && keys >= kSplitKeys * ranks * 2) ranks *= 2;
+  return ranks;
 }
 
 template <int HD>
 cudaError_t prefill_hd(const PrefillParams& P, cudaStream_t stream) {
   CUtensorMap q, k, v;
-  const TileHeads H = heads_per_tile(P);
+  Layout H = layout_of(P);
   cudaError_t e = make_map(&q, P.q, P.tokens_q, P.nq, HD, P.q_token, P.q_head, H.heads);
   if (e != cudaSuccess) return e;
   k = v = q;  // no keys: never read
@@ -629,14 +752,18 @@ cudaError_t prefill_hd(const PrefillParams& P, cudaStream_t stream) {
   if (pairs * P.nkv > 0x7fffffff) return cudaErrorInvalidValue;
   const float scale_log2 = (1.0f / sqrtf((float)HD)) * kLog2e;
   const int smem = (2 + kSlots) * kTile * HD * 2 + 1024;
-  auto launch = [&](auto packed) {
-    constexpr auto kernel = prefill_kernel<HD, decltype(packed)::value>;
+  H.ranks = ranks_for(pairs * P.nkv, P.tokens_k / P.seqs);
+  auto launch = [&](auto packed, auto split) {
+    constexpr auto kernel = prefill_kernel<HD, decltype(packed)::value, decltype(split)::value>;
     const cudaError_t error = ensure_smem_attr<kernel>(smem);
     if (error != cudaSuccess) return error;
-    return launch_ex(kernel, dim3((unsigned)(pairs * P.nkv)), dim3(kThreads), (size_t)smem, stream, 1, true, q, k, v, P, H,
-                     scale_log2);
+    return launch_ex(kernel, dim3((unsigned)(pairs * P.nkv * H.ranks)), dim3(kThreads), (size_t)smem, stream,
+                     dim3((unsigned)H.ranks), true, q, k, v, P, H, scale_log2);
   };
-  return H.heads > 1 ? launch(std::true_type{}) : launch(std::false_type{});
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (H.heads > 1) return H.ranks > 1 ? launch(Yes{}, Yes{}) : launch(Yes{}, No{});
+  return H.ranks > 1 ? launch(No{}, Yes{}) : launch(No{}, No{});
 }
 
 }  // namespace

@@ -517,6 +517,48 @@ def test_prefill_of_few_tokens_each(rep, nkv, hd):
     test_prefill_attention(new, past, rep * nkv, nkv, hd)
 
 
+SPLIT = [  # new, past, nq, nkv: few tiles over long contexts, which several CTAs share
+    ([16], [8000], 8, 2),
+    ([1], [5000], 16, 1),
+    ([200, 3], [3000, 10], 5, 1),
+    ([130], [4100], 2, 1),
+    ([300, 0, 2], [-200, 700, 6000], 3, 1),  # rows without keys beside a long context
+    ([40, 9], [2600, 2047], 24, 2),
+    ([1], [1100], 3, 3),
+]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,past,nq,nkv", SPLIT)
+def test_prefill_over_long_contexts(new, past, nq, nkv, hd):
+    test_prefill_attention(new, past, nq, nkv, hd)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_prefill_over_long_contexts_with_non_finite_values(bad, hd):
+    """A non-finite key or value anywhere in a shared context: the rows that see it are what the formula gives."""
+    n, ctx, nq, nkv = 20, 4500, 4, 2
+    g = _gen(18)
+    q = torch.randn(n, nq, hd, generator=g).half()
+    k, v = (torch.randn(ctx, nkv, hd, generator=g).half() for _ in range(2))
+    for at in (3, 1500, ctx - 5):
+        kb, vb = k.clone(), v.clone()
+        kb[at, 0, 9] = bad
+        vb[at + 1, 1, 7] = bad
+        cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+        got = ops.prefill_attention(q.to(DEV), kb.to(DEV), vb.to(DEV), cu, cu_seqlens_k=_cum([ctx])).cpu().numpy()
+        seen = np.arange(ctx)[None] <= np.arange(n)[:, None] + ctx - n
+        with np.errstate(invalid="ignore"):
+            out, _, _ = oracle.attention(*(t.numpy().astype(np.float64) for t in (q, kb, vb)), seen)
+        _, mag, dot = oracle.attention(*(t.numpy().astype(np.float64) for t in (q, k, v)), seen)
+        mag = np.maximum(mag, np.abs(v.numpy().astype(np.float64)).max())
+        fine = np.isfinite(out)
+        assert np.array_equal(got[~fine], out[~fine], equal_nan=True), at
+        err = np.abs(got[fine].astype(np.float64) - out[fine])
+        assert np.all(err <= oracle.attention_bound(np.where(fine, out, 0), mag, dot)[fine]), at
+
+
 def test_prefill_of_many_sequences_longest_anywhere():
     """More sequences than a warp has lanes, and a few with the longest in the middle."""
     g = _gen(21)
