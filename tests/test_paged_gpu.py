@@ -559,6 +559,50 @@ def test_prefill_over_long_contexts_with_non_finite_values(bad, hd):
         assert np.all(err <= oracle.attention_bound(np.where(fine, out, 0), mag, dot)[fine]), at
 
 
+def test_prefill_and_decode_of_two_streams_at_once_captured():
+    """Shared contexts (clusters) and ranges beside one another on two streams, eager and from graphs: the same bits."""
+    nq, nkv, hd, page = 8, 2, 128, 16
+    g = _gen(19)
+    lens = [9000, 300, 70, 2000]
+    table, pages = _table(lens, page, 3)
+    pools = ops.paged_kv_alloc(pages, nkv, page, hd, 4, device=DEV)
+    k, v = (torch.randn(sum(lens), nkv, hd, generator=g).half().to(DEV) for _ in range(2))
+    one = torch.ones(9000, hd // 2, device=DEV)
+    table = table.to(DEV)
+    ops.paged_kv_append(None, k, v, *pools, table, torch.zeros(4, dtype=torch.int32, device=DEV), one, 0 * one,
+                        cu_seqlens=_cum(lens))
+    q = torch.randn(4, nq, hd, generator=g).half().to(DEV)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    x = torch.randn(24, nq, hd, generator=g).half().to(DEV)
+    cu, ctx = _cum([17, 7]), _cum([9000, 300])
+    calls = [lambda: ops.prefill_attention(x, k[:9300], v[:9300], cu, cu_seqlens_k=ctx),
+             lambda: ops.paged_decode_attention(q, *pools, table, lens_d)]
+    want = [call().clone() for call in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    graphs, outs = [], []
+    for call, stream in zip(calls, streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(call())
+        graphs.append(graph)
+    for _ in range(5):
+        got = []
+        for call, stream in zip(calls, streams):
+            with torch.cuda.stream(stream):
+                got.append(call())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
 def test_prefill_of_many_sequences_longest_anywhere():
     """More sequences than a warp has lanes, and a few with the longest in the middle."""
     g = _gen(21)
