@@ -982,9 +982,9 @@ def _int32(name: str, what: str, t, n: int, dev: int) -> int:
 
 def _out_rows(name: str, out, like, shape) -> torch.Tensor:
     if out is None:
-        if like.shape == shape and like.is_contiguous() and like.dtype is _F16:
-            return torch.empty_like(like)
-        return like.new_empty(shape, dtype=_F16)
+        if like.dtype is not _F16:
+            return like.new_empty(shape, dtype=_F16)
+        return torch.empty_like(like) if like.shape == shape and like.is_contiguous() else like.new_empty(shape)
     if not (out.is_cuda and out.dtype == _F16 and out.shape == shape and out.is_contiguous() and out.data_ptr() % 16 == 0):
         _fail(name, f": out must be a contiguous, 16-byte aligned float16 CUDA tensor of shape {shape}")
     if out.get_device() != like.get_device():
@@ -1059,9 +1059,12 @@ def paged_kv_read(k_pages, v_pages, block_table, cu_seqlens, total: int, out=Non
     cu_at = _int32(name, "cu_seqlens", cu_seqlens, B + 1, dev)
     if total < 0:
         _fail(name, ": total must be >= 0")
-    ko, vo = out if out is not None else (None, None)
-    ko = _out_rows(name, ko, k_pages, (total, nkv, hd))
-    vo = _out_rows(name, vo, k_pages, (total, nkv, hd))
+    shape = (total, nkv, hd)
+    if out is None:
+        ko = _out_rows(name, None, k_pages, shape)
+        vo = torch.empty_like(ko)
+    else:
+        ko, vo = (_out_rows(name, o, k_pages, shape) for o in out)
     if total:
         _call_on(dev, "soinfer_paged_kv_read", cache, cu_at, B, total, ko.data_ptr(), vo.data_ptr())
     return ko, vo
