@@ -892,7 +892,9 @@ _ROWS = struct.Struct("Pqq")                # soinfer_rows
 PAGED_HEAD_DIMS = (64, 128)
 # no workspace up to this many positions in a table row and kv heads x sequences (paged_attention.cu)
 PAGED_CLUSTER_POSITIONS, PAGED_CLUSTER_UNITS = 4096, 37
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# (a torch built without CUDA has neither of torch's direct functions, and no tensor that would get here)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 _F16, _F32, _U8, _I32 = torch.float16, torch.float32, torch.uint8, torch.int32
 
 
