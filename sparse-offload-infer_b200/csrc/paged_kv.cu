@@ -209,10 +209,13 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
 #pragma unroll
           for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
           // 1 / sqrt by Newton's iteration r += r (1 - a r^2) / 2 from the fp32 value: 2^-22 -> 2^-43 -> 64-bit rounding
+          // (not from the 0 of an infinite mean square, which is the result)
           const double a = ss * (1.0 / HD) + (double)P.eps;
           double r = (double)rsqrtf((float)a);
-          r = fma(0.5 * r, fma(-a * r, r, 1.0), r);
-          r = fma(0.5 * r, fma(-a * r, r, 1.0), r);
+          if (r != 0.0) {
+            r = fma(0.5 * r, fma(-a * r, r, 1.0), r);
+            r = fma(0.5 * r, fma(-a * r, r, 1.0), r);
+          }
           inv = (float)r;
         }
 #pragma unroll

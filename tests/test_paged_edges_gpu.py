@@ -1,0 +1,59 @@
+"""Values and calls at the edge of what the paged-cache and prompt operators take."""
+import numpy as np
+import pytest
+import torch
+
+import soinfer.ops as ops
+from tests import paged_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+INF, NAN = float("inf"), float("nan")
+
+
+def _ints(*x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_append_of_non_finite_rows_under_the_head_norm(hd, bits):
+    """A head row with an infinity: 1 / sqrt(inf) = 0, so its finite values become 0 and the infinity NaN, with the partner
+    of its rotation pair; in 4 bits the groups of these two.  A NaN makes the whole row NaN.  Queries and keys alike."""
+    T, nq, nkv, page, eps = 7, 3, 2, 16, 1e-6
+    g = _gen(hd + bits)
+    x = torch.randn(T, nq + 2 * nkv, hd, generator=g).half()
+    for t, (value, d) in enumerate([(INF, 0), (-INF, 5), (NAN, 9), (INF, hd - 1), (-INF, hd // 2 + 3), (INF, 40)]):
+        x[t, 1, d] = x[t, nq + t % nkv, d] = value
+    x[5, nq + 1, 3] = -INF  # two of them
+    cos, sin = (t.cpu() for t in ops.precompute_rope_table(hd, 1e4, 32, "cpu"))
+    qw, kw = ((1 + 0.2 * torch.randn(hd, generator=g)).half() for _ in range(2))
+    pools = ops.paged_kv_alloc(1, nkv, page, hd, bits, DEV)
+    d = x.to(DEV)
+    q, k = ops.paged_kv_append(d[:, :nq], d[:, nq : nq + nkv], d[:, nq + nkv :], *pools, _ints([0]), _ints(3), cos.to(DEV),
+                               sin.to(DEV), cu_seqlens=_ints(0, T), q_norm=qw.to(DEV), k_norm=kw.to(DEV), eps=eps, return_k=True)
+    c, s = cos.numpy()[3 : 3 + T], sin.numpy()[3 : 3 + T]
+    want = [t.cpu().numpy() for t in ops.paged_kv_alloc(1, nkv, page, hd, bits, DEV)]
+    with np.errstate(all="ignore"):
+        for got, rows, w in ((q, x[:, :nq], qw), (k, x[:, nq : nq + nkv], kw)):
+            exact = oracle.rotate(rows.numpy(), w.numpy(), eps, c, s)
+            got = got.cpu().numpy().astype(np.float64)
+            assert np.array_equal(np.isnan(got), np.isnan(exact))
+            bad = ~np.isfinite(rows.numpy()).all(-1)
+            assert np.all(got[bad][np.isfinite(exact[bad])] == 0)
+            # |x^| <= sqrt(hd) |w|: half a step and about twelve fp32 roundings of two such terms
+            most = np.nanmax(np.abs(exact))
+            fine = np.isfinite(exact)
+            assert np.all(np.abs(got - exact)[fine] <= oracle.HALF_ULP16 * np.abs(exact[fine]) + 24 * 2.0**-24 * 2 * most + 2.0**-25)
+        kx = oracle.rotate(x[:, nq : nq + nkv].numpy(), kw.numpy(), eps, c, s, np.float32)
+        for t in range(T):
+            oracle.put(want, bits, page, 0, 3 + t, kx[t], x[t, nq + nkv :].numpy())
+        kr, vr = ops.paged_kv_read(*pools, _ints([0]), _ints(0, 3 + T), 3 + T)
+        for t in range(T):
+            wk, wv = oracle.get(want, bits, page, hd, 0, 3 + t)
+            assert np.array_equal(kr[3 + t].cpu().numpy(), wk.astype(np.float16), equal_nan=True), t
+            assert np.array_equal(vr[3 + t].cpu().numpy(), wv.astype(np.float16), equal_nan=True), t
