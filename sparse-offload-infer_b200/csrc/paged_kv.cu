@@ -166,7 +166,6 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
       const int h = (is_q ? s : is_k ? s - q_steps : s - q_steps - kv_steps) * kRows + sub;
       const bool on = h < (is_q ? P.nq : P.nkv);
       const bool cached = on && id >= 0;
-      if (!placed) cur[r][0] = cur[r][1] = make_uint4(0, 0, 0, 0);
       uint64_t x[2][4];
       unpack8(cur[r][0], x[0]);
       unpack8(cur[r][1], x[1]);
@@ -235,7 +234,8 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
         unpack2(mul2(a, sn[i]), q0, q1);
         x[1][i] = pack2(__fadd_rn(p0, q0), __fadd_rn(p1, q1));
       }
-      const uint4 lo = pack8(x[0]), hi = pack8(x[1]);
+      uint4 lo = pack8(x[0]), hi = pack8(x[1]);
+      if (!placed) lo = hi = make_uint4(0, 0, 0, 0);  // (whatever its row, norm and table hold)
       half* out = is_q ? P.q_out + ((int64_t)t * P.nq + h) * HD : P.k_out + ((int64_t)t * P.nkv + h) * HD;
       if (on && (is_q || P.k_out)) {
         reinterpret_cast<uint4*>(out)[l] = lo;

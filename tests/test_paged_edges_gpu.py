@@ -57,3 +57,20 @@ def test_append_of_non_finite_rows_under_the_head_norm(hd, bits):
             wk, wv = oracle.get(want, bits, page, hd, 0, 3 + t)
             assert np.array_equal(kr[3 + t].cpu().numpy(), wk.astype(np.float16), equal_nan=True), t
             assert np.array_equal(vr[3 + t].cpu().numpy(), wv.astype(np.float16), equal_nan=True), t
+
+
+@pytest.mark.parametrize("eps,weight", [(0.0, 1.0), (1e-6, INF)])
+def test_tokens_without_a_place_are_zeros_whatever_the_norm(eps, weight):
+    """Beyond the tables, of no sequence, with a negative start: zeros, where the norm of a zero row would be NaN."""
+    hd, nkv = 64, 2
+    cos, sin = ops.precompute_rope_table(hd, 1e4, 10, DEV)
+    x = torch.randn(6, 3 * nkv, hd, generator=_gen(1)).half().to(DEV)
+    w = torch.ones(hd, dtype=torch.float16, device=DEV)
+    w[3] = weight
+    pools = ops.paged_kv_alloc(2, nkv, 16, hd, 16, DEV)
+    args = (x[:, :nkv], x[:, nkv : 2 * nkv], x[:, 2 * nkv :], *pools, _ints([0], [1]), _ints(8, -1), cos, sin)
+    q, k = ops.paged_kv_append(*args, cu_seqlens=_ints(0, 3, 4), q_norm=w, k_norm=w, eps=eps, return_k=True)
+    for t in (q, k):  # rows 0, 1 stand at 8 and 9; row 2 at 10, row 3 at -1, rows 4 and 5 nowhere
+        assert torch.count_nonzero(t[2:]) == 0
+        assert torch.all(t[:2].isnan() | (t[:2] != 0) if weight == INF else t[:2].isfinite())
+    assert torch.count_nonzero(pools[0][1]) == 0
