@@ -537,7 +537,8 @@ int soinfer_quantize_pack_int4(const void* w, int32_t dtype, int64_t N, int64_t 
  *            (one per position); positions 2 m and 2 m + 1 share head_dim/4 words, word w holds values 4 w + (0..3), the
  *            even position's in nibbles 0..3, the odd one's in nibbles 4..7.
  *            scale = fp16(max(amax / 7, 2^-14)), code = clamp(rint(x / scale), -7, 7) (two's complement), value =
- *            code * scale.  A group that holds an infinity or a NaN, or whose scale exceeds fp16, reads as NaN. */
+ *            code * scale.  A group that holds an infinity or a NaN, or whose scale exceeds fp16, has code 0 and the
+ *            scale NaN, and reads as NaN (a scale may not be infinite). */
 typedef struct soinfer_paged_cache {
   void* k_pages;
   void* v_pages;

@@ -13,7 +13,7 @@
 //      and the odd one's in the high half (masking gives one value at two positions, the product's reduction axis).  Each
 //      position owns whole 16-bit units, so rows are appended without reading what is there.
 // A scale is fp16(max(amax / 7, 2^-14)) and the code is chosen against the rounded scale.  A row (K: group) that holds
-// an infinity or a NaN gets code 0 and a non-finite scale: it reads as NaN throughout.
+// an infinity or a NaN, or whose scale is beyond fp16, gets code 0 and the scale NaN: it reads as NaN throughout.
 #pragma once
 
 #include "common.cuh"
@@ -64,10 +64,12 @@ __device__ __forceinline__ Owner owner_of(const int32_t* cu, int n, int t, int l
   return {n, 0, 0, 0};
 }
 
-// fp16 scale of a group with largest magnitude amax (NaN and infinity stay what they are).
+// fp16 scale of a group with largest magnitude amax; NaN where that is not finite.  (An infinite scale would be lost where
+// a product with the codes 0 leaves a rounding error below zero: a score of -inf, which has no weight.)
 __device__ __forceinline__ half scale_of(float amax) {
   const float s = __fdiv_rn(amax, 7.f);
-  return __float2half_rn(s < kMinScale ? kMinScale : s);
+  const half h = __float2half_rn(s < kMinScale ? kMinScale : s);
+  return __hisinf(h) ? __ushort_as_half(0x7fff) : h;
 }
 
 // Codes against the fp16 scale s (inv = 1 / s): rint(x / s), which needs no clamp since s is at least (1 - 2^-11) of the

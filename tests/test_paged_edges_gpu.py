@@ -74,3 +74,45 @@ def test_tokens_without_a_place_are_zeros_whatever_the_norm(eps, weight):
         assert torch.count_nonzero(t[2:]) == 0
         assert torch.all(t[:2].isnan() | (t[:2] != 0) if weight == INF else t[:2].isfinite())
     assert torch.count_nonzero(pools[0][1]) == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cols", [2, 640])
+@pytest.mark.parametrize("route", ["infinity", "scale"])
+def test_four_bit_keys_that_read_as_nan_reach_the_output(route, cols, hd):
+    """A key group with an infinity, or whose scale is beyond fp16, reads as NaN: so is every head that attends to it."""
+    B, n, nq, nkv, page = 96, 20, 4, 2, 16
+    g = _gen(hd + cols)
+    k, v = (torch.randn(B * n, nkv, hd, generator=g).half() for _ in range(2))
+    cos, sin = ops.precompute_rope_table(hd, 1e4, n, DEV)
+    table = torch.full((B, cols), -1, dtype=torch.int32)
+    table[:, :2] = torch.arange(2 * B, dtype=torch.int32).view(B, 2)
+    weight = None
+    for b in range(B):  # head 0 of one position of each sequence
+        at = b * n + 1 + b % (n - 1)
+        if route == "infinity":
+            k[at, 0, b * 5 % hd] = INF if b % 2 else -INF
+        else:  # normalised to +- sqrt(hd) at one value, times a weight of 65504: beyond 7 times fp16's largest scale, 458528
+            k[at, 0] = 0
+            k[at, 0, b * 5 % hd] = 1.0 if b % 2 else -1.0
+    if route == "scale":
+        # 8 * 65504 (hd 64) may fall below 458528 after a rotation; the random rows, at most 4.9 * 65504, stay below it
+        grow = 1.3 if hd == 64 else 1.0
+        cos, sin = grow * cos, grow * sin
+        weight = torch.full((hd,), 65504.0, dtype=torch.float16, device=DEV)
+    pools = ops.paged_kv_alloc(2 * B, nkv, page, hd, 4, DEV)
+    cu = _ints(*range(0, B * n + 1, n))
+    ops.paged_kv_append(None, k.to(DEV), v.to(DEV), *pools, table.to(DEV), torch.zeros(B, dtype=torch.int32, device=DEV), cos,
+                        sin, cu_seqlens=cu, k_norm=weight)
+    kr, _ = ops.paged_kv_read(*pools, table.to(DEV), cu, B * n)
+    assert kr.view(B, n, nkv, hd)[:, :, 0].isnan().any(-1).any(-1).all()
+    q = torch.randn(B, nq, hd, generator=g).half().to(DEV)
+    if route == "scale":
+        q *= 2.0**-10
+    lens = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    # (values of very different sizes: sums over the codes' offsets that do not come out exactly)
+    wide = (q.cpu() * torch.exp2(torch.randint(-10, 1, (B, nq, hd), generator=g))).half().to(DEV)
+    for x in (q, wide):
+        got = ops.paged_decode_attention(x, *pools, table.to(DEV), lens)
+        assert got[:, : nq // nkv].isnan().all()
+        assert got[:, nq // nkv :].isfinite().all()
