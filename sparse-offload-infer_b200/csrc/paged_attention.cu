@@ -56,6 +56,7 @@ constexpr int kMostLen = 1 << 30;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;      // the running maximum follows when exceeded by 2^8 (it moves in a few tiles, not in half)
 constexpr float kLift = 7.f;      // factor 2^7 on the probabilities (it cancels)
+constexpr float kNoScore = -3.0e38f;  // the maximum of positions without a finite score: below every score, above no position
 
 // Positions a warp takes at a time, tiles in its ring, CTAs that an SM holds (shared memory and registers), the split's limit
 // and units (see above and below).
@@ -344,10 +345,13 @@ __device__ __forceinline__ void accumulate(float (*acc)[4], const uint8_t* tile,
   }
 }
 
-// The output.  Without positions the sum of weights is 0; else it is at least 2^(7 - 16) (the weight of the position whose
-// score and scale, below 2^16, set the maximum), or NaN: a NaN of the query or of a key never becomes the maximum, but its
-// weight is one.
-__device__ __forceinline__ half result(float num, float den) { return __float2half_rn(den == 0.f ? 0.f : num / den); }
+// The output.  The maximum M is -inf without positions only, and the output 0 then; it is kNoScore where every score is
+// -inf or NaN, and the sum of weights 0 or NaN, which the output 0 / 0 or NaN is too.  Else the sum is at least 2^(7 - 16)
+// (the weight of the position whose score and scale, below 2^16, set the maximum), or NaN: a NaN of the query or of a key
+// never becomes the maximum, but its weight is one.
+__device__ __forceinline__ half result(float num, float den, float M) {
+  return __float2half_rn(M == -INFINITY ? 0.f : num / den);
+}
 
 // Value index of row half r (0: row g, 1: row g + 8) of accumulator i.
 template <int HD, bool Q4>
@@ -519,7 +523,8 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
       const uint8_t* tile = ring + slot * kBytes;
       const bool full_tile = p0 + kTile <= p_end && (held & ((1u << kRuns) - 1)) == (1u << kRuns) - 1;
       float s[kSub][4], sv[kSub][2];
-      float top[2] = {-INFINITY, -INFINITY};
+      float top[2];
+      top[0] = top[1] = held & ((1u << kRuns) - 1) ? kNoScore : -INFINITY;
 #pragma unroll
       for (int u = 0; u < kSub; ++u) {
         scores<HD, Q4>(s[u], tile, 16 * u, qf, bias, g, t);
@@ -645,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
           den = fmaf(f, cluster_read(sums + HD + 1, r), den);
           num = fmaf(f, cluster_read(sums + d, r), num);
         }
-        P.out[(row + h) * HD + d] = result(num, den);
+        P.out[(row + h) * HD + d] = result(num, den, M);
       }
       cluster_sync();  // nobody leaves while its sums are read
     } else {
@@ -654,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
         float num, den, M;
         join_warps<HD, kStride>(s_acc, s_m, s_l, h, d, num, den, M);
         if (done_slot < 0) {
-          P.out[(row + h) * HD + d] = result(num, den);
+          P.out[(row + h) * HD + d] = result(num, den, M);
         } else {
           float* ws = workspace<Q4>(P).pieces + (done_slot * (rep < kCols ? rep : kCols) + h) * (HD + 2);
           ws[d] = num;
@@ -718,7 +723,7 @@ __global__ void __launch_bounds__(HD * kParts) paged_join_kernel(const PagedDeco
     num = fmaf(f, s_num[i][d], num);
     den = fmaf(f, s_den[i], den);
   }
-  P.out[((int64_t)split.b * P.nq + kvh * rep + h) * HD + d] = result(num, den);
+  P.out[((int64_t)split.b * P.nq + kvh * rep + h) * HD + d] = result(num, den, M);
 }
 
 int64_t head_groups(int64_t nq, int64_t nkv) { return (nq / nkv + kCols - 1) / kCols; }

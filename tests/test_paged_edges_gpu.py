@@ -116,3 +116,50 @@ def test_four_bit_keys_that_read_as_nan_reach_the_output(route, cols, hd):
         got = ops.paged_decode_attention(x, *pools, table.to(DEV), lens)
         assert got[:, : nq // nkv].isnan().all()
         assert got[:, nq // nkv :].isfinite().all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cols", [5, 640])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_decode_scores_of_minus_infinity(bits, cols, hd):
+    """exp(-inf) is 0 beside a finite score; where every score is -inf the output is 0 / 0, not that of an empty sequence."""
+    page, nq, nkv, n = 16, 4, 1, 70
+    lens = [n, n, n, 0, 1]
+    B, g = len(lens), _gen(3)
+    k, v = (torch.randn(B, n, nkv, hd, generator=g).half() for _ in range(2))
+    q = torch.randn(B, nq, hd, generator=g).half()
+    channel = 5  # one value of every key that a query of infinity meets
+    k[:, :, :, channel] = -1 - k[:, :, :, channel].abs()
+    q[0, 1, channel] = INF             # every score -inf: NaN; the other heads are not touched
+    q[3, :, channel] = q[4, 2, channel] = INF
+    q[1:3, :, channel] = 1 + q[1:3, :, channel].abs()
+    if bits == 16:
+        k[1, :40, :, channel] = -INF   # whole tiles of -inf, then finite ones
+        k[2, :, :, channel] = -INF     # nothing else: every head NaN
+    need = -(-n // page)
+    table = torch.full((B, cols), -1, dtype=torch.int32)
+    table[:, :need] = torch.arange(B * need, dtype=torch.int32).view(B, need)
+    pools = ops.paged_kv_alloc(B * need, nkv, page, hd, bits, DEV)
+    if bits == 16:
+        for pool, rows in zip(pools, (k, v)):
+            at = torch.zeros(B, need * page, nkv, hd, dtype=torch.float16)
+            at[:, :n] = rows
+            pool.copy_(at.view(B * need, page, nkv, hd).transpose(1, 2))
+    else:
+        one = torch.ones(n, hd // 2, device=DEV)
+        ops.paged_kv_append(None, *(t.reshape(B * n, nkv, hd).to(DEV) for t in (k, v)), *pools, table.to(DEV),
+                            torch.zeros(B, dtype=torch.int32, device=DEV), one, 0 * one,
+                            cu_seqlens=_ints(*range(0, B * n + 1, n)))
+    got = ops.paged_decode_attention(q.to(DEV), *pools, table.to(DEV), _ints(*lens)).cpu()
+    nan = torch.zeros(B, nq, dtype=torch.bool)
+    nan[0, 1] = nan[4, 2] = True
+    if bits == 16:
+        nan[2] = True
+    assert torch.equal(got.isnan().all(-1), nan) and torch.equal(got.isnan().any(-1), nan)
+    assert torch.count_nonzero(got[3]) == 0
+    if bits == 16:
+        out, mag, dot = oracle.attention(q[1:2].numpy(), k[1, 40:].numpy().astype(np.float64), v[1, 40:].numpy().astype(np.float64),
+                                         np.ones((1, n - 40), bool))
+        assert np.all(np.abs(got[1:2].numpy().astype(np.float64) - out) <= oracle.attention_bound(out, mag, dot))
+    none = torch.full_like(table, -1)  # positions, but no page: nothing to attend to, whatever the query
+    assert torch.count_nonzero(ops.paged_decode_attention(q.to(DEV), *pools, none.to(DEV), _ints(*lens))) == 0
