@@ -130,10 +130,20 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
   } else if (t < P.seqs) {
     pos = __ldg(P.start + t);
   }
-  const bool placed = pos >= 0 && pos < P.table_rows;  // a token of no sequence, or beyond the tables: zeros, no row
+  if (pos < 0 || pos >= P.table_rows) {  // of no sequence, or beyond the tables: zeros, whatever the row and the norm hold
+    for (int s = s0; s < s_end && s < q_steps + kv_steps; ++s) {
+      const bool is_q = s < q_steps;
+      const int h = (is_q ? s : s - q_steps) * kRows + sub;
+      half* out = is_q ? P.q_out + ((int64_t)t * P.nq + h) * HD : P.k_out + ((int64_t)t * P.nkv + h) * HD;
+      if (h < (is_q ? P.nq : P.nkv) && (is_q || P.k_out)) {
+        reinterpret_cast<uint4*>(out)[l] = make_uint4(0, 0, 0, 0);
+        reinterpret_cast<uint4*>(out)[kLanes + l] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    return;
+  }
   const int page = 1 << P.cache.page_shift;
-  int id = -1;
-  if (placed) id = page_of(P.cache, b, (int)pos);
+  const int id = page_of(P.cache, b, (int)pos);
   const int slot = (int)pos & (page - 1);
   const int64_t k_block = k_block_bytes(page, HD, Q4), v_block = v_block_bytes(page, HD, Q4);
   uint8_t* k_base = P.cache.k + (int64_t)id * P.nkv * k_block;
@@ -141,7 +151,7 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
 
   uint64_t c[4], sn[4];  // pairs, as the rows'
   {
-    const int64_t row = (placed ? pos : 0) * (HD / 2) + 8 * l;
+    const int64_t row = pos * (HD / 2) + 8 * l;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float4 a = __ldg(reinterpret_cast<const float4*>(P.cos_t + row) + i);
@@ -234,8 +244,7 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
         unpack2(mul2(a, sn[i]), q0, q1);
         x[1][i] = pack2(__fadd_rn(p0, q0), __fadd_rn(p1, q1));
       }
-      uint4 lo = pack8(x[0]), hi = pack8(x[1]);
-      if (!placed) lo = hi = make_uint4(0, 0, 0, 0);  // (whatever its row, norm and table hold)
+      const uint4 lo = pack8(x[0]), hi = pack8(x[1]);
       half* out = is_q ? P.q_out + ((int64_t)t * P.nq + h) * HD : P.k_out + ((int64_t)t * P.nkv + h) * HD;
       if (on && (is_q || P.k_out)) {
         reinterpret_cast<uint4*>(out)[l] = lo;
