@@ -1111,7 +1111,7 @@ def prefill_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None) -> torch
         _fail(name, ": num_q_heads must be a multiple of num_kv_heads")
     for x in (q, k, v):
         # rows are loaded as boxes of a tensor map, which has no zero strides (an expanded dimension)
-        if 0 in x.stride() and any(n > 1 and st == 0 for n, st in zip(x.shape, x.stride())):
+        if 0 in x.stride() and x.numel() and any(n > 1 and st == 0 for n, st in zip(x.shape, x.stride())):
             return prefill_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu_seqlens, cu_seqlens_k, out)
     n = cu_seqlens.numel()
     if n < 1:

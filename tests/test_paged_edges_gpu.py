@@ -163,3 +163,13 @@ def test_decode_scores_of_minus_infinity(bits, cols, hd):
         assert np.all(np.abs(got[1:2].numpy().astype(np.float64) - out) <= oracle.attention_bound(out, mag, dot))
     none = torch.full_like(table, -1)  # positions, but no page: nothing to attend to, whatever the query
     assert torch.count_nonzero(ops.paged_decode_attention(q.to(DEV), *pools, none.to(DEV), _ints(*lens))) == 0
+
+
+def test_prefill_of_empty_expanded_rows():
+    """Keys shared by expansion, of which there are none: every query gives zeros."""
+    q = torch.randn(5, 4, 64, generator=_gen(2)).half().to(DEV)
+    none = torch.empty(0, 1, 64, dtype=torch.float16, device=DEV).expand(0, 2, 64)
+    got = ops.prefill_attention(q, none, none, _ints(0, 5), cu_seqlens_k=_ints(0, 0))
+    assert got.shape == q.shape and torch.count_nonzero(got) == 0
+    empty = torch.empty(0, 1, 64, dtype=torch.float16, device=DEV).expand(0, 4, 64)
+    assert ops.prefill_attention(empty, none, none, _ints(0, 0)).shape == (0, 4, 64)
