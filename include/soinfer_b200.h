@@ -572,7 +572,7 @@ int soinfer_paged_kv_append(const soinfer_paged_cache* cache, const soinfer_rows
 /* Positions 0 .. of every sequence b as packed fp16 rows cu_seqlens[b] ..
  * cu_seqlens[b + 1] of k_out / v_out [tokens, num_kv_heads, head_dim] (4-bit
  * rows as the values they stand for; a position without a page: zeros; rows of
- * no sequence: left as they were). */
+ * no sequence: left as they were).  k_out and v_out must not overlap. */
 int soinfer_paged_kv_read(const soinfer_paged_cache* cache, const int32_t* cu_seqlens, int64_t num_seqs, int64_t tokens,
                           soinfer_half* k_out, soinfer_half* v_out, void* stream);
 

@@ -1067,6 +1067,8 @@ def paged_kv_read(k_pages, v_pages, block_table, cu_seqlens, total: int, out=Non
         vo = torch.empty_like(ko)
     else:
         ko, vo = (_out_rows(name, o, k_pages, shape) for o in out)
+        if abs(ko.data_ptr() - vo.data_ptr()) < 2 * ko.numel():
+            _fail(name, ": the outputs must not overlap")
     if total:
         _call_on(dev, "soinfer_paged_kv_read", cache, cu_at, B, total, ko.data_ptr(), vo.data_ptr())
     return ko, vo

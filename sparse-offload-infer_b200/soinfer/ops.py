@@ -260,8 +260,8 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: tor
                   total: int, out: tuple[torch.Tensor, torch.Tensor] | None = None):
     """B200 addition: the first cu_seqlens[b + 1] - cu_seqlens[b] cached positions of every sequence as packed fp16 rows
     (k, v), each [total, NKV, hd], total = cu_seqlens[-1] -- the context that prefill_attention needs to continue a
-    prompt.  4-bit rows come back as the values they stand for, positions without a page as zeros.  out = (k, v): rows of
-    no sequence are left as they were (in fresh outputs they are unset)."""
+    prompt.  4-bit rows come back as the values they stand for, positions without a page as zeros.  out = (k, v), which
+    must not overlap: rows of no sequence are left as they were (in fresh outputs they are unset)."""
     return _C.paged_kv_read(k_pages, v_pages, block_table, cu_seqlens, total, out)
 
 

@@ -173,3 +173,14 @@ def test_prefill_of_empty_expanded_rows():
     assert got.shape == q.shape and torch.count_nonzero(got) == 0
     empty = torch.empty(0, 1, 64, dtype=torch.float16, device=DEV).expand(0, 4, 64)
     assert ops.prefill_attention(empty, none, none, _ints(0, 0)).shape == (0, 4, 64)
+
+
+def test_read_into_overlapping_outputs_is_refused():
+    pools = ops.paged_kv_alloc(2, 2, 16, 64, 16, DEV)
+    buf = torch.zeros(2 * 20 * 2 * 64, dtype=torch.float16, device=DEV)
+    a, b = buf[: 20 * 128].view(20, 2, 64), buf[20 * 128 :].view(20, 2, 64)
+    ops.paged_kv_read(*pools, _ints([0, 1]), _ints(0, 20), 20, out=(a, b))
+    shifted = buf[128 : 21 * 128].view(20, 2, 64)
+    for out in ((a, a), (a, shifted), (shifted, a)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.paged_kv_read(*pools, _ints([0, 1]), _ints(0, 20), 20, out=out)
