@@ -28,7 +28,7 @@
 // rows whose scores or result are not finite are computed again one by one over exactly the keys they see.
 //
 // The grid holds one CTA per pair of tiles and kv head, an upper bound from the token counts (row bounds are read on the
-// device).  Where those leave at least half of the SMs idle and the contexts are long, a cluster of two, four or eight CTAs
+// device).  Where the GPU holds two, four or eight times as many CTAs and the contexts are long, a cluster of as many
 // shares a pair's keys and joins its sums through distributed shared memory: 32 / 8 heads, 512 tokens over 8000 107 -> 69 us
 // and over 30000 382 -> 228, 128 over 32000 383 -> 116, four times 5 over 16000 182 -> 56, 64 over 1000 20.0 -> 19.8.
 //
@@ -728,10 +728,15 @@ Layout layout_of(const PrefillParams& P) {
   return {heads, kTile / heads, (int)rep / heads, (65536 + heads - 1) / heads, 1};
 }
 
-// CTAs that share the keys of a pair of tiles: as many as the GPU has to spare, with at least kSplitKeys keys each.
+// CTAs that share the keys of a pair of tiles: as many as the GPU holds at once, with at least kSplitKeys keys each on the
+// average (one long context among many short sequences is not seen: 5 tokens over 16000 beside 40 of one token 180 us).  A
+// cluster lies within one group of SMs, so that fewer than 148 / 4 and 148 / 8 clusters fit at one CTA per SM.  One token each
+// of 8 / 1 heads over 16000: clusters of eight 34.2 us for 15 pairs and 63.6 for 16, of four 55 for 16 and 57 for 33 but 107
+// for 34, of two 99 for 34.
 int ranks_for(int64_t ctas, int64_t keys) {
+  constexpr int64_t kFit[3] = {74, 33, 15};  // clusters of 2, 4, 8
   int ranks = 1;
-  while (ranks < 8 && ctas * ranks * 2 <= 148 && keys >= kSplitKeys * ranks * 2) ranks *= 2;
+  for (int i = 0; i < 3 && ctas <= kFit[i] && keys >= kSplitKeys * ranks * 2; ++i) ranks *= 2;
   return ranks;
 }
 
@@ -746,9 +751,11 @@ cudaError_t prefill_hd(const PrefillParams& P, cudaStream_t stream) {
     if ((e = make_map(&k, P.k, P.tokens_k, P.nkv, HD, P.k_token, P.k_head, 1)) != cudaSuccess) return e;
     if ((e = make_map(&v, P.v, P.tokens_k, P.nkv, HD, P.v_token, P.v_head, 1)) != cudaSuccess) return e;
   }
-  // sum over sequences of ceil(n ceil(lq / rows) / 2) <= (n (tokens / rows + seqs') + seqs') / 2, seqs' of them not empty
+  // the most that sum over sequences of ceil(n t / 2), t = ceil(lq / rows), may be with seqs of them not empty: t is at most
+  // (lq + rows - 1) / rows, and a half is rounded up only where n is odd
   const int64_t n = H.groups, seqs = P.seqs < P.tokens_q ? P.seqs : P.tokens_q;
-  const int64_t pairs = (n * (P.tokens_q / H.rows + seqs) + seqs + 1) / 2;
+  const int64_t tiles = (P.tokens_q + seqs * (H.rows - 1)) / H.rows;
+  const int64_t pairs = (n * tiles + n % 2 * seqs) / 2;
   if (pairs * P.nkv > 0x7fffffff) return cudaErrorInvalidValue;
   const float scale_log2 = (1.0f / sqrtf((float)HD)) * kLog2e;
   const int smem = (2 + kSlots) * kTile * HD * 2 + 1024;

@@ -132,3 +132,18 @@ def test_prompts(new, past, nq, nkv, hd):
                     err = cover.off(got[at : at + n, h], want, tolerance)
                     assert err <= 1, (layout, tolerance, b, h, err)
                 at += n
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("seqs,past", [(15, 8200), (16, 4200), (33, 2100), (34, 1100), (74, 1100), (75, 1100)])
+def test_prompts_where_clusters_just_fit(seqs, past, hd):
+    """Contexts shared by eight, four and two CTAs in as many clusters as the GPU holds, and in one more."""
+    test_prompts([1] * (seqs - 1) + [17], [past] * seqs, 8, 1, hd)  # (17 of 16 rows: the last one's second tile)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,nq,nkv", [([17] * 5, 8, 1), ([16, 33, 1, 0, 17], 8, 1), ([129, 1, 128], 1, 1), ([129] * 3, 130, 1),
+                                        ([26, 25, 51], 5, 1), ([1] * 9, 384, 2)])
+def test_prompts_that_need_every_pair_of_tiles(new, nq, nkv, hd):
+    """Lengths one beyond a tile, in layouts with one and several head groups: the grid holds every pair there may be."""
+    test_prompts(new, [0] * len(new), nq, nkv, hd)
