@@ -16,7 +16,7 @@
 // The softmax statistics and both sums are fp32.
 //
 // Work split.  A sequence's kv head with up to 8 of its query heads is a unit.
-//   Few units (kClusterUnits) over tables that name few positions (kClusterMost): a unit is one cluster of eight CTAs, each
+//   Few units (cluster_units) over tables that name few positions (kClusterMost): a unit is one cluster of eight CTAs, each
 //   an eighth of the positions; they join through distributed shared memory.  One launch, no workspace: 777 4-bit positions of
 //   8 kv heads 5.0 us against 7.8 by ranges; 8 unequal sequences of up to 4096 fp16 positions, 4 kv heads, 11.3 against 12.9.
 //   Beyond, a cluster's idle CTAs and the eight-fold start cost more than they bring (64 unequal sequences of up to 4000 4-bit
@@ -50,7 +50,11 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kCluster = 8;
-constexpr int kClusterUnits = 148 * 2 / kCluster;  // one wave of CTAs
+// The most units that go to clusters: two CTAs per SM, or as many clusters as the GPU holds at once where those are fewer.  (A
+// cluster lies within one group of SMs: 33 with fp16 rows of 128, whose rings let an SM hold two; 48 and more with the
+// others.  fp16, hd 128, 34 units of 500 / 2000 / 4000 positions: 9.0 / 13.8 / 19.5 us against 8.9 / 11.3 / 15.3 by ranges,
+// 33 units 7.2 / 10.4 / 14.9 against 8.9 / 11.2 / 15.3.)
+constexpr int cluster_units(bool q4, int64_t hd) { return !q4 && hd == 128 ? 33 : 148 * 2 / kCluster; }
 constexpr int kCols = 8;          // query heads per CTA
 constexpr int kMostLen = 1 << 30;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -735,7 +739,7 @@ cudaError_t decode_runs(const PagedDecodeParams& P, cudaStream_t stream) {
   constexpr int kSmem = kWarps * Plan<Q4>::kStages * Tile<HD, Q4>::kBytes, kCtas = Plan<Q4>::kCtas;
   cudaError_t e;
   const int64_t all = (int64_t)P.seqs * units;
-  if (all <= kClusterUnits && (int64_t)P.cache.table_cols << P.cache.page_shift <= Plan<Q4>::kClusterMost) {
+  if (all <= cluster_units(Q4, HD) && (int64_t)P.cache.table_cols << P.cache.page_shift <= Plan<Q4>::kClusterMost) {
     if ((e = ensure_smem_attr<paged_decode_kernel<HD, Q4, kRuns, true>>(kSmem)) != cudaSuccess) return e;
     return launch_ex(paged_decode_kernel<HD, Q4, kRuns, true>, dim3((unsigned)units, (unsigned)P.seqs, kCluster),
                      dim3(kThreads), kSmem, stream, dim3(1, 1, kCluster), true, P, groups, scale_log2);
@@ -764,7 +768,8 @@ cudaError_t decode_hd(const PagedDecodeParams& P, cudaStream_t stream) {
 int64_t paged_decode_workspace_bytes(int64_t seqs, int64_t nq, int64_t nkv, int64_t hd, int64_t positions) {
   // for either type of page
   const int64_t most = std::min(Plan<true>::kClusterMost, Plan<false>::kClusterMost);
-  if (seqs * nkv * head_groups(nq, nkv) <= kClusterUnits && positions <= most) return 0;
+  const int64_t units = std::min(cluster_units(true, hd), cluster_units(false, hd));
+  if (seqs * nkv * head_groups(nq, nkv) <= units && positions <= most) return 0;
   const int64_t ctas = std::max(Plan<true>::kCtas, Plan<false>::kCtas), heads = std::min<int64_t>(nq / nkv, kCols);
   return ctas * (int64_t)(sizeof(Split) + 2 * heads * (hd + 2) * sizeof(float));
 }

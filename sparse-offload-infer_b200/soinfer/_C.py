@@ -890,8 +890,8 @@ def head_norm_rope(q, k, v, q_norm, k_norm, cos_vals, sin_vals, k_cache, v_cache
 _PAGED_CACHE = struct.Struct("PPPqqqqqqq")  # soinfer_paged_cache
 _ROWS = struct.Struct("Pqq")                # soinfer_rows
 PAGED_HEAD_DIMS = (64, 128)
-# no workspace up to this many positions in a table row and kv heads x sequences (paged_attention.cu)
-PAGED_CLUSTER_POSITIONS, PAGED_CLUSTER_UNITS = 4096, 37
+# no workspace up to this many positions in a table row and kv heads x sequences, head_dim 64 and 128 (paged_attention.cu)
+PAGED_CLUSTER_POSITIONS, PAGED_CLUSTER_UNITS, PAGED_CLUSTER_UNITS_128 = 4096, 37, 33
 # (a torch built without CUDA has neither of torch's direct functions, and no tensor that would get here)
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
@@ -1088,7 +1088,8 @@ def paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, out=None)
     out = _out_rows(name, out, q, shape)
     if B:
         positions, nbytes, ws_at = block_table.shape[1] * page, 0, None
-        if positions > PAGED_CLUSTER_POSITIONS or B * nkv * -(-nq // (8 * nkv)) > PAGED_CLUSTER_UNITS:
+        units = B * nkv * -(-nq // (8 * nkv))
+        if positions > PAGED_CLUSTER_POSITIONS or units > (PAGED_CLUSTER_UNITS if hd == 64 else PAGED_CLUSTER_UNITS_128):
             # a workspace of the call's own: two captured graphs or streams never share one
             nbytes = lib().soinfer_paged_decode_workspace_bytes(B, nq, nkv, hd, positions)
             ws = q.new_empty((nbytes // 2,))

@@ -134,6 +134,14 @@ def test_prompts(new, past, nq, nkv, hd):
                 at += n
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("seqs", [33, 34, 37, 38])
+def test_decode_where_clusters_just_fit(seqs, hd, bits):
+    """The most sequences that clusters take, and one more."""
+    _decode([300 + 7 * i for i in range(seqs)], 16, 8, 1, hd, bits, 0)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("seqs,past", [(15, 8200), (16, 4200), (33, 2100), (34, 1100), (74, 1100), (75, 1100)])
 def test_prompts_where_clusters_just_fit(seqs, past, hd):
