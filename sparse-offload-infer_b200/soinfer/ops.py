@@ -281,5 +281,6 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     """B200 addition: decode_attention for sequences of different lengths over a paged cache (fp16 or 4-bit pages): one
     query per sequence, q [B, NQ, hd], over its first seq_lens[b] positions (int32 [B], read on the device:
     graph-capturable; at most max_pages * page_size).  Positions without a page are skipped; a sequence without positions
-    gives zeros."""
+    gives zeros, one whose scores are all -inf gives NaN.  An infinite fp16 value gives an infinity, or NaN where its weight
+    is below 2^-31 of the largest."""
     return _C.paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, out)

@@ -184,3 +184,26 @@ def test_read_into_overlapping_outputs_is_refused():
     for out in ((a, a), (a, shifted), (shifted, a)):
         with pytest.raises(RuntimeError, match="overlap"):
             ops.paged_kv_read(*pools, _ints([0, 1]), _ints(0, 20), 20, out=out)
+
+
+@pytest.mark.parametrize("cols", [20, 640])
+@pytest.mark.parametrize("bad", [INF, -INF, NAN])
+def test_decode_of_non_finite_values(bad, cols):
+    """A value that is not finite reaches that value of its kv head's outputs, as the formula has it where its weight is not
+    far below the others', and nothing if it lies behind the sequence."""
+    lens, page, nq, nkv, hd = [300, 300, 20], 16, 6, 2, 64
+    table = torch.full((3, cols), -1, dtype=torch.int32)
+    table[:, :19] = torch.arange(57, dtype=torch.int32).view(3, 19)
+    g = _gen(5)
+    q = torch.randn(3, nq, hd, generator=g).half().to(DEV)
+    k, v = (torch.randn(57, nkv, page, hd, generator=g).half().to(DEV) for _ in range(2))
+    lens = _ints(*lens)
+    want = ops.paged_decode_attention(q, k, v, table.to(DEV), lens)
+    v[19 * 0 + 7, 1, 3, 9] = bad   # position 115 of the first
+    v[19 * 1 + 18, 0, 12, 5] = bad  # position 300 of the second: behind it
+    v[19 * 2 + 1, 0, 4:] = bad     # position 20 and on of the third
+    got = ops.paged_decode_attention(q, k, v, table.to(DEV), lens)
+    hit = got[0, 3:, 9]
+    assert hit.isnan().all() if bad != bad else torch.all(hit == bad)
+    got[0, 3:, 9] = want[0, 3:, 9] = 0
+    assert torch.equal(got, want)
