@@ -100,7 +100,7 @@ __device__ __forceinline__ float ex2(float x) {
 // Positions of sequence b: its length, at most what its table can name (the length limit keeps positions in 32 bits).
 __device__ __forceinline__ int seq_len(const PagedDecodeParams& P, int b) {
   const int64_t table = (int64_t)P.cache.table_cols << P.cache.page_shift;
-  const int most = table < kMostLen ? (int)table : kMostLen, n = __ldg(P.lens + b);
+  const int most = table < kMostLen ? (int)table : kMostLen, n = ld_i32(P.lens + b);
   return n < 0 ? 0 : n > most ? most : n;
 }
 
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, Plan<Q4>::kPerSm)
     for (int j = 0; j < G; ++j) {
       uint4 u = make_uint4(0, 0, 0, 0);
       if (g < heads)
-        u = __ldg(reinterpret_cast<const uint4*>(P.q + b * P.q_token + (qh0 + g) * P.q_head) + 4 * j + t);
+        u = reinterpret_cast<const uint4*>(P.q + b * P.q_token + (qh0 + g) * P.q_head)[4 * j + t];
       qf[j][0] = u.x, qf[j][1] = u.y, qf[j][2] = u.z, qf[j][3] = u.w;
       if (Q4) {
         float sum = 0.f;

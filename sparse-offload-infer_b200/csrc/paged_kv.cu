@@ -112,8 +112,8 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
                            : is_k ? P.k + t * P.k_token + h * P.k_head : P.v + t * P.v_token + h * P.v_head;
     x[0] = x[1] = make_uint4(0, 0, 0, 0);
     if (s < s_end && h < (is_q ? P.nq : P.nkv)) {
-      x[0] = ldg_stream_u4(src + 8 * l);
-      x[1] = ldg_stream_u4(src + HD / 2 + 8 * l);
+      x[0] = ld_stream_u4(src + 8 * l);
+      x[1] = ld_stream_u4(src + HD / 2 + 8 * l);
     }
   };
   // the first rows before anything else: their loads do not wait for the position
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
     b = o.b;
     if (b < P.seqs && t >= o.first) pos = (int64_t)o.x + (t - o.first);
   } else if (t < P.seqs) {
-    pos = __ldg(P.start + t);
+    pos = P.start[t];
   }
   if (pos < 0 || pos >= P.table_rows) {  // of no sequence, or beyond the tables: zeros, whatever the row and the norm hold
     for (int s = s0; s < s_end && s < q_steps + kv_steps; ++s) {
@@ -268,8 +268,7 @@ __global__ void __launch_bounds__(32 * kWarps, 5) paged_append_kernel(const Page
 // all of them the pair's values (hd = 64: half as many bytes each).  Every lane reads 16 + 16 bytes of codes and writes 128.
 template <int HD, bool Q4>
 __global__ void __launch_bounds__(32 * kWarps)
-    paged_read_kernel(const PagedCache C, const int32_t* __restrict__ cu, const int seqs, const int tokens,
-                      half* __restrict__ k_out, half* __restrict__ v_out) {
+    paged_read_kernel(const PagedCache C, const int32_t* cu, const int seqs, const int tokens, half* k_out, half* v_out) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -295,8 +294,8 @@ __global__ void __launch_bounds__(32 * kWarps)
         for (int h = lane / kLanes; h < C.nkv; h += kRows) {
           uint4 ko = make_uint4(0, 0, 0, 0), vo = ko;
           if (id >= 0) {
-            ko = ldg_stream_u4(reinterpret_cast<const uint4*>(k_base + h * kbb) + (int64_t)(slot + r) * kLanes + l);
-            vo = ldg_stream_u4(reinterpret_cast<const uint4*>(v_base + h * vbb) + (int64_t)(slot + r) * kLanes + l);
+            ko = ld_stream_u4(reinterpret_cast<const uint4*>(k_base + h * kbb) + (int64_t)(slot + r) * kLanes + l);
+            vo = ld_stream_u4(reinterpret_cast<const uint4*>(v_base + h * vbb) + (int64_t)(slot + r) * kLanes + l);
           }
           const int64_t o = ((int64_t)(t + r) * C.nkv + h) * kLanes + l;
           reinterpret_cast<uint4*>(k_out)[o] = ko;
@@ -321,16 +320,16 @@ __global__ void __launch_bounds__(32 * kWarps)
           const uint32_t* kg = reinterpret_cast<const uint32_t*>(kb + (int64_t)page * (HD / 2) + (slot + kr) * (2 * G));
           const uint32_t* vc = reinterpret_cast<const uint32_t*>(vb + (int64_t)(slot >> 1) * HD) + l * G;
           if constexpr (G == 4) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(kc)), e = __ldg(reinterpret_cast<const uint4*>(vc));
-            const uint2 f = __ldg(reinterpret_cast<const uint2*>(kg));
+            const uint4 a = *reinterpret_cast<const uint4*>(kc), e = *reinterpret_cast<const uint4*>(vc);
+            const uint2 f = *reinterpret_cast<const uint2*>(kg);
             kw[0] = a.x, kw[1] = a.y, kw[2] = a.z, kw[3] = a.w, vw[0] = e.x, vw[1] = e.y, vw[2] = e.z, vw[3] = e.w;
             ks[0] = f.x, ks[1] = f.y;
           } else {
-            const uint2 a = __ldg(reinterpret_cast<const uint2*>(kc)), e = __ldg(reinterpret_cast<const uint2*>(vc));
+            const uint2 a = *reinterpret_cast<const uint2*>(kc), e = *reinterpret_cast<const uint2*>(vc);
             kw[0] = a.x, kw[1] = a.y, vw[0] = e.x, vw[1] = e.y;
-            ks[0] = __ldg(kg);
+            ks[0] = *kg;
           }
-          const half2 v2 = u32_as_h2(__ldg(reinterpret_cast<const uint32_t*>(vb + (int64_t)page * (HD / 2)) + (slot >> 1)));
+          const half2 v2 = u32_as_h2(reinterpret_cast<const uint32_t*>(vb + (int64_t)page * (HD / 2))[slot >> 1]);
           vs[0] = __low2float(v2), vs[1] = __high2float(v2);
         }
         uint4* ko = reinterpret_cast<uint4*>(k_out + ((int64_t)(t + kr) * C.nkv + h) * HD);

@@ -155,7 +155,7 @@ __device__ __forceinline__ bool find_work(const PrefillParams& P, const Layout& 
     const int i = base + lane;
     int q0 = 0, lq = 0, k0 = 0, lk = 0;
     if (i < P.seqs) {
-      const int a = __ldg(P.cu_q + i), e = __ldg(P.cu_q + i + 1), c = __ldg(P.cu_k + i), f = __ldg(P.cu_k + i + 1);
+      const int a = P.cu_q[i], e = P.cu_q[i + 1], c = P.cu_k[i], f = P.cu_k[i + 1];
       q0 = max(a, 0);
       lq = max(min(e, P.tokens_q) - q0, 0);
       k0 = max(c, 0);

@@ -218,3 +218,60 @@ def test_two_threads_at_once():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_chains_without_other_kernels_between(bits, wide):
+    """Each operator's kernel may be scheduled before the one in front of it has ended: appended rows, queries, outputs and
+    lengths are what the calls before have written, eager and replayed, as when each call is waited for."""
+    B, nq, nkv, hd, page, steps = 3, 8, 2, 128, 16, 40
+    have = [30, 1, 555]
+    pools, table, _, _ = _filled([h + steps for h in have], page, nkv, hd, bits, 1, 300 if wide else 0)
+    first = [t.clone() for t in pools]
+    cos, sin = ops.precompute_rope_table(hd, 1e4, 700, DEV)
+    w = 1 + _randn(2, hd) / 8
+    starts = [_ints([h + i for h in have]) for i in range(steps)]
+    lens = [_ints([h + i + 1 for h in have]) for i in range(steps)]
+    ctx = [_cum([h + i + 1 for h in have]) for i in range(steps)]
+    totals = [sum(h + i + 1 for h in have) for i in range(steps)]
+    cu = _cum([1] * B)
+    x0 = _randn(3, B, nq, hd)
+    outs = [torch.empty_like(x0) for _ in range(2 * steps)]
+    rows = [tuple(torch.empty(totals[-1], nkv, hd, dtype=torch.float16, device=DEV) for _ in range(2)) for _ in range(2)]
+
+    def run(wait):
+        x = x0
+        for i in range(steps):
+            # the outputs of one step are the queries, keys and values of the next
+            q, _ = ops.paged_kv_append(x, x[:, :nkv], x[:, nkv : 2 * nkv], *pools, table, starts[i], cos, sin, q_norm=w, k_norm=w)
+            wait()
+            ops.paged_decode_attention(q, *pools, table, lens[i], out=outs[2 * i])
+            wait()
+            k, v = (t[: totals[i]] for t in rows[i % 2])
+            ops.paged_kv_read(*pools, table, ctx[i], totals[i], out=(k, v))
+            wait()
+            x = ops.prefill_attention(q, k, v, cu, cu_seqlens_k=ctx[i], out=outs[2 * i + 1])
+            wait()
+
+    def reset():
+        for t, f in zip(pools, first):
+            t.copy_(f)
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+
+    reset()
+    run(torch.cuda.synchronize)
+    want, held = [o.clone() for o in outs], [t.clone() for t in pools]
+    assert all(o.isfinite().all() and o.abs().sum() > 0 for o in want)
+    graph = torch.cuda.CUDAGraph()
+    reset()
+    with torch.cuda.graph(graph):
+        run(lambda: None)
+    for again in (lambda: run(lambda: None), graph.replay) * 4:
+        reset()
+        again()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pools, held))
