@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import soinfer.ops as ops
+from soinfer import _C
 from tests import paged_oracle as oracle
 
 pytestmark = pytest.mark.gpu
@@ -275,3 +276,47 @@ def test_chains_without_other_kernels_between(bits, wide):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pools, held))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_position_advanced_in_the_chain(bits):
+    """A decode loop whose position and length the framework's own step kernel advances, nothing else between."""
+    nq, nkv, hd, page, have, steps = 8, 2, 64, 16, 14, 120
+    pools, table, _, _ = _filled([have + steps + 1], page, nkv, hd, bits, 1)
+    first = [t.clone() for t in pools]
+    cos, sin = ops.precompute_rope_table(hd, 1e4, 200, DEV)
+    start, length, zero = _ints([have]), _ints([have + 1]), _ints([0])
+    ids = torch.zeros(500, dtype=torch.int32, device=DEV)
+    x0 = _randn(2, 1, nq, hd)
+    outs = [torch.empty_like(x0) for _ in range(steps)]
+
+    def run(wait):
+        x = x0
+        for out in outs:
+            q, _ = ops.paged_kv_append(x, x[:, :nkv], x[:, nkv : 2 * nkv], *pools, table, start, cos, sin)
+            wait()
+            x = ops.paged_decode_attention(q, *pools, table, length, out=out)
+            wait()
+            for t in (start, length):
+                _C.decode_step_advance(ids, t, zero, zero)
+                wait()
+
+    def reset():
+        for t, f in zip((*pools, start, length), (*first, _ints([have]), _ints([have + 1]))):
+            t.copy_(f)
+        torch.cuda.synchronize()
+
+    reset()
+    run(torch.cuda.synchronize)
+    assert start.item() == have + steps and length.item() == have + steps + 1
+    want = [o.clone() for o in outs]
+    assert not torch.equal(want[-1], want[-2])
+    graph = torch.cuda.CUDAGraph()
+    reset()
+    with torch.cuda.graph(graph):
+        run(lambda: None)
+    for again in (lambda: run(lambda: None), graph.replay) * 4:
+        reset()
+        again()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
