@@ -18,7 +18,8 @@
 // Work split.  A sequence's kv head with up to 8 of its query heads is a unit.
 //   Few units (cluster_units) over tables that name few positions (kClusterMost): a unit is one cluster of eight CTAs, each
 //   an eighth of the positions; they join through distributed shared memory.  One launch, no workspace: 777 4-bit positions of
-//   8 kv heads 5.0 us against 7.8 by ranges; 8 unequal sequences of up to 4096 fp16 positions, 4 kv heads, 11.3 against 12.9.
+//   8 kv heads 5.2 us against 7.3 by ranges; 8 unequal sequences of up to 4096 fp16 positions, 4 kv heads, 12.5 against 14.0.
+//   What a table can name decides, not the lengths, which the host does not know: short sequences under wide tables go by ranges.
 //   Beyond, a cluster's idle CTAs and the eight-fold start cost more than they bring (64 unequal sequences of up to 4000 4-bit
 //   positions 91 us against 56, 256 of 500 252 against 58; one of 8000 fp16 positions 14.3 against 11.3, 4-bit 11.0 against
 //   11.3).
@@ -33,12 +34,12 @@
 // Feeding: each warp has its own ring of tiles in shared memory, filled by 16-byte asynchronous copies, so loads run ahead and
 // the registers hold only what is being multiplied.  The pieces' places are exchanged within 128 bytes by row, since rows
 // that lie end to end put the lanes of a load on the same banks (fp16, 8 sequences of up to 4096, 4 kv heads: bulk copies
-// without exchange 15.5 us, a bulk copy per padded row 18.2, this 12.3).
+// without exchange 15.5 us, a bulk copy per padded row 18.2, this 12.3, all at an earlier state of the kernel).
 //
-// Measured (GPU time): 4 bits, two sequences of 131072 and 100003, 40 / 8 heads: 61 us for 255 MB = 4.2 TB/s (0.64 of the
+// Measured (GPU time): 4 bits, two sequences of 131072 and 100003, 40 / 8 heads: 62 us for 255 MB = 4.1 TB/s (0.63 of the
 // measured copy rate), bound by issuing 303 instructions per 16 positions and kv head (integer pipe 47%, fp16 / fp32 pipe
 // 25%, tensor pipe 25% busy); register tiles without a ring 96 us, 32-position tiles 81.  One sequence of 777
-// positions: 5.0 us in one launch, against 8.7 with a second kernel that joins.
+// positions: 5.2 us in one launch (an earlier form with a second kernel that joins: 8.7).
 #include <algorithm>
 
 #include "launch.cuh"

@@ -1,9 +1,10 @@
 // Appending rotated keys and values to a paged cache, and reading cached rows back.
 //
 // Both move rows of hd fp16 values once: what bounds them is memory (a prompt) or the launch (one token).
-// Measured (GPU time): 8675 tokens of 40 / 8 heads of 128 into fp16 pages 50 us for 266 MB (0.83 of the measured copy rate);
-// one token 2.4 us; 65431 4-bit positions of 8 heads read back 60 us for 340 MB (0.87); 3759 tokens of 16 / 8 heads into 4
-// bits 20 us (the code choice's arithmetic and the look-ups' latency: 58 MB alone would take 9).
+// Measured (GPU time): 8675 tokens of 40 / 8 heads of 128 into fp16 pages 50 us for 266 MB (0.82 of the measured copy rate);
+// one token 2.3 us; 65431 4-bit positions of 8 heads read back 61 us for 340 MB (0.86); 3759 tokens of 16 / 8 heads into 4
+// bits 20 us, where 58 MB alone would take 9: 0.53 instructions per cycle and scheduler from the 3.9 warps that 96 registers a
+// thread leave, DRAM 17% busy -- latency that few warps leave open -- and 2.5 waves of CTAs.
 #include "launch.cuh"
 #include "paged_cache.cuh"
 

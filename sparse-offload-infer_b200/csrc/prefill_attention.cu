@@ -29,13 +29,13 @@
 //
 // The grid holds one CTA per pair of tiles and kv head, an upper bound from the token counts (row bounds are read on the
 // device).  Where the GPU holds two, four or eight times as many CTAs and the contexts are long, a cluster of as many
-// shares a pair's keys and joins its sums through distributed shared memory: 32 / 8 heads, 512 tokens over 8000 107 -> 69 us
-// and over 30000 382 -> 228, 128 over 32000 383 -> 116, four times 5 over 16000 182 -> 56, 64 over 1000 20.0 -> 19.8.
+// shares a pair's keys and joins its sums through distributed shared memory: 32 / 8 heads, 512 tokens over 8000 107 -> 71 us
+// and over 30000 382 -> 229, 128 over 32000 383 -> 115, four times 5 over 16000 182 -> 57, 64 over 1000 20.0 -> 19.8.
 //
 // Measured (8192 tokens, 40 / 8 heads, hd 128): products issued from a single lane's branch 832 us, maxima over eight chains
-// and packed pairs 685, products issued by a convergent warp 600, registers / halves / fp32 pipe / coalesced output 555 =
-// 1238 TFLOP/s, 0.77 of the measured burst rate of a library product and 0.90 of its sustained one, whose power limit this
-// kernel reaches too.  7 unequal prompts (3828 tokens, 16 / 8 heads): 29 us, the longest one's 12 steps of 1.6 us plus 6 us
+// and packed pairs 685, products issued by a convergent warp 600, registers / halves / fp32 pipe / coalesced output 555 in
+// short runs = 1238 TFLOP/s, 0.77 of the measured burst rate of a library product; called back to back, at the power limit, 640
+// to 652 = 1054 to 1075 TFLOP/s, 0.77 of its sustained rate.  7 unequal prompts (3828 tokens, 16 / 8 heads): 29 us, the longest one's 12 steps of 1.6 us plus 6 us
 // of start and end and a second round of CTAs.  One in eight / three in eight / half of the pairs on the fp32 pipe: 31.6 /
 // 31.7 / 32.3 us against 31.2 there.  hd 64, two chunks of 512 and 1000 rows over 4012 and 3047 keys, 32 / 4 heads: 68 us,
 // 192 CTAs in two rounds; P beside S in the tensor memory, so that scores run ahead, measured the same (the two warps of a
