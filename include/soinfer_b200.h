@@ -580,7 +580,7 @@ int soinfer_paged_kv_read(const soinfer_paged_cache* cache, const int32_t* cu_se
  * table_cols * page_size; read on the device), grouped heads, scale
  * 1/sqrt(head_dim), fp32 softmax and sums: out [num_seqs, num_q_heads,
  * head_dim].  Positions without a page are skipped; a sequence without
- * positions gives zeros.  num_seqs <= 32768.  The workspace holds partial
+ * positions gives zeros, one whose scores are all -inf NaN.  num_seqs <= 32768.  The workspace holds partial
  * results; its size (0: none needed, workspace may be NULL) follows from the
  * sequences, the heads and max_positions = table_cols * page_size. */
 int64_t soinfer_paged_decode_workspace_bytes(int64_t num_seqs, int64_t num_q_heads, int64_t num_kv_heads,

@@ -35,11 +35,11 @@
 // Measured (8192 tokens, 40 / 8 heads, hd 128): products issued from a single lane's branch 832 us, maxima over eight chains
 // and packed pairs 685, products issued by a convergent warp 600, registers / halves / fp32 pipe / coalesced output 555 in
 // short runs = 1238 TFLOP/s, 0.77 of the measured burst rate of a library product; called back to back, at the power limit, 640
-// to 652 = 1054 to 1075 TFLOP/s, 0.77 of its sustained rate.  7 unequal prompts (3828 tokens, 16 / 8 heads): 29 us, the longest one's 12 steps of 1.6 us plus 6 us
-// of start and end and a second round of CTAs.  One in eight / three in eight / half of the pairs on the fp32 pipe: 31.6 /
-// 31.7 / 32.3 us against 31.2 there.  hd 64, two chunks of 512 and 1000 rows over 4012 and 3047 keys, 32 / 4 heads: 68 us,
-// 192 CTAs in two rounds; P beside S in the tensor memory, so that scores run ahead, measured the same (the two warps of a
-// scheduler spend their exponentials' phases together).
+// to 652 = 1054 to 1075 TFLOP/s, 0.77 of its sustained rate.  7 unequal prompts (3828 tokens, 16 / 8 heads): 29 us, the longest
+// one's 12 steps of 1.6 us plus 6 us of start and end and a second round of CTAs.  One in eight / three in eight / half of the
+// pairs on the fp32 pipe: 31.6 / 31.7 / 32.3 us against 31.2 there.  hd 64, two chunks of 512 and 1000 rows over 4012 and 3047
+// keys, 32 / 4 heads: 68 us, 192 CTAs in two rounds; P beside S in the tensor memory, so that scores run ahead, measured the
+// same (the two warps of a scheduler spend their exponentials' phases together).
 #include <cuda.h>
 
 #include <type_traits>
